@@ -209,6 +209,26 @@ SD3_API int sd3_layernorm_modulate(const float* x, int B, int T, int E, float ep
                            const float* scale2, void* out2, long mod_stride, int out_dtype,
                            void* stream);
 
+/* Layer norm with weight and bias: y = (x - mean) * rstd * w + b over the C columns of every row, with the statistics
+ * that its gradient needs.  x (rows, C) of dtype, rows ldx >= C elements apart (ldx 0: one row for all); y (rows, C)
+ * of the same dtype, contiguous; w and b (C) f32, NULL for 1 and 0; mean and rstd = 1 / sqrt(var + eps) (rows) f32,
+ * either may be NULL.  y may be x where ldx == C.  rows may be 0.
+ * Replaces LayerNorm_forward with save_for_backward (modules.cpp:51-86). */
+SD3_API int sd3_layer_norm(const void* x, long ldx, int dtype, const float* w, const float* b, float eps, void* y,
+                           float* mean, float* rstd, long rows, int C, void* stream);
+
+/* Gradient of sd3_layer_norm for dy (rows, C) of dtype, rows lddy elements apart: dx (rows, C) of dtype, contiguous,
+ * dw = sum over rows of dy * (x - mean) * rstd and db = sum over rows of dy, (C) f32 each, written (not added to);
+ * dw or db may be NULL.  x, ldx, w, mean and rstd as given to and left by the forward.  dx may be dy or x where those
+ * are contiguous.  The sums are formed in a fixed order: the same bits on every call.  scratch: device memory of at
+ * least sd3_layer_norm_backward_scratch_bytes(rows, C) bytes on the current device, 4-byte aligned, used by this call
+ * alone until it is complete.  rows may be 0: dw = db = 0.
+ * Replaces LayerNorm_backward (modules.cpp:87-152). */
+SD3_API long sd3_layer_norm_backward_scratch_bytes(long rows, int C);
+SD3_API int sd3_layer_norm_backward(const void* dy, long lddy, const void* x, long ldx, int dtype, const float* w,
+                                    const float* mean, const float* rstd, void* dx, float* dw, float* db, long rows,
+                                    int C, void* scratch, long scratch_bytes, void* stream);
+
 /* out[b, n] = act(sum_k in[b,k] w[n,k] + bias[n] + add[b,n]) for a handful of
  * rows (the conditioning MLPs and every block's AdaLN projection in one
  * launch).  in/out/add f32, w (N,K) of w_dtype, act: 0 none, 1 SiLU.

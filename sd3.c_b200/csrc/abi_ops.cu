@@ -328,6 +328,40 @@ int sd3_layernorm_modulate(const float* x, int B, int T, int E, float eps, const
   return launch_ln_modulate(p, nullptr, E, eps, mod_stride, out_dtype == SD3_DTYPE_F32, S(stream));
 }
 
+int sd3_layer_norm(const void* x, long ldx, int dtype, const float* w, const float* b, float eps, void* y, float* mean,
+                   float* rstd, long rows, int C, void* stream) {
+  if (!dtype_ok(dtype) || rows < 0 || C <= 0 || C > (1 << 24) || (ldx < C && ldx != 0) || !(eps >= 0.f) ||
+      (rows > 0 && (!x || !y)) || (y == x && ldx != C)) {
+    set_last_error("sd3_layer_norm: invalid argument (dtype %d rows %ld C %d ldx %ld)", dtype, rows, C, ldx);
+    return SD3_ERR_INVALID_ARG;
+  }
+  if (rows == 0) return SD3_OK;
+  return launch_layer_norm(x, ldx, dtype == SD3_DTYPE_F32, w, b, eps, y, mean, rstd, rows, C, S(stream));
+}
+
+long sd3_layer_norm_backward_scratch_bytes(long rows, int C) {
+  return static_cast<long>(layer_norm_backward_scratch_bytes(rows, C));
+}
+
+int sd3_layer_norm_backward(const void* dy, long lddy, const void* x, long ldx, int dtype, const float* w,
+                            const float* mean, const float* rstd, void* dx, float* dw, float* db, long rows, int C,
+                            void* scratch, long scratch_bytes, void* stream) {
+  if (!dtype_ok(dtype) || rows < 0 || C <= 0 || C > (1 << 24) || (ldx < C && ldx != 0) || (lddy < C && lddy != 0) ||
+      (rows > 0 && (!dy || !x || !mean || !rstd || !dx)) || (dx == x && ldx != C) || (dx == dy && lddy != C)) {
+    set_last_error("sd3_layer_norm_backward: invalid argument (dtype %d rows %ld C %d ldx %ld lddy %ld)", dtype, rows, C,
+                   ldx, lddy);
+    return SD3_ERR_INVALID_ARG;
+  }
+  if (rows > 0 && (!scratch || (reinterpret_cast<uintptr_t>(scratch) & 3) ||
+                   scratch_bytes < sd3_layer_norm_backward_scratch_bytes(rows, C))) {
+    set_last_error("sd3_layer_norm_backward: %ld bytes of scratch needed, got %ld",
+                   sd3_layer_norm_backward_scratch_bytes(rows, C), scratch ? scratch_bytes : 0L);
+    return SD3_ERR_INVALID_ARG;
+  }
+  return launch_layer_norm_backward(dy, lddy, x, ldx, dtype == SD3_DTYPE_F32, w, mean, rstd, dx, dw, db, rows, C,
+                                    static_cast<float*>(scratch), S(stream));
+}
+
 int sd3_skinny_linear(const float* in, long ld_in, const void* w, int w_dtype, const float* bias,
                       const float* add, long ld_add, float* out, long ld_out, int B, int N, int K,
                       int act, void* stream) {

@@ -211,6 +211,16 @@ struct LnProblem {
 int launch_ln_modulate(const LnProblem& a, const LnProblem* b, int E, float eps, long mod_stride, int out_f32,
                        cudaStream_t stream);
 
+// Layer norm with weight and bias (w, b: fp32 or null), x (rows, C) of fp32 or bf16 with rows ldx elements apart, y (rows, C) of
+// the same type; mean and rstd: (rows) fp32 or null.  Backward: dx (rows, C) of x's type, dw and db (C) fp32, either may
+// be null; scratch: layer_norm_backward_scratch_bytes(rows, C) bytes.
+int launch_layer_norm(const void* x, long ldx, int f32, const float* w, const float* b, float eps, void* y, float* mean,
+                      float* rstd, long rows, int C, cudaStream_t stream);
+size_t layer_norm_backward_scratch_bytes(long rows, int C);
+int launch_layer_norm_backward(const void* dy, long lddy, const void* x, long ldx, int f32, const float* w,
+                               const float* mean, const float* rstd, void* dx, float* dw, float* db, long rows, int C,
+                               float* scratch, cudaStream_t stream);
+
 // Skinny linear for M = B <= 64 rows:  out[b, n] = act_out(sum_k in[b,k] W[n,k] + bias[n] + add[b,n])
 // W is (N, K) row-major, bf16 or fp32 (w_f32).  act: 0 none, 1 SiLU.  w_static: no kernel that may
 // still be running when this one is launched writes W.

@@ -32,8 +32,10 @@ namespace {
 using torch::Tensor;
 typedef std::unordered_map<std::string, Tensor> ParamDict;
 
+// Numbers go into messages through std::to_string: a number streamed into an std::ostream by an extension that was built
+// with another libstdc++ than torch's ends the process with a segmentation fault.
 void ok(int rc, const char* what) {
-  TORCH_CHECK(rc == 0, what, " failed (", rc, "): ", sd3_last_error());
+  TORCH_CHECK(rc == 0, what, " failed (", std::to_string(rc), "): ", sd3_last_error());
 }
 
 void* stream() { return static_cast<void*>(at::cuda::getCurrentCUDAStream().stream()); }
@@ -258,10 +260,43 @@ Tensor MLP(Tensor& x, Tensor& W1, Tensor& b1, Tensor& W2, Tensor& b2, std::strin
   return linear_impl(h, W2, b2, SD3_ACT_NONE);
 }
 
-// layer_norm(x (B,T,C), w, b, eps, save_for_backward) -> [out]
+// A tensor as rows of its last dimension: 2-D tensors keep their row stride (slices of wider rows, one row for all),
+// others are made contiguous.
+struct Rows {
+  Tensor t;
+  int64_t rows, C, ld;
+};
+Rows rows_of(const Tensor& t, const char* name) {
+  TORCH_CHECK(t.is_cuda(), "custom_modules: '", name, "' must be a CUDA tensor (this build has no CPU path)");
+  TORCH_CHECK(t.dim() >= 1 && t.size(-1) > 0, name, ": rows of at least one value expected");
+  const int64_t C = t.size(-1), rows = t.numel() / C;
+  if (t.dim() == 2 && t.stride(1) == 1 && rows > 1 && (t.stride(0) >= C || t.stride(0) == 0)) return {t, rows, C, t.stride(0)};
+  return {t.contiguous(), rows, C, C};
+}
+
+// a vector of n fp32 values next to x
+Tensor vector_f32(const Tensor& v, int64_t n, const Tensor& x, const char* name) {
+  TORCH_CHECK(v.is_cuda() && v.device() == x.device() && v.numel() == n, name, ": ", std::to_string(n),
+              " values on ", x.device().str(), " expected");
+  return v.to(torch::kFloat32).contiguous();
+}
+
+// layer_norm(x (..., C), w, b, eps, save_for_backward) -> [out], or [out, mean, rstd] with the statistics (one per row,
+// fp32) that layer_norm_backward takes
 std::vector<Tensor> LayerNorm_forward(Tensor& x_in, Tensor& w, Tensor& b, float eps,
                                       bool save_for_backward) {
-  TORCH_CHECK(!save_for_backward, "layer_norm: forward only (no statistics are saved)");
+  if (save_for_backward) {
+    Rows x = rows_of(x_in, "x");
+    c10::cuda::CUDAGuard guard(x.t.device());
+    Tensor wf = vector_f32(w, x.C, x.t, "w"), bf = vector_f32(b, x.C, x.t, "b");
+    Tensor out = torch::empty(x_in.sizes(), x_in.options());
+    Tensor stats = torch::empty({2, x.rows}, wf.options());
+    float* mean = stats.data_ptr<float>();
+    ok(sd3_layer_norm(x.t.data_ptr(), x.ld, tag(x.t), wf.data_ptr<float>(), bf.data_ptr<float>(), eps, out.data_ptr(),
+                      mean, mean + x.rows, x.rows, (int)x.C, stream()),
+       "sd3_layer_norm");
+    return {out, stats[0], stats[1]};
+  }
   Tensor x = dev(x_in, "x");
   c10::cuda::CUDAGuard guard(x.device());
   const int64_t C = x.size(-1), rows = x.numel() / C;
@@ -275,6 +310,26 @@ std::vector<Tensor> LayerNorm_forward(Tensor& x_in, Tensor& w, Tensor& b, float 
                             tag(out), stream()),
      "sd3_layernorm_modulate");
   return {out};
+}
+
+// layer_norm_backward(dout (..., C), x (..., C), w, mean, rstd) -> [dx, dw, db]; dx of x's type, dw and db fp32
+std::vector<Tensor> LayerNorm_backward(Tensor& dout, Tensor& x_in, Tensor& w, Tensor& mean, Tensor& rstd) {
+  Rows x = rows_of(x_in, "x");
+  Rows dy = rows_of(dout, "dout");
+  c10::cuda::CUDAGuard guard(x.t.device());
+  TORCH_CHECK(dy.t.device() == x.t.device() && dy.t.scalar_type() == x.t.scalar_type() && dy.rows == x.rows && dy.C == x.C,
+              "layer_norm_backward: dout and x must have one shape, type and device");
+  Tensor wf = vector_f32(w, x.C, x.t, "w"), mf = vector_f32(mean, x.rows, x.t, "mean");
+  Tensor rf = vector_f32(rstd, x.rows, x.t, "rstd");
+  Tensor dx = torch::empty(x_in.sizes(), x_in.options());
+  const long bytes = sd3_layer_norm_backward_scratch_bytes(x.rows, (int)x.C);
+  Tensor dw = torch::empty({x.C}, wf.options()), db = torch::empty({x.C}, wf.options());
+  Tensor scratch = torch::empty({bytes / 4}, wf.options());
+  ok(sd3_layer_norm_backward(dy.t.data_ptr(), dy.ld, x.t.data_ptr(), x.ld, tag(x.t), wf.data_ptr<float>(),
+                             mf.data_ptr<float>(), rf.data_ptr<float>(), dx.data_ptr(), dw.data_ptr<float>(),
+                             db.data_ptr<float>(), x.rows, (int)x.C, scratch.data_ptr(), bytes, stream()),
+     "sd3_layer_norm_backward");
+  return {dx, dw, db};
 }
 
 // rms_norm(x (..., C), w (C,), eps, save_for_backward) -> [out]
@@ -381,6 +436,7 @@ Tensor mha(Tensor& Q, Tensor& K, Tensor& V, int num_heads) {
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("layer_norm", &LayerNorm_forward, "LayerNorm forward");
+  m.def("layer_norm_backward", &LayerNorm_backward, "LayerNorm backward: gradients of x, weight and bias");
   m.def("rms_norm", &RMSNorm_forward, "RMSNorm forward");
   m.def("linear", &Linear_forward, "Linear forward");
   m.def("conv2d", &conv2d_forward, "Conv2d forward (patch embedding form)");

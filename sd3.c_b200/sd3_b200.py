@@ -73,6 +73,9 @@ PROTOTYPES = {
     "sd3_cross_attention": (c_int, [c_void_p, c_void_p, c_void_p, c_long, c_long, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p, c_long, c_int, c_float, c_void_p]),
     "sd3_conv2d": (c_int, [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p]),
     "sd3_layernorm_modulate": (c_int, [c_void_p, c_int, c_int, c_int, c_float, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_long, c_int, c_void_p]),
+    "sd3_layer_norm": (c_int, [c_void_p, c_long, c_int, c_void_p, c_void_p, c_float, c_void_p, c_void_p, c_void_p, c_long, c_int, c_void_p]),
+    "sd3_layer_norm_backward_scratch_bytes": (c_long, [c_long, c_int]),
+    "sd3_layer_norm_backward": (c_int, [c_void_p, c_long, c_void_p, c_long, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_long, c_int, c_void_p, c_long, c_void_p]),
     "sd3_skinny_linear": (c_int, [c_void_p, c_long, c_void_p, c_int, c_void_p, c_void_p, c_long, c_void_p, c_long, c_int, c_int, c_int, c_int, c_void_p]),
     "sd3_sinusoidal_embedding": (c_int, [c_void_p, c_void_p, c_int, c_int, c_void_p]),
     "sd3_pos_embed_table": (c_int, [c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p]),
@@ -292,6 +295,61 @@ def layernorm_modulate(x, B, T, E, eps, shift1, scale1, shift2=None, scale2=None
                                        ptr(out2), ms, dtype_tag(out1), stream_ptr()),
           "sd3_layernorm_modulate")
     return out1, out2
+
+
+def _rows(t, what, like=None):
+    """(rows, C, row stride) of a 2-D tensor whose rows are contiguous, and checks it against `like`."""
+    if t.dim() != 2 or not t.is_cuda or t.shape[1] < 1:
+        raise Sd3Error("%s: 2-D CUDA tensor expected" % what)
+    rows, C = t.shape
+    if C > 1 and t.stride(1) != 1:
+        raise Sd3Error("%s: rows must be contiguous" % what)
+    if like is not None and (t.shape != like.shape or t.dtype != like.dtype or t.device != like.device):
+        raise Sd3Error("%s: %s of %s on %s expected" % (what, tuple(like.shape), like.dtype, like.device))
+    return rows, C, t.stride(0) if rows > 1 else C
+
+
+def _vector(t, n, device, what):
+    if t is None:
+        return None
+    if t.dtype != _torch().float32 or t.numel() != n or t.device != device or not t.is_contiguous():
+        raise Sd3Error("%s: contiguous float32 tensor of %d values on %s expected" % (what, n, device))
+    return ptr(t)
+
+
+def layer_norm(x, w=None, b=None, eps=1e-5):
+    """Layer norm of the rows of x (rows, C), float32 or bfloat16, with float32 weight and bias (None: 1 and 0).
+    Returns (y, mean, rstd): y of x's type, the statistics of each row in float32 for layer_norm_backward."""
+    torch = _torch()
+    rows, C, ld = _rows(x, "layer_norm: x")
+    y = torch.empty((rows, C), device=x.device, dtype=x.dtype)
+    mean = torch.empty(rows, device=x.device, dtype=torch.float32)
+    rstd = torch.empty_like(mean)
+    with torch.cuda.device(x.device):
+        check(lib().sd3_layer_norm(c_void_p(x.data_ptr()), ld, dtype_tag(x), _vector(w, C, x.device, "layer_norm: w"),
+                                   _vector(b, C, x.device, "layer_norm: b"), eps, ptr(y), ptr(mean), ptr(rstd), rows, C,
+                                   stream_ptr()), "sd3_layer_norm")
+    return y, mean, rstd
+
+
+def layer_norm_backward(dy, x, w, mean, rstd):
+    """Gradient of layer_norm: (dx, dw, db), dx of x's type, dw and db float32 (the same bits on every call)."""
+    torch = _torch()
+    rows, C, ld = _rows(x, "layer_norm_backward: x")
+    lddy = _rows(dy, "layer_norm_backward: dy", x)[2]
+    dx = torch.empty((rows, C), device=x.device, dtype=x.dtype)
+    dw = torch.empty(C, device=x.device, dtype=torch.float32)
+    db = torch.empty_like(dw)
+    with torch.cuda.device(x.device):
+        nbytes = lib().sd3_layer_norm_backward_scratch_bytes(rows, C)
+        scratch = torch.empty(nbytes, device=x.device, dtype=torch.uint8)
+        check(lib().sd3_layer_norm_backward(c_void_p(dy.data_ptr()), lddy, c_void_p(x.data_ptr()), ld, dtype_tag(x),
+                                            _vector(w, C, x.device, "layer_norm_backward: w"),
+                                            _vector(mean, rows, x.device, "layer_norm_backward: mean"),
+                                            _vector(rstd, rows, x.device, "layer_norm_backward: rstd"), ptr(dx), ptr(dw),
+                                            ptr(db), rows, C, ptr(scratch), nbytes, stream_ptr()),
+              "sd3_layer_norm_backward")
+    return dx, dw, db
 
 
 def skinny_linear(inp, w_nk, bias=None, add=None, act=0):
