@@ -93,6 +93,37 @@ int sd3_linear(const void* x, const void* w, const float* bias, void* out, int o
   return launch_gemm(x, K, w, K, OPERAND_BF16, M, N, K, e, device_status_word(), S(stream));
 }
 
+int sd3_linear_residual(const void* x, long ldx, const void* w, long ldw, const float* bias, int act, const void* residual,
+                        long ld_residual, void* out, long ldo, int dtype, int M, int N, int K, void* stream) {
+  if (!dtype_ok(dtype) || act < SD3_ACT_NONE || act > SD3_ACT_RELU || M < 0 || N <= 0 || K <= 0) {
+    set_last_error("sd3_linear_residual: bad dtype %d, act %d or size (M %d N %d K %d)", dtype, act, M, N, K);
+    return SD3_ERR_INVALID_ARG;
+  }
+  if (M == 0) return SD3_OK;
+  const uintptr_t esz = dtype == SD3_DTYPE_F32 ? 4 : 2;
+  if (!x || !w || !out || ldx < K || ldw < K || ldo < N || (residual && ld_residual < N) ||
+      (reinterpret_cast<uintptr_t>(bias) & 3) || reinterpret_cast<uintptr_t>(out) % esz ||
+      reinterpret_cast<uintptr_t>(residual) % esz || (residual == out && ld_residual != ldo)) {
+    set_last_error("sd3_linear_residual: null or misaligned pointer, or rows that overlap (ldx %ld ldw %ld ldo %ld)", ldx, ldw, ldo);
+    return SD3_ERR_INVALID_ARG;
+  }
+  if (ldx % 8 || ldw % 8 || (reinterpret_cast<uintptr_t>(x) & 15) || (reinterpret_cast<uintptr_t>(w) & 15)) {
+    set_last_error("sd3_linear_residual: the rows of x and w must be 16-byte aligned (ldx %ld ldw %ld)", ldx, ldw);
+    return SD3_ERR_UNSUPPORTED;
+  }
+  GemmEpilogue e;
+  e.mode = EPI_ACT_RESID;
+  e.bias = bias;
+  e.act = act;
+  e.add = residual;
+  e.ld_add = ld_residual;
+  e.out = out;
+  e.out_f32 = dtype == SD3_DTYPE_F32;
+  e.ldo = ldo;
+  return launch_linear_residual(static_cast<const bf16*>(x), ldx, static_cast<const bf16*>(w), ldw, M, N, K, e,
+                                status_word_for(S(stream)), S(stream));
+}
+
 int sd3_linear_e4m3(const void* x, const void* w, const float* bias, void* out, int out_dtype, int M,
                     int N, int K, float scale, int act, void* stream) {
   if (!dtype_ok(out_dtype) || (act != SD3_ACT_NONE && act != SD3_ACT_GELU_TANH)) {

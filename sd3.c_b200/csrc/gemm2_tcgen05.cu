@@ -58,20 +58,24 @@ __host__ __device__ constexpr int pair_stage_bytes(int pbn) { return P_A_BYTES +
 // epilogue warp.
 constexpr int P_RED_BYTES = 4096;
 __host__ __device__ constexpr bool pair_stages_out(int epi, bool out_f32) {
-  return epi == EPI_GATE_RESID || (!out_f32 && (epi == EPI_BIAS || epi == EPI_BIAS_GELU || epi == EPI_QKV_NORM));
+  return epi == EPI_GATE_RESID || epi == EPI_ACT_RESID || (!out_f32 && (epi == EPI_BIAS || epi == EPI_BIAS_GELU || epi == EPI_QKV_NORM));
 }
 // Six stages of 32 KiB (eight of 24 KiB), handed over in slots of one (two): a full and an empty barrier, one
 // wait and one commit each.  A stage of the wide tile is 512 cycles of MMA and single hand-overs refill the
 // ring sooner (N = 1536, K = 6144, 4429 rows: 69.1 us against 70.9 with slots of two; 13287 rows: 191 against 207);
 // one of the narrow tile is 256 cycles, less than a hand-over takes (589 rows: 24.6 us, with slots of two 20.4).
-__host__ __device__ constexpr int pair_stages(int pbn) { return pbn == 256 ? 6 : 8; }
+// EPI_ACT_RESID has two 4 KiB boxes per epilogue warp, which cost it a stage (two).
+__host__ __device__ constexpr int pair_stages(int pbn, int epi) {
+  return epi == EPI_ACT_RESID ? (pbn == 256 ? 5 : 6) : pbn == 256 ? 6 : 8;
+}
 __host__ __device__ constexpr int pair_slot(int pbn) { return pbn == 256 ? 1 : 2; }
 __host__ __device__ constexpr int pair_red_bytes(int epi, bool out_f32) {
-  return pair_stages_out(epi, out_f32) ? EPI_WARPS * P_RED_BYTES : 0;
+  return pair_stages_out(epi, out_f32) ? EPI_WARPS * P_RED_BYTES * (epi == EPI_ACT_RESID ? 2 : 1) : 0;
 }
 constexpr int P_THREADS = 64 + 32 * EPI_WARPS;
 __host__ __device__ constexpr int pair_smem_bytes(int epi, bool out_f32, int pbn) {
-  return pair_stages(pbn) * pair_stage_bytes(pbn) + pair_red_bytes(epi, out_f32) + 256 + 1024;
+  return pair_stages(pbn, epi) * pair_stage_bytes(pbn) + pair_red_bytes(epi, out_f32) +
+         (epi == EPI_ACT_RESID ? 512 : 256) + 1024;
 }
 
 // One problem of a (possibly grouped) launch
@@ -94,7 +98,7 @@ gemm_pair_tcgen05_kernel(const __grid_constant__ PairProblem p0, const __grid_co
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
-  constexpr int P_STAGES = pair_stages(PBN);
+  constexpr int P_STAGES = pair_stages(PBN, EPI);
   static_assert(EPI_WARPS * ((PBN + 63) / 64) * P_RED_BYTES <= P_STAGES * P_STAGE_BYTES, "the last tile's boxes fit the ring");
   uint8_t* red_smem = smem + P_STAGES * P_STAGE_BYTES;  // 1024-byte aligned: stages are 32 / 24 / 20 KiB each
   uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + P_STAGES * P_STAGE_BYTES + pair_red_bytes(EPI, OUT_F32));
@@ -103,6 +107,7 @@ gemm_pair_tcgen05_kernel(const __grid_constant__ PairProblem p0, const __grid_co
   uint64_t* tempty_bar = tfull_bar + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty_bar + 2);
   int* s_abort = reinterpret_cast<int*>(tmem_slot + 1);
+  uint64_t* add_bar = reinterpret_cast<uint64_t*>(tmem_slot + 2);  // EPI_ACT_RESID: two per epilogue warp
 
   const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0);  // known uniform
   const int lane = threadIdx.x & 31;
@@ -122,6 +127,8 @@ gemm_pair_tcgen05_kernel(const __grid_constant__ PairProblem p0, const __grid_co
       mbar_init(&tfull_bar[a], 1);
       mbar_init(&tempty_bar[a], 2 * EPI_WARPS);  // epilogue warps of both CTAs (leader's copy is used)
     }
+    if constexpr (EPI == EPI_ACT_RESID)
+      for (int i = 0; i < 2 * EPI_WARPS; ++i) mbar_init(&add_bar[i], 1);
     *s_abort = 0;
     fence_barrier_init();
     prefetch_tmap(&p0.tmA);
@@ -252,6 +259,11 @@ gemm_pair_tcgen05_kernel(const __grid_constant__ PairProblem p0, const __grid_co
     const int row = quad * 32 + lane;
     int acc = 0;
     uint32_t acc_phase = 0;
+    // EPI_ACT_RESID is a launch of one problem; its rows to add are described by p1.tmR
+    ActResidBoxes<PBN, OUT_F32> boxes;
+    if constexpr (EPI == EPI_ACT_RESID)
+      boxes.init(&p0.tmR, &p1.tmR, p0.g, red_smem + (warp - 2) * 2 * P_RED_BYTES, add_bar + 2 * (warp - 2), quad, half,
+                 static_cast<int>(rank), pair, num_pairs);
     for (int tile = pair; tile < num_tiles; tile = tiles.next(tile, num_pairs)) {
       const PairProblem& pp = tile < end0 ? p0 : tile < end1 ? p1 : p2;
       const GemmArgs& g = pp.g;
@@ -271,7 +283,9 @@ gemm_pair_tcgen05_kernel(const __grid_constant__ PairProblem p0, const __grid_co
       constexpr int BOXES = PBN / 2 / (EPI == EPI_GATE_RESID ? 32 : 64);  // of a warp and tile
       uint8_t* box = last ? smem + (warp - 2) * (BOXES * P_RED_BYTES) : red_smem + (warp - 2) * P_RED_BYTES;
       const int box_step = last ? P_RED_BYTES : 0;
-      if constexpr (EPI == EPI_GATE_RESID)
+      if constexpr (EPI == EPI_ACT_RESID)
+        drained = boxes.drain(t_row, m0 + quad * 32, n0, &tfull_bar[acc], acc_phase, wc);
+      else if constexpr (EPI == EPI_GATE_RESID)
         drained = drain_tile_gate_reduce<PBN>(t_row, m0 + quad * 32, n0, half, g, &pp.tmR, &tfull_bar[acc],
                                               acc_phase, wc, box, box_step, tiles.sum && tile >= end1);
       else
@@ -326,7 +340,7 @@ int launch_pair_inst(const PairProblem* p, const PairTiles& tiles, cudaStream_t 
 // the epilogues that a forward uses exist for both tile widths, the others for 256 only
 template <int EPI, bool OUT_F32, bool FP8>
 int launch_pair_width(int pbn, const PairProblem* p, const PairTiles& tiles, cudaStream_t stream) {
-  constexpr bool narrow_built = (OUT_F32 && (EPI == EPI_GATE_RESID || EPI == EPI_BIAS || EPI == EPI_ADD_TABLE)) ||
+  constexpr bool narrow_built = EPI == EPI_ACT_RESID || (OUT_F32 && (EPI == EPI_GATE_RESID || EPI == EPI_BIAS || EPI == EPI_ADD_TABLE)) ||
                                 (!OUT_F32 && (EPI == EPI_BIAS || EPI == EPI_BIAS_GELU || EPI == EPI_QKV_NORM));
   if constexpr (narrow_built) {
     if (pbn == 128) return launch_pair_inst<EPI, OUT_F32, FP8, 128>(p, tiles, stream);
@@ -338,6 +352,7 @@ int launch_pair_width(int pbn, const PairProblem* p, const PairTiles& tiles, cud
 }
 
 bool narrow_tiles_built(const GemmEpilogue& epi) {
+  if (epi.mode == EPI_ACT_RESID) return true;
   if (epi.out_f32) return epi.mode == EPI_GATE_RESID || epi.mode == EPI_BIAS || epi.mode == EPI_ADD_TABLE;
   return epi.mode == EPI_BIAS || epi.mode == EPI_BIAS_GELU || epi.mode == EPI_QKV_NORM;
 }
@@ -353,7 +368,7 @@ int build_problem(PairProblem* pp, const GemmProblem& q, int operand_dtype, int 
   g.M = M; g.N = N; g.K = K;
   g.k_blocks = (K + kel - 1) / kel;
   g.tiles_m = (M + 2 * P_BM - 1) / (2 * P_BM);
-  g.tiles_n = N / pbn;
+  g.tiles_n = (N + pbn - 1) / pbn;
   g.epi = epi;
   g.status = dev_status;
   {
@@ -373,6 +388,11 @@ int build_problem(PairProblem* pp, const GemmProblem& q, int operand_dtype, int 
       return ST_INVALID_ARG;
     }
     rc = encode_tmap_2d(&pp->tmR, epi.resid, 4, (uint64_t)N, (uint64_t)M, (uint64_t)epi.ldo * 4, 32, 32);
+    if (rc) return rc;
+  }
+  if (epi.mode == EPI_ACT_RESID) {  // boxes of 128 bytes x 32 rows; what lies outside (M, N) is neither read nor written
+    rc = encode_tmap_2d(&pp->tmR, epi.out, f32 ? 4 : 2, (uint64_t)N, (uint64_t)M, (uint64_t)epi.ldo * (f32 ? 4 : 2),
+                        f32 ? 32 : 64, 32);
     if (rc) return rc;
   }
   // bf16 outputs leave through a TMA store when every warp's 32 rows are 32 consecutive
@@ -427,7 +447,7 @@ int launch_gemm_pair(const GemmProblem* q, int n, int operand_dtype, int N, int 
       set_last_error("gemm_pair: grouped problems need the same epilogue kind");
       return ST_INVALID_ARG;
     }
-    tiles256 += static_cast<long>((q[i].M + 255) / 256) * (N / 256);
+    tiles256 += static_cast<long>((q[i].M + 255) / 256) * ((N + 255) / 256);
   }
   const long after256 = sum ? static_cast<long>((a.M + 255) / 256) * (N / 256) : 0;
   const int pbn = !narrow_tiles_built(a.epi) ? 256
@@ -447,6 +467,12 @@ int launch_gemm_pair(const GemmProblem* q, int n, int operand_dtype, int N, int 
     end[i] = count;
   }
   const PairTiles tiles{end[0], end[1], end[2], sum ? 1 : 0};
+  if (a.epi.mode == EPI_ACT_RESID && a.epi.add) {
+    const int esz = a.epi.out_f32 ? 4 : 2;
+    int rc = encode_tmap_2d(&p[1].tmR, a.epi.add, esz, (uint64_t)N, (uint64_t)a.M, (uint64_t)a.epi.ld_add * esz,
+                            128 / esz, 32);
+    if (rc) return rc;
+  }
   const bool f32 = a.epi.out_f32 != 0;
   if (fp8) {
     switch (a.epi.mode) {
@@ -475,6 +501,10 @@ int launch_gemm_pair(const GemmProblem* q, int n, int operand_dtype, int N, int 
     case EPI_ADD_TABLE:
       if (!f32) break;
       return launch_pair_width<EPI_ADD_TABLE, true, false>(pbn, p, tiles, stream);
+    case EPI_ACT_RESID:
+      if (n != 1) break;
+      return f32 ? launch_pair_width<EPI_ACT_RESID, true, false>(pbn, p, tiles, stream)
+                 : launch_pair_width<EPI_ACT_RESID, false, false>(pbn, p, tiles, stream);
     default:
       break;
   }

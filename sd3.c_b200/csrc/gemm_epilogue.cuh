@@ -412,5 +412,186 @@ __device__ __forceinline__ bool drain_tile_gate_reduce(uint32_t t_row, int m_w0,
   return true;
 }
 
+// ----------------------------------------------------------------------------
+// EPI_ACT_RESID: out = act(acc + bias) + add
+// ----------------------------------------------------------------------------
+// 1 / (1 + exp(-z)): the exponential overflows to infinity for z below -88, where the quotient is 0
+__device__ __forceinline__ float sigmoid_f(float z) { return __fdividef(1.0f, 1.0f + __expf(-z)); }
+
+// The activation in fp32, accurate to a few units of 2^-22 relative to max(|y|, |act(y)|) so that fp32 outputs keep
+// their precision: GELU's tanh form as y sigmoid(2 u) (0.5 (1 + tanh u) = sigmoid(2 u); tanh.approx alone is off by 2^-11),
+// its erf form by Abramowitz and Stegun 7.1.26, erfc(x) = (a1 t + ... + a5 t^5) exp(-x^2), t = 1 / (1 + p x), off by
+// 1.5e-7 at most.
+__device__ __forceinline__ float activate(float y, int act) {
+  if (act == ACT_GELU_TANH) {
+    const float u2 = 1.5957691216057308f * y * fmaf(0.044715f, y * y, 1.0f);
+    return y * sigmoid_f(u2);
+  }
+  if (act == ACT_GELU_ERF) {
+    const float x = fabsf(y) * 0.7071067811865476f;
+    const float t = __fdividef(1.0f, fmaf(0.3275911f, x, 1.0f));
+    float p = fmaf(t, 1.061405429f, -1.453152027f);
+    p = fmaf(p, t, 1.421413741f);
+    p = fmaf(p, t, -0.284496736f);
+    p = fmaf(p, t, 0.254829592f);
+    const float half_erfc = 0.5f * p * t * __expf(-x * x);  // of |y| / sqrt(2)
+    return y > 0.f ? fmaf(-y, half_erfc, y) : y * half_erfc;
+  }
+  if (act == ACT_SILU) return y * sigmoid_f(y);
+  return y;
+}
+__device__ __forceinline__ float relu_f(float y) { return y < 0.f ? 0.f : y; }  // NaN stays NaN
+
+// v[j] = act(v[j]) for a chunk; the branch is the same for the whole launch
+template <int COUNT>
+__device__ __forceinline__ void activate_chunk(float (&v)[COUNT], int act) {
+  if (act == ACT_GELU_TANH) {
+#pragma unroll
+    for (int j = 0; j < COUNT; ++j) v[j] = activate(v[j], ACT_GELU_TANH);
+  } else if (act == ACT_GELU_ERF) {
+#pragma unroll
+    for (int j = 0; j < COUNT; ++j) v[j] = activate(v[j], ACT_GELU_ERF);
+  } else if (act == ACT_SILU) {
+#pragma unroll
+    for (int j = 0; j < COUNT; ++j) v[j] = activate(v[j], ACT_SILU);
+  } else if (act == ACT_RELU) {
+#pragma unroll
+    for (int j = 0; j < COUNT; ++j) v[j] = relu_f(v[j]);
+  }
+}
+
+// 32 bias values starting at column n, zeros past N or without a bias; whole: p is 16-byte aligned
+__device__ __forceinline__ void load_bias32(const float* p, int n, int N, bool whole, float (&dst)[32]) {
+  if (whole && n + 32 <= N) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float4 t = *(reinterpret_cast<const float4*>(p + n) + i);
+      dst[4 * i] = t.x; dst[4 * i + 1] = t.y; dst[4 * i + 2] = t.z; dst[4 * i + 3] = t.w;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 32; ++i) dst[i] = p != nullptr && n + i < N ? p[n + i] : 0.f;
+  }
+}
+
+// What an epilogue warp of the CTA-pair kernel does for EPI_ACT_RESID.  Its share of a tile is cut into boxes of 32 rows x
+// 128 bytes (32 fp32 or 64 bf16 columns), and both directions go through shared memory as TMA boxes: reading and writing
+// rows from registers (a row per thread) costs more load/store instructions than the products take (the gate + residual
+// epilogue, out-projection of 32768 rows: 0.18 ms by registers, 0.14 through boxes).  Two buffers: the box to
+// add is requested two boxes ahead, across tiles, into the buffer that its result will leave from.  Chunk c (16 bytes) of
+// row r lies at chunk c ^ (r & 7): the 128-byte swizzle of the tensor maps, free of bank conflicts row by row.
+template <int BN, bool OUT_F32>
+struct ActResidBoxes {
+  static constexpr int COLS = OUT_F32 ? 32 : 64;  // of a box
+  static constexpr int BOXES = BN / 2 / COLS;     // of a tile
+  const void *tm_out, *tm_add;
+  const GemmArgs* g;
+  uint8_t* buf;     // two boxes of 4 KiB
+  uint64_t* bar;    // two: the box to add has landed
+  int quad, half, rank, num_pairs;
+  int ahead_tile, ahead_box;  // the next box to be requested
+  uint32_t count;   // boxes done
+
+  __device__ __forceinline__ void init(const void* out_map, const void* add_map, const GemmArgs& args, uint8_t* buffers,
+                                       uint64_t* bars, int quad_, int half_, int rank_, int pair, int num_pairs_) {
+    tm_out = out_map; tm_add = add_map; g = &args; buf = buffers; bar = bars;
+    quad = quad_; half = half_; rank = rank_; num_pairs = num_pairs_;
+    ahead_tile = pair; ahead_box = 0; count = 0;
+    if (g->epi.add) {
+      request(0);
+      request(1);
+    }
+  }
+  __device__ __forceinline__ static bool exists(const GemmArgs& g, int m, int n) { return m < g.M && n < g.N; }
+  // requests the next box that exists into a buffer that nobody uses
+  __device__ __forceinline__ void request(int b) {
+    const int tiles = g->tiles_m * g->tiles_n;
+    while (ahead_tile < tiles) {
+      const int m = (ahead_tile / g->tiles_n) * 256 + rank * 128 + quad * 32;
+      const int n = (ahead_tile % g->tiles_n) * BN + half * (BN / 2) + ahead_box * COLS;
+      if (++ahead_box == BOXES) { ahead_box = 0; ahead_tile += num_pairs; }
+      if (exists(*g, m, n)) {
+        if ((threadIdx.x & 31) == 0) {
+          mbar_expect_tx(&bar[b], 4096);
+          tma_load_2d(buf + b * 4096, tm_add, &bar[b], n, m);
+        }
+        return;
+      }
+    }
+  }
+  __device__ __forceinline__ bool drain(uint32_t t_row, int m, int n0, uint64_t* tfull_bar, uint32_t phase, const WaitCtx& wc) {
+    const GemmEpilogue& e = g->epi;
+    const int lane = threadIdx.x & 31, swz = lane & 7;
+    const int nw = n0 + half * (BN / 2);
+    const bool whole = (reinterpret_cast<uintptr_t>(e.bias) & 15) == 0 && e.bias != nullptr;
+    float bb[32];
+    load_bias32(e.bias, nw, g->N, whole, bb);
+    if (!mbar_wait_warp(tfull_bar, phase, wc, DEV_TIMEOUT_TMEM_FULL)) return false;
+    tc_fence_after_sync();
+#pragma unroll 1
+    for (int i = 0; i < BOXES; ++i) {
+      const int n = nw + i * COLS;
+      if (!exists(*g, m, n)) break;
+      const int b = count & 1;
+      uint8_t* my_row = buf + b * 4096 + lane * 128;
+      if (e.add) {
+        if (!mbar_wait_warp(&bar[b], (count >> 1) & 1, wc, DEV_TIMEOUT_FULL)) return false;
+      } else {
+        if (lane == 0) bulk_wait_group_read1();  // the store before the last has read this buffer
+        __syncwarp();
+      }
+#pragma unroll
+      for (int h = 0; h < COLS / 32; ++h) {
+        uint32_t r[32];
+        tmem_ld_32x32b_x32(t_row + half * (BN / 2) + i * COLS + h * 32, r);
+        tmem_wait_ld();
+        float v[32];
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]) + bb[j];
+        load_bias32(e.bias, n + (h + 1) * 32, g->N, whole, bb);  // the next chunk's
+        activate_chunk(v, e.act);
+        if constexpr (OUT_F32) {
+#pragma unroll
+          for (int c = 0; c < 8; ++c) {
+            float4* p = reinterpret_cast<float4*>(my_row + ((c ^ swz) << 4));
+            float4 o = make_float4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
+            if (e.add) {
+              const float4 x = *p;
+              o.x += x.x; o.y += x.y; o.z += x.z; o.w += x.w;
+            }
+            *p = o;
+          }
+        } else {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            uint4* p = reinterpret_cast<uint4*>(my_row + (((4 * h + c) ^ swz) << 4));
+            float* o = &v[8 * c];
+            if (e.add) {
+              const uint4 x = *p;
+              const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                o[2 * k] += __uint_as_float(w[k] << 16);
+                o[2 * k + 1] += __uint_as_float(w[k] & 0xffff0000u);
+              }
+            }
+            *p = make_uint4(pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3]), pack_bf16x2(o[4], o[5]), pack_bf16x2(o[6], o[7]));
+          }
+        }
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+        tma_store_2d(tm_out, buf + b * 4096, n, m);
+        bulk_commit_group();
+        if (e.add) bulk_wait_group_read0();
+      }
+      if (e.add) request(b);
+      ++count;
+    }
+    return true;
+  }
+};
+
 }  // namespace gemm_detail
 }  // namespace sd3

@@ -54,6 +54,27 @@ inline void launch_dependent(void (*kernel)(Params...), dim3 grid, dim3 block, s
   cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...);  // an error is picked up by after_launch
 }
 
+// The same in clusters of `cluster` CTAs; `grid` is a multiple of it.
+template <typename... Params, typename... Args>
+inline void launch_dependent_cluster(void (*kernel)(Params...), unsigned grid, unsigned cluster, unsigned block, size_t smem,
+                                     cudaStream_t stream, Args&&... args) {
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(block);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...);  // an error is picked up by after_launch
+}
+
 // ----------------------------------------------------------------------------
 // tcgen05 GEMM:  acc[m, n] = sum_k A[m, k] * W[n, k]   (A: M x K row-major,
 // W: N x K row-major, i.e. both operands K-major), fp32 accumulation in TMEM,
@@ -66,7 +87,11 @@ enum GemmEpi : int {
   EPI_QKV_NORM = 3,    // out = per-head RMSNorm on the q and k column ranges of (acc + bias)
   EPI_ADD_TABLE = 4,   // out = acc + bias + table[m % rows_in, n]         (fp32 out)
   EPI_UNPATCHIFY = 5,  // out[b, c, 2r+ph, 2s+pw] = acc + bias, n = ph*(p*C) + pw*C + c
+  EPI_ACT_RESID = 6,   // out = act(acc + bias) + add                      (launch_linear_residual)
 };
+
+// activations of EPI_ACT_RESID, numbered like SD3_ACT_*
+enum LinearAct : int { ACT_NONE = 0, ACT_GELU_TANH = 1, ACT_GELU_ERF = 2, ACT_SILU = 3, ACT_RELU = 4 };
 
 struct GemmEpilogue {
   int mode = EPI_BIAS;
@@ -107,6 +132,10 @@ struct GemmEpilogue {
   int up_h = 0;      // patches per image column
   int up_cin = 0;    // latent channels
   int up_patch = 0;  // patch size
+  // EPI_ACT_RESID: add (M, N) of out's type, rows ld_add elements apart, or null; may be out itself
+  int act = ACT_NONE;
+  const void* add = nullptr;
+  long ld_add = 0;
   // No kernel that may still be running when this one is launched writes W (a model's packed
   // weights): the first weight tiles are then requested before the wait for the preceding kernel
   // (forward of one 256x256 image 3061 -> 2993 us, 512x512 4415 -> 4380 us).
@@ -136,6 +165,11 @@ struct GemmProblem {
 // second QKV projection of a dual block.
 int launch_gemm_grouped(const GemmProblem* q, int n, int operand_dtype, int N, int K, int* dev_status,
                         cudaStream_t stream);
+
+// out = act(x w^T + bias) + add: x (M, K) and w (N, K) bf16 with 16-byte aligned rows lda and ldw elements apart, any M and N;
+// epi: mode EPI_ACT_RESID, bias, out, ldo, out_f32, act, add, ld_add (add of out's type).
+int launch_linear_residual(const bf16* x, long lda, const bf16* w, long ldw, int M, int N, int K,
+                           const GemmEpilogue& epi, int* dev_status, cudaStream_t stream);
 
 // fp32 GEMM on the tensor cores: A and W are three bf16 planes each (split3.cuh), a_plane / w_plane
 // elements apart, rows of K elements; the result has fp32 accuracy.  One to three problems of the

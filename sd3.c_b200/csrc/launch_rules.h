@@ -67,4 +67,19 @@ inline int pair_tile_width(long tiles256, long after256, int K, bool fp8, bool g
   return 64 * narrow * k_blocks < 100 * wide * k_blocks + epilogue ? 128 : 256;
 }
 
+// linear_residual: the CTA-pair GEMM, or tiles of 128 x bn whose K a cluster of `split` CTAs shares.
+struct LinearPlan {
+  bool pair;
+  int bn, split;
+};
+inline LinearPlan linear_plan(int M, int N, int k_blocks, bool tma_out, int sms) {
+  if (tma_out && M >= 256 && N >= 128) return {true, 0, 1};
+  const int bn = N <= 64 ? 64 : 128;
+  const long tiles = static_cast<long>((M + 127) / 128) * ((N + bn - 1) / bn);
+  long split = sms / tiles;
+  if (split > 8) split = 8;
+  if (split > k_blocks) split = k_blocks;
+  return {false, bn, split < 1 ? 1 : static_cast<int>(split)};
+}
+
 }  // namespace sd3

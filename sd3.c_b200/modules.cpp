@@ -224,6 +224,27 @@ Tensor bias_f32(const Tensor& b, int64_t n) {
   return r;
 }
 
+// A tensor as rows of its last dimension: 2-D tensors keep their row stride (slices of wider rows, one row for all),
+// others are made contiguous.
+struct Rows {
+  Tensor t;
+  int64_t rows, C, ld;
+};
+Rows rows_of(const Tensor& t, const char* name) {
+  TORCH_CHECK(t.is_cuda(), "custom_modules: '", name, "' must be a CUDA tensor (this build has no CPU path)");
+  TORCH_CHECK(t.dim() >= 1 && t.size(-1) > 0, name, ": rows of at least one value expected");
+  const int64_t C = t.size(-1), rows = t.numel() / C;
+  if (t.dim() == 2 && t.stride(1) == 1 && rows > 1 && (t.stride(0) >= C || t.stride(0) == 0)) return {t, rows, C, t.stride(0)};
+  return {t.contiguous(), rows, C, C};
+}
+
+// a vector of n fp32 values next to x
+Tensor vector_f32(const Tensor& v, int64_t n, const Tensor& x, const char* name) {
+  TORCH_CHECK(v.is_cuda() && v.device() == x.device() && v.numel() == n, name, ": ", std::to_string(n),
+              " values on ", x.device().str(), " expected");
+  return v.to(torch::kFloat32).contiguous();
+}
+
 Tensor linear_impl(const Tensor& x_in, const Tensor& W, const Tensor& b, int act) {
   Tensor x = dev(x_in, "x");
   c10::cuda::CUDAGuard guard(x.device());
@@ -250,6 +271,64 @@ Tensor linear_impl(const Tensor& x_in, const Tensor& W, const Tensor& b, int act
 
 Tensor Linear_forward(Tensor& x, Tensor& W, Tensor& b) { return linear_impl(x, W, b, SD3_ACT_NONE); }
 
+int activation_tag(const std::string& a) {
+  if (a == "none") return SD3_ACT_NONE;
+  if (a == "gelu_tanh") return SD3_ACT_GELU_TANH;
+  if (a == "gelu") return SD3_ACT_GELU_ERF;
+  if (a == "silu") return SD3_ACT_SILU;
+  if (a == "relu") return SD3_ACT_RELU;
+  TORCH_CHECK(false, "linear_residual: activation none, gelu_tanh, gelu, silu or relu expected, got '", a, "'");
+}
+
+// rows of a tensor that is read or written where it lies
+Rows rows_in_place(const Tensor& t, const char* name) {
+  Rows r = rows_of(t, name);
+  TORCH_CHECK(r.t.data_ptr() == t.data_ptr() && (r.rows <= 1 || r.ld >= r.C), "linear_residual: ", name,
+              " must be contiguous, or 2-D with contiguous rows");
+  return r;
+}
+
+// linear_residual(x (..., K) bf16, w (N, K) bf16, bias (N) or None, residual (..., N) or None, activation, dtype, out)
+//   -> act(x w^T + bias) + residual of `dtype` (None: the residual's, or bf16); w is packed, (out, in).  out: optional, may
+// be the residual.
+Tensor LinearResidual_forward(const Tensor& x_in, const Tensor& w, const c10::optional<Tensor>& bias,
+                              const c10::optional<Tensor>& residual, const std::string& activation,
+                              c10::optional<torch::ScalarType> dtype, const c10::optional<Tensor>& out_in) {
+  const int act = activation_tag(activation);
+  Rows x = rows_of(x_in, "x");
+  c10::cuda::CUDAGuard guard(x.t.device());
+  if (x.ld == 0) x = {x.t.contiguous(), x.rows, x.C, x.C};
+  TORCH_CHECK(x.t.scalar_type() == torch::kBFloat16 && w.scalar_type() == torch::kBFloat16 && w.dim() == 2 &&
+                  w.device() == x.t.device() && w.size(1) == x.C && w.size(0) > 0,
+              "linear_residual: bfloat16 x (..., K) and w (N, K) on one device expected");
+  Rows wr = rows_of(w, "w");
+  if (wr.ld == 0) wr = {wr.t.contiguous(), wr.rows, wr.C, wr.C};
+  const int64_t N = wr.rows;
+  const auto dt = dtype ? *dtype : out_in ? out_in->scalar_type() : residual ? residual->scalar_type() : torch::kBFloat16;
+  TORCH_CHECK(dt == torch::kBFloat16 || dt == torch::kFloat32, "linear_residual: output of bfloat16 or float32");
+  TORCH_CHECK(x.rows < (1ll << 31) && N < (1ll << 31) && x.C < (1ll << 31), "linear_residual: sizes below 2^31 expected");
+  Tensor b;
+  if (bias) b = vector_f32(*bias, N, x.t, "bias");
+  std::vector<int64_t> shape(x_in.sizes().begin(), x_in.sizes().end());
+  shape.back() = N;
+  Tensor out = out_in ? *out_in : torch::empty(shape, x_in.options().dtype(dt));
+  TORCH_CHECK(out.sizes() == torch::IntArrayRef(shape) && out.scalar_type() == dt && out.device() == x.t.device(),
+              "linear_residual: out must have the output's shape, type and device");
+  Rows o = rows_in_place(out, "out");
+  Rows r{};
+  if (residual) {
+    TORCH_CHECK(residual->sizes() == out.sizes() && residual->scalar_type() == dt && residual->device() == x.t.device(),
+                "linear_residual: the residual must have the output's shape, type and device");
+    r = rows_of(*residual, "residual");
+    if (r.ld == 0) r = {r.t.contiguous(), r.rows, r.C, r.C};
+  }
+  ok(sd3_linear_residual(x.t.data_ptr(), x.ld, wr.t.data_ptr(), wr.ld, bias ? b.data_ptr<float>() : nullptr, act,
+                         residual ? r.t.data_ptr() : nullptr, r.ld, o.t.data_ptr(), o.ld, tag(out), (int)x.rows, (int)N,
+                         (int)x.C, stream()),
+     "sd3_linear_residual");
+  return out;
+}
+
 // mlp(x, W1, b1, W2, b2, activation, B, C_in, C_hid, C_out) -- "gelu_tanh" only
 Tensor MLP(Tensor& x, Tensor& W1, Tensor& b1, Tensor& W2, Tensor& b2, std::string activation, int B,
            int C_in, int C_hid, int C_out) {
@@ -258,27 +337,6 @@ Tensor MLP(Tensor& x, Tensor& W1, Tensor& b1, Tensor& W2, Tensor& b2, std::strin
   TORCH_CHECK(W1.size(0) == C_in && W1.size(1) == C_hid && W2.size(1) == C_out, "mlp: shape mismatch");
   Tensor h = linear_impl(x, W1, b1, SD3_ACT_GELU_TANH);
   return linear_impl(h, W2, b2, SD3_ACT_NONE);
-}
-
-// A tensor as rows of its last dimension: 2-D tensors keep their row stride (slices of wider rows, one row for all),
-// others are made contiguous.
-struct Rows {
-  Tensor t;
-  int64_t rows, C, ld;
-};
-Rows rows_of(const Tensor& t, const char* name) {
-  TORCH_CHECK(t.is_cuda(), "custom_modules: '", name, "' must be a CUDA tensor (this build has no CPU path)");
-  TORCH_CHECK(t.dim() >= 1 && t.size(-1) > 0, name, ": rows of at least one value expected");
-  const int64_t C = t.size(-1), rows = t.numel() / C;
-  if (t.dim() == 2 && t.stride(1) == 1 && rows > 1 && (t.stride(0) >= C || t.stride(0) == 0)) return {t, rows, C, t.stride(0)};
-  return {t.contiguous(), rows, C, C};
-}
-
-// a vector of n fp32 values next to x
-Tensor vector_f32(const Tensor& v, int64_t n, const Tensor& x, const char* name) {
-  TORCH_CHECK(v.is_cuda() && v.device() == x.device() && v.numel() == n, name, ": ", std::to_string(n),
-              " values on ", x.device().str(), " expected");
-  return v.to(torch::kFloat32).contiguous();
 }
 
 // layer_norm(x (..., C), w, b, eps, save_for_backward) -> [out], or [out, mean, rstd] with the statistics (one per row,
@@ -439,6 +497,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("layer_norm_backward", &LayerNorm_backward, "LayerNorm backward: gradients of x, weight and bias");
   m.def("rms_norm", &RMSNorm_forward, "RMSNorm forward");
   m.def("linear", &Linear_forward, "Linear forward");
+  m.def("linear_residual", &LinearResidual_forward, "Linear with bias, activation and residual in its epilogue",
+        pybind11::arg("x"), pybind11::arg("w"), pybind11::arg("bias") = pybind11::none(),
+        pybind11::arg("residual") = pybind11::none(), pybind11::arg("activation") = "none",
+        pybind11::arg("dtype") = pybind11::none(), pybind11::arg("out") = pybind11::none());
   m.def("conv2d", &conv2d_forward, "Conv2d forward (patch embedding form)");
   m.def("sinusoidal_embedding", &sinusoidal_embedding, "Temporal sinusoidal embeddings");
   m.def("positional_embedding", &positional_embedding2D_forward, "2D positional embeddings");

@@ -25,6 +25,9 @@ PRECISION_F32 = 1
 PRECISION_FP8 = 2
 ACT_NONE = 0
 ACT_GELU_TANH = 1
+ACT_GELU_ERF = 2  # this one and the next two: linear_residual alone
+ACT_SILU = 3
+ACT_RELU = 4
 
 
 class Sd3Error(RuntimeError):
@@ -57,6 +60,7 @@ PROTOTYPES = {
     "sd3_last_error": (c_char_p, []),
     "sd3_device_status": (c_int, [POINTER(c_int)]),
     "sd3_linear": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p]),
+    "sd3_linear_residual": (c_int, [c_void_p, c_long, c_void_p, c_long, c_void_p, c_int, c_void_p, c_long, c_void_p, c_long, c_int, c_int, c_int, c_int, c_void_p]),
     "sd3_linear_f32": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p]),
     "sd3_linear_e4m3": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_float, c_int, c_void_p]),
     "sd3_quantize_e4m3": (c_int, [c_void_p, c_int, c_void_p, c_long, c_float, c_void_p]),
@@ -194,6 +198,50 @@ def linear(x_bf16, w_nk_bf16, bias=None, act=ACT_NONE, out_dtype=None):
     return out
 
 
+def _rows(t, what, like=None):
+    """(rows, C, row stride) of a 2-D tensor whose rows are contiguous, and checks it against `like`."""
+    if t.dim() != 2 or not t.is_cuda or t.shape[1] < 1:
+        raise Sd3Error("%s: 2-D CUDA tensor expected" % what)
+    rows, C = t.shape
+    if C > 1 and t.stride(1) != 1:
+        raise Sd3Error("%s: rows must be contiguous" % what)
+    if like is not None and (t.shape != like.shape or t.dtype != like.dtype or t.device != like.device):
+        raise Sd3Error("%s: %s of %s on %s expected" % (what, tuple(like.shape), like.dtype, like.device))
+    return rows, C, t.stride(0) if rows > 1 else C
+
+
+def _vector(t, n, device, what):
+    if t is None:
+        return None
+    if t.dtype != _torch().float32 or t.numel() != n or t.device != device or not t.is_contiguous():
+        raise Sd3Error("%s: contiguous float32 tensor of %d values on %s expected" % (what, n, device))
+    return ptr(t)
+
+
+def linear_residual(x_bf16, w_nk_bf16, bias=None, act=ACT_NONE, residual=None, out_dtype=None, out=None):
+    """act(x w^T + bias) + residual, rounded once to out's type (bf16 or float32; the residual's, bf16 without one): see
+    sd3_linear_residual.  x, w, residual and out may be slices of wider rows; out may be the residual."""
+    torch = _torch()
+    M, K, ldx = _rows(x_bf16, "linear_residual: x")
+    N, Kw, ldw = _rows(w_nk_bf16, "linear_residual: w")
+    if x_bf16.dtype != torch.bfloat16 or w_nk_bf16.dtype != torch.bfloat16 or K != Kw or w_nk_bf16.device != x_bf16.device:
+        raise Sd3Error("linear_residual: bfloat16 x (M, K) and w (N, K) on one device expected")
+    if out is None:
+        out = torch.empty((M, N), device=x_bf16.device,
+                          dtype=out_dtype or (residual.dtype if residual is not None else torch.bfloat16))
+    if out.shape != (M, N) or out.device != x_bf16.device or (out_dtype is not None and out.dtype != out_dtype):
+        raise Sd3Error("linear_residual: out must have the output's shape, type and device")
+    ldo = _rows(out, "linear_residual: out")[2]
+    ldr = _rows(residual, "linear_residual: residual", out)[2] if residual is not None else 0
+    with torch.cuda.device(x_bf16.device):
+        check(lib().sd3_linear_residual(c_void_p(x_bf16.data_ptr()), ldx, c_void_p(w_nk_bf16.data_ptr()), ldw,
+                                        _vector(bias, N, x_bf16.device, "linear_residual: bias"), act,
+                                        c_void_p(residual.data_ptr()) if residual is not None else None, ldr,
+                                        c_void_p(out.data_ptr()), ldo, dtype_tag(out), M, N, K, stream_ptr()),
+              "sd3_linear_residual")
+    return out
+
+
 def linear_f32(x, w_nk, bias=None, act=ACT_NONE):
     torch = _torch()
     M, K = x.shape
@@ -295,26 +343,6 @@ def layernorm_modulate(x, B, T, E, eps, shift1, scale1, shift2=None, scale2=None
                                        ptr(out2), ms, dtype_tag(out1), stream_ptr()),
           "sd3_layernorm_modulate")
     return out1, out2
-
-
-def _rows(t, what, like=None):
-    """(rows, C, row stride) of a 2-D tensor whose rows are contiguous, and checks it against `like`."""
-    if t.dim() != 2 or not t.is_cuda or t.shape[1] < 1:
-        raise Sd3Error("%s: 2-D CUDA tensor expected" % what)
-    rows, C = t.shape
-    if C > 1 and t.stride(1) != 1:
-        raise Sd3Error("%s: rows must be contiguous" % what)
-    if like is not None and (t.shape != like.shape or t.dtype != like.dtype or t.device != like.device):
-        raise Sd3Error("%s: %s of %s on %s expected" % (what, tuple(like.shape), like.dtype, like.device))
-    return rows, C, t.stride(0) if rows > 1 else C
-
-
-def _vector(t, n, device, what):
-    if t is None:
-        return None
-    if t.dtype != _torch().float32 or t.numel() != n or t.device != device or not t.is_contiguous():
-        raise Sd3Error("%s: contiguous float32 tensor of %d values on %s expected" % (what, n, device))
-    return ptr(t)
 
 
 def layer_norm(x, w=None, b=None, eps=1e-5):
