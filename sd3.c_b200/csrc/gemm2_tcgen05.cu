@@ -72,7 +72,18 @@ __host__ __device__ constexpr int pair_slot(int pbn) { return pbn == 256 ? 1 : 2
 __host__ __device__ constexpr int pair_red_bytes(int epi, bool out_f32) {
   return pair_stages_out(epi, out_f32) ? EPI_WARPS * P_RED_BYTES * (epi == EPI_ACT_RESID ? 2 : 1) : 0;
 }
-constexpr int P_THREADS = 64 + 32 * EPI_WARPS;
+// The tensor cores cut a sum off, rather than round it, at every step of 16 of K: over K = 6144 a result is off by 4.8e-6
+// (2-norm, against 64 bits), where fp32 additions that round are off by 5.6e-7.  fp32 outputs of EPI_ACT_RESID are therefore
+// accumulated over 512 of K at a time; the epilogue warps add these sums in registers, which rounds.
+__host__ __device__ constexpr bool pair_in_chunks(int epi, bool out_f32) { return epi == EPI_ACT_RESID && out_f32; }
+constexpr int P_CHUNK = 8;  // K blocks
+// Half a row of running sums is 128 registers.  The epilogue warps of that kernel are two whole warpgroups (warps 4 to 11;
+// 2 and 3 idle) that take over registers of the first one: 384 threads x 168 at launch, then 128 x 64 + 256 x 216.
+// (128-wide tiles, whose sums fit, take 338 us for 16384 x 1536 with K 6144 where 256-wide ones take 255.)
+constexpr int P_REGS_LAUNCH = 168, P_REGS_ISSUE = 64, P_REGS_EPI = 216;
+__host__ __device__ constexpr int pair_epi_warp0(int epi, bool out_f32) { return pair_in_chunks(epi, out_f32) ? 4 : 2; }
+__host__ __device__ constexpr int pair_threads(int epi, bool out_f32) { return 32 * (pair_epi_warp0(epi, out_f32) + EPI_WARPS); }
+static_assert(128 * P_REGS_ISSUE + 32 * EPI_WARPS * P_REGS_EPI <= (128 + 32 * EPI_WARPS) * P_REGS_LAUNCH, "the shares fit the launch");
 __host__ __device__ constexpr int pair_smem_bytes(int epi, bool out_f32, int pbn) {
   return pair_stages(pbn, epi) * pair_stage_bytes(pbn) + pair_red_bytes(epi, out_f32) +
          (epi == EPI_ACT_RESID ? 512 : 256) + 1024;
@@ -85,7 +96,7 @@ struct PairProblem {
 };
 
 template <int EPI, bool OUT_F32, bool FP8, int PBN>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair_threads(EPI, OUT_F32), 1)
 gemm_pair_tcgen05_kernel(const __grid_constant__ PairProblem p0, const __grid_constant__ PairProblem p1,
                          const __grid_constant__ PairProblem p2, const PairTiles all) {
   // M = 256 across the pair; operands bf16, or e4m3 (128 K-elements per 128-byte stage row,
@@ -157,10 +168,15 @@ gemm_pair_tcgen05_kernel(const __grid_constant__ PairProblem p0, const __grid_co
   const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_slot, 0);
   const WaitCtx wc{s_abort, p0.g.status};
 
+  constexpr bool CHUNKS = pair_in_chunks(EPI, OUT_F32);
+  constexpr int EPI_WARP0 = pair_epi_warp0(EPI, OUT_F32);
+  static_assert(P_CHUNK % pair_slot(PBN) == 0, "a slot belongs to one chunk");
   constexpr int SLOT = pair_slot(PBN);
   constexpr int NSLOT = P_STAGES / SLOT;
   const int KB = p0.g.k_blocks;  // the same K for all problems
 
+  if (warp < EPI_WARP0) {
+  if constexpr (CHUNKS) setmaxnreg_dec<P_REGS_ISSUE>();
   if (warp == 0) {
     // ------------------------------ TMA producer (both CTAs, one warp) --------
     int stage = 0;
@@ -223,12 +239,19 @@ gemm_pair_tcgen05_kernel(const __grid_constant__ PairProblem p0, const __grid_co
       const bool issuer = elect_one();
       const uint64_t desc0 = make_smem_desc_sw128(smem_u32(smem), 16, 1024);
       for (int tile = pair; tile < num_tiles && ok; tile = tiles.next(tile, num_pairs)) {
-        const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * PBN);
+        uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * PBN);
         if (!mbar_wait_all(&tempty_bar[acc], acc_phase ^ 1, wc, DEV_TIMEOUT_TMEM_EMPTY)) break;
         for (int kb = 0; kb < KB; kb += SLOT) {
+          if (CHUNKS && kb > 0 && kb % P_CHUNK == 0) {  // the next chunk's accumulator
+            acc ^= 1;
+            if (acc == 0) acc_phase ^= 1;
+            d_tmem = tmem_base + static_cast<uint32_t>(acc * PBN);
+            if (!mbar_wait_all(&tempty_bar[acc], acc_phase ^ 1, wc, DEV_TIMEOUT_TMEM_EMPTY)) { ok = false; break; }
+          }
           if (!mbar_wait_all(&full_bar[stage], phase, wc, DEV_TIMEOUT_FULL)) { ok = false; break; }
           tc_fence_after_sync();
           if (issuer) {
+            const int kc = CHUNKS ? kb % P_CHUNK : kb;
 #pragma unroll
             for (int i = 0; i < SLOT; ++i) {
               if (SLOT > 1 && kb + i >= KB) break;
@@ -238,13 +261,14 @@ gemm_pair_tcgen05_kernel(const __grid_constant__ PairProblem p0, const __grid_co
               for (int k = 0; k < P_KBYTES / 32; ++k) {
                 const uint64_t adv = static_cast<uint64_t>((k * 32) >> 4);
                 if constexpr (FP8)
-                  mma_f8_ss_pair(d_tmem, a_desc + adv, b_desc + adv, IDESC, (kb | i | k) != 0);
+                  mma_f8_ss_pair(d_tmem, a_desc + adv, b_desc + adv, IDESC, (kc | i | k) != 0);
                 else
-                  mma_f16_ss_pair(d_tmem, a_desc + adv, b_desc + adv, IDESC, (kb | i | k) != 0);
+                  mma_f16_ss_pair(d_tmem, a_desc + adv, b_desc + adv, IDESC, (kc | i | k) != 0);
               }
             }
             mma_commit_pair(&empty_bar[stage], 3);                     // frees the slot in both CTAs
-            if (kb + SLOT >= KB) mma_commit_pair(&tfull_bar[acc], 3);  // accumulator ready in both CTAs
+            if (kb + SLOT >= KB || (CHUNKS && (kb + SLOT) % P_CHUNK == 0))
+              mma_commit_pair(&tfull_bar[acc], 3);  // accumulator ready in both CTAs
           }
           if (++stage == NSLOT) { stage = 0; phase ^= 1; }
         }
@@ -252,17 +276,19 @@ gemm_pair_tcgen05_kernel(const __grid_constant__ PairProblem p0, const __grid_co
         if (acc == 0) acc_phase ^= 1;
       }
     }
+  }
   } else {
     // ------------------------------ epilogue (both CTAs) ----------------------
+    if constexpr (CHUNKS) setmaxnreg_inc<P_REGS_EPI>();
     const int quad = warp & 3;
-    const int half = (warp - 2) >> 2;
+    const int half = (warp - EPI_WARP0) >> 2;
     const int row = quad * 32 + lane;
     int acc = 0;
     uint32_t acc_phase = 0;
     // EPI_ACT_RESID is a launch of one problem; its rows to add are described by p1.tmR
     ActResidBoxes<PBN, OUT_F32> boxes;
     if constexpr (EPI == EPI_ACT_RESID)
-      boxes.init(&p0.tmR, &p1.tmR, p0.g, red_smem + (warp - 2) * 2 * P_RED_BYTES, add_bar + 2 * (warp - 2), quad, half,
+      boxes.init(&p0.tmR, &p1.tmR, p0.g, red_smem + (warp - EPI_WARP0) * 2 * P_RED_BYTES, add_bar + 2 * (warp - EPI_WARP0), quad, half,
                  static_cast<int>(rank), pair, num_pairs);
     for (int tile = pair; tile < num_tiles; tile = tiles.next(tile, num_pairs)) {
       const PairProblem& pp = tile < end0 ? p0 : tile < end1 ? p1 : p2;
@@ -272,6 +298,32 @@ gemm_pair_tcgen05_kernel(const __grid_constant__ PairProblem p0, const __grid_co
       const int n0 = (lt % g.tiles_n) * PBN;
       const uint32_t t_row = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) +
                              static_cast<uint32_t>(acc * PBN);
+      if constexpr (CHUNKS) {
+        float sums[PBN / 2];
+        boxes.start(sums, n0);
+#pragma unroll 1
+        for (int kb = 0; kb < KB; kb += P_CHUNK) {
+          if (!mbar_wait_warp(&tfull_bar[acc], acc_phase, wc, DEV_TIMEOUT_TMEM_FULL)) break;
+          tc_fence_after_sync();
+          const uint32_t t_chunk = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) +
+                                   static_cast<uint32_t>(acc * PBN + half * (PBN / 2));
+#pragma unroll
+          for (int c = 0; c < PBN / 2; c += 16) {  // 32 at a time, and the compiler spills
+            uint32_t r[16];
+            tmem_ld_32x32b_x16(t_chunk + c, r);
+            tmem_wait_ld();
+#pragma unroll
+            for (int j = 0; j < 16; ++j) sums[c + j] += __uint_as_float(r[j]);
+          }
+          tc_fence_before_sync();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster(map_to_cta(smem_u32(&tempty_bar[acc]), 0));
+          acc ^= 1;
+          if (acc == 0) acc_phase ^= 1;
+        }
+        if (*wc.s_abort || !boxes.finish(sums, m0 + quad * 32, n0, wc)) break;
+        continue;
+      }
       bool drained;
       // After the pair's last tile the operand ring is idle (its accumulator is complete, so every load has landed
       // and every MMA has read it): each box of the epilogue gets a buffer of its own there, and none waits for the
@@ -281,7 +333,7 @@ gemm_pair_tcgen05_kernel(const __grid_constant__ PairProblem p0, const __grid_co
       constexpr bool OWN_BOXES = !(EPI == EPI_QKV_NORM && PBN == 256);
       const bool last = OWN_BOXES && tiles.next(tile, num_pairs) >= num_tiles;
       constexpr int BOXES = PBN / 2 / (EPI == EPI_GATE_RESID ? 32 : 64);  // of a warp and tile
-      uint8_t* box = last ? smem + (warp - 2) * (BOXES * P_RED_BYTES) : red_smem + (warp - 2) * P_RED_BYTES;
+      uint8_t* box = last ? smem + (warp - EPI_WARP0) * (BOXES * P_RED_BYTES) : red_smem + (warp - EPI_WARP0) * P_RED_BYTES;
       const int box_step = last ? P_RED_BYTES : 0;
       if constexpr (EPI == EPI_ACT_RESID)
         drained = boxes.drain(t_row, m0 + quad * 32, n0, &tfull_bar[acc], acc_phase, wc);
@@ -328,12 +380,21 @@ int launch_pair_inst(const PairProblem* p, const PairTiles& tiles, cudaStream_t 
     if (!attr_done[dev]) {
       cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
       if (e != cudaSuccess) return check_cuda(e, "cudaFuncSetAttribute(gemm_pair)");
+      if constexpr (pair_in_chunks(EPI, OUT_F32)) {
+        cudaFuncAttributes fa;
+        e = cudaFuncGetAttributes(&fa, kern);
+        if (e != cudaSuccess) return check_cuda(e, "cudaFuncGetAttributes(gemm_pair)");
+        if (fa.numRegs != P_REGS_LAUNCH) {  // the epilogue's share would never come together
+          set_last_error("gemm_pair: built with %d registers a thread, %d expected", fa.numRegs, P_REGS_LAUNCH);
+          return ST_UNSUPPORTED;
+        }
+      }
       attr_done[dev] = true;
     }
   }
   const int max_pairs = device_sm_count() / 2;
   const int pairs = tiles.starts() < max_pairs ? tiles.starts() : max_pairs;
-  launch_dependent(kern, 2 * pairs, P_THREADS, SMEM, stream, p[0], p[1], p[2], tiles);
+  launch_dependent(kern, 2 * pairs, pair_threads(EPI, OUT_F32), SMEM, stream, p[0], p[1], p[2], tiles);
   return after_launch("gemm_pair_tcgen05_kernel");
 }
 

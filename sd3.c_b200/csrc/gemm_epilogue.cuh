@@ -415,49 +415,69 @@ __device__ __forceinline__ bool drain_tile_gate_reduce(uint32_t t_row, int m_w0,
 // ----------------------------------------------------------------------------
 // EPI_ACT_RESID: out = act(acc + bias) + add
 // ----------------------------------------------------------------------------
-// 1 / (1 + exp(-z)): the exponential overflows to infinity for z below -88, where the quotient is 0
-__device__ __forceinline__ float sigmoid_f(float z) { return __fdividef(1.0f, 1.0f + __expf(-z)); }
-
-// The activation in fp32, accurate to a few units of 2^-22 relative to max(|y|, |act(y)|) so that fp32 outputs keep
-// their precision: GELU's tanh form as y sigmoid(2 u) (0.5 (1 + tanh u) = sigmoid(2 u); tanh.approx alone is off by 2^-11),
-// its erf form by Abramowitz and Stegun 7.1.26, erfc(x) = (a1 t + ... + a5 t^5) exp(-x^2), t = 1 / (1 + p x), off by
-// 1.5e-7 at most.
-__device__ __forceinline__ float activate(float y, int act) {
-  if (act == ACT_GELU_TANH) {
-    const float u2 = 1.5957691216057308f * y * fmaf(0.044715f, y * y, 1.0f);
-    return y * sigmoid_f(u2);
-  }
-  if (act == ACT_GELU_ERF) {
-    const float x = fabsf(y) * 0.7071067811865476f;
-    const float t = __fdividef(1.0f, fmaf(0.3275911f, x, 1.0f));
-    float p = fmaf(t, 1.061405429f, -1.453152027f);
-    p = fmaf(p, t, 1.421413741f);
-    p = fmaf(p, t, -0.284496736f);
-    p = fmaf(p, t, 0.254829592f);
-    const float half_erfc = 0.5f * p * t * __expf(-x * x);  // of |y| / sqrt(2)
-    return y > 0.f ? fmaf(-y, half_erfc, y) : y * half_erfc;
-  }
-  if (act == ACT_SILU) return y * sigmoid_f(y);
+__device__ __forceinline__ float ex2_f(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-__device__ __forceinline__ float relu_f(float y) { return y < 0.f ? 0.f : y; }  // NaN stays NaN
+__device__ __forceinline__ float rcp_f(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float2 two(float x) { return make_float2(x, x); }
+// y / (1 + 2^z): 2^z is infinite for z above 128, where the quotient is 0
+__device__ __forceinline__ float2 over_one_plus_exp2(float2 y, float2 z) {
+  const float2 d = __fadd2_rn(make_float2(ex2_f(z.x), ex2_f(z.y)), two(1.0f));
+  return __fmul2_rn(y, make_float2(rcp_f(d.x), rcp_f(d.y)));
+}
 
+// Two activations in fp32, accurate to a few units of 2^-22 of max(|y|, 1) so that fp32 outputs keep their precision, with
+// packed instructions: an epilogue has as many issue slots per value as the products of 64 of K take (16384 x 6144, K 1536,
+// erf form: 283 us with scalar ones, 230 packed).
+// GELU's tanh form is y sigmoid(2 u), since 0.5 (1 + tanh u) = sigmoid(2 u) (tanh.approx alone is off by 2^-11).  Its erf
+// form is max(y, 0) - |y| erfc(|y| / sqrt 2) / 2 with Abramowitz and Stegun 7.1.26: erfc(x) = (a1 t + ... + a5 t^5)
+// exp(-x^2), t = 1 / (1 + p x), off by 1.5e-7 at most.
+template <int ACT>
+__device__ __forceinline__ float2 activate2(float2 y) {
+  if constexpr (ACT == ACT_GELU_TANH) {
+    // 2^z = exp(-2 u), u = sqrt(2 / pi) (y + 0.044715 y^3)
+    const float2 q = __ffma2_rn(__fmul2_rn(y, y), two(-2.3022082f * 0.044715f), two(-2.3022082f));
+    return over_one_plus_exp2(y, __fmul2_rn(q, y));
+  } else if constexpr (ACT == ACT_GELU_ERF) {
+    const float2 a = make_float2(fabsf(y.x), fabsf(y.y));
+    const float2 d = __ffma2_rn(a, two(0.3275911f * 0.70710678f), two(1.0f));
+    const float2 t = make_float2(rcp_f(d.x), rcp_f(d.y));
+    float2 p = __ffma2_rn(t, two(0.5f * 1.061405429f), two(0.5f * -1.453152027f));
+    p = __ffma2_rn(p, t, two(0.5f * 1.421413741f));
+    p = __ffma2_rn(p, t, two(0.5f * -0.284496736f));
+    p = __ffma2_rn(p, t, two(0.5f * 0.254829592f));
+    const float2 z = __fmul2_rn(__fmul2_rn(y, y), two(-0.72134752f));  // exp(-y^2 / 2) = 2^z
+    const float2 h = __fmul2_rn(__fmul2_rn(p, t), make_float2(ex2_f(z.x), ex2_f(z.y)));
+    return __ffma2_rn(make_float2(-a.x, -a.y), h, make_float2(fmaxf(y.x, 0.f), fmaxf(y.y, 0.f)));
+  } else if constexpr (ACT == ACT_SILU) {
+    return over_one_plus_exp2(y, __fmul2_rn(y, two(-1.44269504f)));
+  } else if constexpr (ACT == ACT_RELU) {
+    return make_float2(y.x < 0.f ? 0.f : y.x, y.y < 0.f ? 0.f : y.y);  // NaN stays NaN
+  }
+  return y;
+}
+template <int ACT, int COUNT>
+__device__ __forceinline__ void activate_all(float (&v)[COUNT]) {
+#pragma unroll
+  for (int j = 0; j < COUNT; j += 2) {
+    const float2 o = activate2<ACT>(make_float2(v[j], v[j + 1]));
+    v[j] = o.x;
+    v[j + 1] = o.y;
+  }
+}
 // v[j] = act(v[j]) for a chunk; the branch is the same for the whole launch
 template <int COUNT>
 __device__ __forceinline__ void activate_chunk(float (&v)[COUNT], int act) {
-  if (act == ACT_GELU_TANH) {
-#pragma unroll
-    for (int j = 0; j < COUNT; ++j) v[j] = activate(v[j], ACT_GELU_TANH);
-  } else if (act == ACT_GELU_ERF) {
-#pragma unroll
-    for (int j = 0; j < COUNT; ++j) v[j] = activate(v[j], ACT_GELU_ERF);
-  } else if (act == ACT_SILU) {
-#pragma unroll
-    for (int j = 0; j < COUNT; ++j) v[j] = activate(v[j], ACT_SILU);
-  } else if (act == ACT_RELU) {
-#pragma unroll
-    for (int j = 0; j < COUNT; ++j) v[j] = relu_f(v[j]);
-  }
+  if (act == ACT_GELU_TANH) activate_all<ACT_GELU_TANH>(v);
+  else if (act == ACT_GELU_ERF) activate_all<ACT_GELU_ERF>(v);
+  else if (act == ACT_SILU) activate_all<ACT_SILU>(v);
+  else if (act == ACT_RELU) activate_all<ACT_RELU>(v);
 }
 
 // 32 bias values starting at column n, zeros past N or without a bias; whole: p is 16-byte aligned
@@ -519,11 +539,66 @@ struct ActResidBoxes {
       }
     }
   }
+  // before the warp writes box number `count`: what it adds has landed, or the store before the last has read the buffer
+  __device__ __forceinline__ bool open_box(const WaitCtx& wc) {
+    if (g->epi.add) return mbar_wait_warp(&bar[count & 1], (count >> 1) & 1, wc, DEV_TIMEOUT_FULL);
+    if ((threadIdx.x & 31) == 0) bulk_wait_group_read1();
+    __syncwarp();
+    return true;
+  }
+  // 32 finished columns of this lane's row into the box, columns [32 h, +32) of it, with what is to be added
+  __device__ __forceinline__ void put(float (&v)[32], int h) {
+    const int lane = threadIdx.x & 31, swz = lane & 7;
+    uint8_t* my_row = buf + (count & 1) * 4096 + lane * 128;
+    const bool add = g->epi.add != nullptr;
+    if constexpr (OUT_F32) {
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {
+        float4* p = reinterpret_cast<float4*>(my_row + ((c ^ swz) << 4));
+        float4 o = make_float4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
+        if (add) {
+          const float4 x = *p;
+          o.x += x.x; o.y += x.y; o.z += x.z; o.w += x.w;
+        }
+        *p = o;
+      }
+    } else {
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        uint4* p = reinterpret_cast<uint4*>(my_row + (((4 * h + c) ^ swz) << 4));
+        float* o = &v[8 * c];
+        if (add) {
+          const uint4 x = *p;
+          const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            o[2 * k] += __uint_as_float(w[k] << 16);
+            o[2 * k + 1] += __uint_as_float(w[k] & 0xffff0000u);
+          }
+        }
+        *p = make_uint4(pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3]), pack_bf16x2(o[4], o[5]), pack_bf16x2(o[6], o[7]));
+      }
+    }
+  }
+  // the box leaves for rows m, columns n; the box after the next is requested into its buffer
+  __device__ __forceinline__ void close_box(int m, int n) {
+    const int b = count & 1;
+    fence_proxy_async_smem();
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) {
+      tma_store_2d(tm_out, buf + b * 4096, n, m);
+      bulk_commit_group();
+      if (g->epi.add) bulk_wait_group_read0();
+    }
+    if (g->epi.add) request(b);
+    ++count;
+  }
+
+  // bf16 outputs: one accumulator holds the whole sum
   __device__ __forceinline__ bool drain(uint32_t t_row, int m, int n0, uint64_t* tfull_bar, uint32_t phase, const WaitCtx& wc) {
     const GemmEpilogue& e = g->epi;
-    const int lane = threadIdx.x & 31, swz = lane & 7;
     const int nw = n0 + half * (BN / 2);
-    const bool whole = (reinterpret_cast<uintptr_t>(e.bias) & 15) == 0 && e.bias != nullptr;
+    const bool whole = e.bias != nullptr && (reinterpret_cast<uintptr_t>(e.bias) & 15) == 0;
     float bb[32];
     load_bias32(e.bias, nw, g->N, whole, bb);
     if (!mbar_wait_warp(tfull_bar, phase, wc, DEV_TIMEOUT_TMEM_FULL)) return false;
@@ -532,14 +607,7 @@ struct ActResidBoxes {
     for (int i = 0; i < BOXES; ++i) {
       const int n = nw + i * COLS;
       if (!exists(*g, m, n)) break;
-      const int b = count & 1;
-      uint8_t* my_row = buf + b * 4096 + lane * 128;
-      if (e.add) {
-        if (!mbar_wait_warp(&bar[b], (count >> 1) & 1, wc, DEV_TIMEOUT_FULL)) return false;
-      } else {
-        if (lane == 0) bulk_wait_group_read1();  // the store before the last has read this buffer
-        __syncwarp();
-      }
+      if (!open_box(wc)) return false;
 #pragma unroll
       for (int h = 0; h < COLS / 32; ++h) {
         uint32_t r[32];
@@ -550,44 +618,42 @@ struct ActResidBoxes {
         for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]) + bb[j];
         load_bias32(e.bias, n + (h + 1) * 32, g->N, whole, bb);  // the next chunk's
         activate_chunk(v, e.act);
-        if constexpr (OUT_F32) {
-#pragma unroll
-          for (int c = 0; c < 8; ++c) {
-            float4* p = reinterpret_cast<float4*>(my_row + ((c ^ swz) << 4));
-            float4 o = make_float4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
-            if (e.add) {
-              const float4 x = *p;
-              o.x += x.x; o.y += x.y; o.z += x.z; o.w += x.w;
-            }
-            *p = o;
-          }
-        } else {
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            uint4* p = reinterpret_cast<uint4*>(my_row + (((4 * h + c) ^ swz) << 4));
-            float* o = &v[8 * c];
-            if (e.add) {
-              const uint4 x = *p;
-              const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                o[2 * k] += __uint_as_float(w[k] << 16);
-                o[2 * k + 1] += __uint_as_float(w[k] & 0xffff0000u);
-              }
-            }
-            *p = make_uint4(pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3]), pack_bf16x2(o[4], o[5]), pack_bf16x2(o[6], o[7]));
-          }
-        }
+        put(v, h);
       }
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) {
-        tma_store_2d(tm_out, buf + b * 4096, n, m);
-        bulk_commit_group();
-        if (e.add) bulk_wait_group_read0();
+      close_box(m, n);
+    }
+    return true;
+  }
+
+  // fp32 outputs: this lane's BN / 2 running sums start from the bias, loaded while the first products are under way
+  __device__ __forceinline__ void start(float (&sums)[BN / 2], int n0) const {
+    const int nw = n0 + half * (BN / 2);
+    const float* p = g->epi.bias;
+    if (p != nullptr && (reinterpret_cast<uintptr_t>(p) & 15) == 0 && nw + BN / 2 <= g->N) {
+#pragma unroll
+      for (int i = 0; i < BN / 2; i += 4) {
+        const float4 t = *reinterpret_cast<const float4*>(p + nw + i);
+        sums[i] = t.x; sums[i + 1] = t.y; sums[i + 2] = t.z; sums[i + 3] = t.w;
       }
-      if (e.add) request(b);
-      ++count;
+    } else {
+#pragma unroll
+      for (int i = 0; i < BN / 2; ++i) sums[i] = p != nullptr && nw + i < g->N ? p[nw + i] : 0.f;
+    }
+  }
+  __device__ __forceinline__ bool finish(float (&sums)[BN / 2], int m, int n0, const WaitCtx& wc) {
+    const GemmEpilogue& e = g->epi;
+    const int nw = n0 + half * (BN / 2);
+#pragma unroll
+    for (int i = 0; i < BOXES; ++i) {
+      const int n = nw + i * COLS;
+      if (!exists(*g, m, n)) break;
+      float v[32];
+#pragma unroll
+      for (int j = 0; j < 32; ++j) v[j] = sums[i * 32 + j];
+      activate_chunk(v, e.act);
+      if (!open_box(wc)) return false;
+      put(v, 0);
+      close_box(m, n);
     }
     return true;
   }

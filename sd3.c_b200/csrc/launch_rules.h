@@ -67,19 +67,39 @@ inline int pair_tile_width(long tiles256, long after256, int K, bool fp8, bool g
   return 64 * narrow * k_blocks < 100 * wide * k_blocks + epilogue ? 128 : 256;
 }
 
-// linear_residual: the CTA-pair GEMM, or tiles of 128 x bn whose K a cluster of `split` CTAs shares.
+// linear_residual: the CTA-pair GEMM, or tiles of 128 x bn whose K a cluster of `split` CTAs shares (one CTA an SM).  What
+// decides is how many SMs load operands: a lone SM takes 75 to 90 bytes a clock.  64-wide tiles where they fit one wave, with
+// the largest split of 1, 2, 4 or 8 that still does (clusters of 3, 5 and 6 leave SMs of a GPC idle); else pairs, or for one tile of
+// rows, where half of a pair's would be idle, 128-wide tiles.  Measured, us, bf16 with residual, weights from HBM
+// (P: pairs; 64/2: 64-wide, split 2):
+//   M    N     K      the rule's    others
+//   1    6144  1536   64/1  8.0     64/2 13.3   128/2  8.1   128/1  9.0
+//   1    1536  6144   64/4  8.8     64/2 11.9   64/8  13.7   128/8  8.3
+//   1    24576 1536   128/1 20.6    64/1 24.1   P 34.7
+//   64   1536  1536   64/4  5.7     64/2  6.2   64/8   6.9   128/4  6.7    P  9.2
+//   77   12288 1536   128/1 13.0    64/1 17.2   P 15.5
+//   154  1536  1536   64/2  8.0     64/1  8.6   64/4  12.9   P  9.5
+//   154  6144  1536   P 10.5        64/1 15.7   128/1 14.8
+//   256  1536  6144   64/2 14.3     64/1 22.5   128/4 16.4   P 25.0
+//   512  1536  1536   64/1  9.2     P  9.6
+//   600  1536  1536   64/1  8.7     P  9.6
+//   1024 1536  6144   P 24.9        128/1 36.1
+//   1357 1001  1544   128/1 17.3    64/1 24.4   (rows that no TMA store can write)
 struct LinearPlan {
   bool pair;
   int bn, split;
 };
-inline LinearPlan linear_plan(int M, int N, int k_blocks, bool tma_out, int sms) {
-  if (tma_out && M >= 256 && N >= 128) return {true, 0, 1};
-  const int bn = N <= 64 ? 64 : 128;
-  const long tiles = static_cast<long>((M + 127) / 128) * ((N + bn - 1) / bn);
-  long split = sms / tiles;
-  if (split > 8) split = 8;
-  if (split > k_blocks) split = k_blocks;
-  return {false, bn, split < 1 ? 1 : static_cast<int>(split)};
+inline LinearPlan linear_plan(int M, int N, int k_blocks, bool tma_out, bool f32, int sms) {
+  const long rows = (M + 127) / 128;
+  const long tiles64 = rows * ((N + 63) / 64);
+  if (tiles64 <= sms) {
+    int split = 1;
+    while (split < 8 && 2 * split <= k_blocks && 2 * split * tiles64 <= sms) split *= 2;
+    return {false, 64, split};
+  }
+  if (tma_out && rows > 1) return {true, 0, 1};
+  // fp32 sums of more than 2048 of K want more accumulators than 128-wide tiles leave room for
+  return {false, f32 && k_blocks > 32 ? 64 : 128, 1};
 }
 
 }  // namespace sd3

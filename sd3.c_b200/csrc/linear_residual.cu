@@ -9,10 +9,12 @@
 // loads only the rows there are) and leaves the accumulator in the shared memory of the CTAs of its cluster: CTA r gets
 // the columns r of the cluster's split of the tile from everyone.  It adds the partial sums in the CTAs' order (the same
 // bits every time), applies bias, activation and residual and writes its columns, neighbouring threads neighbouring
-// columns: coalesced whatever the row pitch, element by element where rows are not aligned.
+// columns: coalesced whatever the row pitch, element by element where rows are not aligned.  fp32 outputs are summed in
+// several accumulators, added in registers: the tensor cores cut a sum off at every step (gemm2_tcgen05.cu).
 #include <cuda.h>
 
 #include <mutex>
+#include <type_traits>
 
 #include "gemm_epilogue.cuh"
 #include "kernels.h"
@@ -33,8 +35,8 @@ using namespace gemm_detail;
 
 constexpr int LR_BM = 128;
 constexpr int LR_KBYTES = 128;  // bytes of K per stage row: 64 bf16
+constexpr int LR_SLOT = 2;  // K blocks of a stage: a hand-over takes longer than the MMAs of one (350 cycles a block one by one)
 constexpr int LR_MAX_STAGES = 12;
-constexpr int LR_MAX_SPLIT = 8;
 constexpr int LR_THREADS = 64 + 32 * EPI_WARPS;
 constexpr int LR_SMEM = 227 * 1024;
 
@@ -43,60 +45,138 @@ struct LinearArgs {
   int split;        // CTAs of a cluster, each with its share of the K blocks
   int cols;         // columns that a CTA of the cluster finishes, a multiple of 4
   int a_rows;       // rows of x that a stage loads
-  int stages, stage_bytes;
+  int stages, stage_bytes, block_bytes;  // a block: 64 of K
+  int accs, chunk;  // accumulators, and the K blocks that each takes
   int vec_store;    // groups of four columns of out and add are aligned
   GemmEpilogue epi;
   int* status;
 };
 
-// room for the partial sums of `cols` columns from `split` CTAs; rows 4 floats longer than the columns need, so that the
-// 16-byte writes of eight consecutive rows fall into different banks
-__host__ __device__ inline int partial_bytes(int split, int cols) { return split * LR_BM * (cols + 4) * 4; }
+// Room for the partial sums of `cols` columns of `rows` rows from `split` CTAs, and for what an MMA may read behind the last
+// stage.  Rows are 4 floats longer than the columns need, so that the 16-byte writes of eight consecutive rows fall into
+// different banks.
+__host__ __device__ inline int partial_bytes(int split, int rows, int cols) {
+  const int bytes = split * rows * (cols + 4) * 4;
+  return bytes > LR_BM * LR_KBYTES ? bytes : LR_BM * LR_KBYTES;
+}
 
-template <bool OUT_F32>
-__device__ __forceinline__ void finish4(const LinearArgs& a, int m, int n, const float4& acc) {
-  const GemmEpilogue& e = a.epi;
-  float v[4] = {acc.x, acc.y, acc.z, acc.w};
-  const bool whole = a.vec_store != 0 && n + 4 <= a.N;
-  if (e.bias) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (n + j < a.N) v[j] += e.bias[n + j];
-  }
-  activate_chunk(v, e.act);
-  const long at = static_cast<long>(m) * e.ldo + n, from = static_cast<long>(m) * e.ld_add + n;
-  if constexpr (OUT_F32) {
-    float* out = static_cast<float*>(e.out) + at;
-    const float* add = static_cast<const float*>(e.add) + from;
-    if (whole) {
-      if (e.add) {
-        const float4 r = *reinterpret_cast<const float4*>(add);
-        v[0] += r.x; v[1] += r.y; v[2] += r.z; v[3] += r.w;
-      }
-      *reinterpret_cast<float4*>(out) = make_float4(v[0], v[1], v[2], v[3]);
+// Four columns of add as they lie in memory (WHOLE: aligned, all four exist; else one by one, the last again for those that
+// do not), and as floats.
+template <bool OUT_F32, bool WHOLE>
+struct Add4 {
+  float4 f;           // fp32
+  uint2 h;            // bf16, WHOLE
+  unsigned short s[4];  // bf16, one by one
+  __device__ __forceinline__ void load(const void* p, long at, int last) {
+    if constexpr (OUT_F32) {
+      const float* q = static_cast<const float*>(p) + at;
+      if constexpr (WHOLE) f = *reinterpret_cast<const float4*>(q);
+      else f = make_float4(q[0], q[min(1, last)], q[min(2, last)], q[min(3, last)]);
+    } else if constexpr (WHOLE) {
+      h = *reinterpret_cast<const uint2*>(static_cast<const bf16*>(p) + at);
     } else {
+      const unsigned short* q = static_cast<const unsigned short*>(p) + at;
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (n + j < a.N) out[j] = e.add ? v[j] + add[j] : v[j];
-    }
-  } else {
-    bf16* out = static_cast<bf16*>(e.out) + at;
-    const bf16* add = static_cast<const bf16*>(e.add) + from;
-    if (whole) {
-      if (e.add) {
-        const uint2 r = *reinterpret_cast<const uint2*>(add);
-        v[0] += __uint_as_float(r.x << 16);
-        v[1] += __uint_as_float(r.x & 0xffff0000u);
-        v[2] += __uint_as_float(r.y << 16);
-        v[3] += __uint_as_float(r.y & 0xffff0000u);
-      }
-      *reinterpret_cast<uint2*>(out) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
-    } else {
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (n + j < a.N) out[j] = __float2bfloat16_rn(e.add ? v[j] + __bfloat162float(add[j]) : v[j]);
+      for (int j = 0; j < 4; ++j) s[j] = q[min(j, last)];
     }
   }
+  __device__ __forceinline__ void zero() {
+    f = make_float4(0.f, 0.f, 0.f, 0.f);
+    h = make_uint2(0u, 0u);
+    s[0] = s[1] = s[2] = s[3] = 0;
+  }
+  __device__ __forceinline__ float4 get() const {
+    if constexpr (OUT_F32) return f;
+    else if constexpr (WHOLE)
+      return make_float4(__uint_as_float(h.x << 16), __uint_as_float(h.x & 0xffff0000u), __uint_as_float(h.y << 16),
+                         __uint_as_float(h.y & 0xffff0000u));
+    else
+      return make_float4(__uint_as_float(static_cast<uint32_t>(s[0]) << 16), __uint_as_float(static_cast<uint32_t>(s[1]) << 16),
+                         __uint_as_float(static_cast<uint32_t>(s[2]) << 16), __uint_as_float(static_cast<uint32_t>(s[3]) << 16));
+  }
+};
+
+// The columns of one epilogue thread: four, rows r0, r0 + rstep, ... of the tile.
+template <bool OUT_F32, bool WHOLE>
+struct Finisher {
+  static constexpr int GROUP = 4;  // rows at a time
+  Add4<OUT_F32, WHOLE> add[GROUP];
+  float bias[4];
+
+  // Rows behind the last are read as the last row again: without branches between them the loads are in flight together
+  // (eight one by one took 2500 cycles).
+  __device__ __forceinline__ void load(const void* p, long ld, int m0, int n, int first, int rstep, int rows, int last) {
+#pragma unroll
+    for (int i = 0; i < GROUP; ++i)
+      add[i].load(p, static_cast<long>(m0 + min(first + i * rstep, rows - 1)) * ld + n, last);
+  }
+  __device__ __forceinline__ void begin(const float* bias_at, const void* p, long ld, int m0, int n, int r0, int rstep, int rows,
+                                        int last) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) bias[j] = bias_at ? bias_at[n + min(j, last)] : 0.f;
+#pragma unroll
+    for (int i = 0; i < GROUP; ++i) add[i].zero();
+    if (p) load(p, ld, m0, n, r0, rstep, rows, last);
+  }
+  // Sums, bias and activation go back to shared memory row by row in a loop, then a group of rows gets its residual and
+  // leaves.  Loops, because this runs once per launch and instructions out of the cache are what it waits for (unrolled by eight
+  // rows and five activations, 200 KB of code, a single row took 1800 cycles).
+  __device__ __forceinline__ void run(float4* p4, int pitch, int split, int a_rows, int act, const void* p, long ld, void* out,
+                                      long ldo, int m0, int n, int r0, int rstep, int rows, int last) {
+#pragma unroll 1
+    for (int first = r0; first < rows; first += GROUP * rstep) {
+      if (first != r0 && p) load(p, ld, m0, n, first, rstep, rows, last);
+      const int end = min(rows, first + GROUP * rstep);
+#pragma unroll 1
+      for (int r = first; r < end; r += rstep) {
+        float4 s = p4[r * pitch];
+#pragma unroll 1
+        for (int k = 1; k < split; ++k) {
+          const float4 u = p4[(k * a_rows + r) * pitch];
+          s.x += u.x; s.y += u.y; s.z += u.z; s.w += u.w;
+        }
+        float v[4] = {s.x + bias[0], s.y + bias[1], s.z + bias[2], s.w + bias[3]};
+        activate_chunk(v, act);
+        p4[r * pitch] = make_float4(v[0], v[1], v[2], v[3]);
+      }
+#pragma unroll
+      for (int i = 0; i < GROUP; ++i) {
+        const int r = first + i * rstep;
+        if (r < rows) {
+          const float4 s = p4[r * pitch], u = add[i].get();
+          const float v[4] = {s.x + u.x, s.y + u.y, s.z + u.z, s.w + u.w};
+          const long at = static_cast<long>(m0 + r) * ldo + n;
+          if constexpr (OUT_F32) {
+            float* q = static_cast<float*>(out) + at;
+            if constexpr (WHOLE) *reinterpret_cast<float4*>(q) = make_float4(v[0], v[1], v[2], v[3]);
+            else
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                if (j <= last) q[j] = v[j];
+          } else {
+            bf16* q = static_cast<bf16*>(out) + at;
+            if constexpr (WHOLE) *reinterpret_cast<uint2*>(q) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
+            else
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                if (j <= last) q[j] = __float2bfloat16_rn(v[j]);
+          }
+        }
+      }
+    }
+  }
+};
+
+// v in a register from here on: the compiler cannot read it again from where it came
+template <typename T>
+__device__ __forceinline__ T pin(T v) {
+  if constexpr (sizeof(T) == 8) asm volatile("" : "+l"(v));
+  else asm volatile("" : "+r"(v));
+  return v;
+}
+
+__device__ __forceinline__ uint32_t tmem_columns(int wanted) {  // a power of two from 32
+  return wanted <= 64 ? 64 : wanted <= 128 ? 128 : wanted <= 256 ? 256 : 512;
 }
 
 template <int BN, bool OUT_F32>
@@ -108,9 +188,9 @@ linear_residual_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_con
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   // a stage: the W tile, then the rows of x (an MMA reads 128 of them: what lies behind the loaded ones gives accumulator
-  // rows that nobody stores; the last stage is followed by the partial sums, which are at least 16 KiB)
+  // rows that nobody stores; the last stage is followed by the partial sums)
   float* partial = reinterpret_cast<float*>(smem + a.stages * a.stage_bytes);
-  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + a.stages * a.stage_bytes + partial_bytes(a.split, a.cols));
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + a.stages * a.stage_bytes + partial_bytes(a.split, a.a_rows, a.cols));
   uint64_t* empty_bar = full_bar + LR_MAX_STAGES;
   uint64_t* tfull_bar = empty_bar + LR_MAX_STAGES;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tfull_bar + 1);
@@ -136,7 +216,7 @@ linear_residual_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_con
     prefetch_tmap(&tmW);
   }
   if (warp == 1) {
-    tmem_alloc(tmem_slot, BN);
+    tmem_alloc(tmem_slot, tmem_columns(a.accs * BN));
     tmem_relinquish();
   }
   tc_fence_before_sync();
@@ -146,20 +226,45 @@ linear_residual_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_con
   grid_dep_launch();
   const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_slot, 0);
   const WaitCtx wc{s_abort, a.status};
-  if (a.split > 1) cluster_sync_all();  // every CTA of the cluster runs before its shared memory is written to
+  // What the epilogue needs of the arguments, read now: the first access to a line of them costs a trip to L2 in every launch,
+  // one after the other where the compiler reads them as it goes.
+  void* out = pin(a.epi.out);
+  const void* addend = pin(a.epi.add);
+  const long ldo = pin(a.epi.ldo), ld_add = pin(a.epi.ld_add);
+  const int split = pin(a.split), cols = pin(a.cols), a_rows = pin(a.a_rows), act_of = pin(a.epi.act), N = pin(a.N);
+  if (split > 1) cluster_arrive();  // waited for before a CTA of the cluster is written to: it runs by then
+
+  // Epilogue threads: four columns each, rows r0, r0 + rstep, ...  The bias and the first rows of add are requested before
+  // the products are waited for.
+  const int et = static_cast<int>(threadIdx.x) - 64;
+  const int rows = min(LR_BM, a.M - m0);
+  const int quads = max(0, min(cols, BN - rank * cols)) / 4;
+  const int rstep = quads > 0 ? 32 * EPI_WARPS / quads : 1;
+  const int r0 = quads > 0 ? et / quads : LR_BM;
+  const int col = quads > 0 ? 4 * (et - r0 * quads) : 0;
+  const int n = n0 + rank * cols + col;
+  const bool works = et >= 0 && r0 < rstep && r0 < rows && n < N;
+  const int last = min(3, N - 1 - n);  // of its four columns
+  const bool whole = a.vec_store != 0 && last == 3;
+  Finisher<OUT_F32, true> vec;
+  Finisher<OUT_F32, false> odd;
 
   if (warp == 0) {
     // ------------------------------ TMA producer (a converged warp, one lane issues) ------
     const bool issuer = elect_one();
     int stage = 0;
     uint32_t phase = 0;
-    for (int kb = 0; kb < KB; ++kb) {
+    for (int kb = 0; kb < KB; kb += LR_SLOT) {
       if (!mbar_wait_all(&empty_bar[stage], phase ^ 1, wc, DEV_TIMEOUT_EMPTY)) break;
       if (issuer) {
         uint8_t* st = smem + stage * a.stage_bytes;
-        mbar_expect_tx(&full_bar[stage], W_BYTES + a.a_rows * LR_KBYTES);
-        tma_load_2d(st, &tmW, &full_bar[stage], (kb0 + kb) * (LR_KBYTES / 2), n0);
-        tma_load_2d(st + W_BYTES, &tmA, &full_bar[stage], (kb0 + kb) * (LR_KBYTES / 2), m0);
+        mbar_expect_tx(&full_bar[stage], min(LR_SLOT, KB - kb) * a.block_bytes);
+#pragma unroll
+        for (int i = 0; i < LR_SLOT; ++i)
+          if (kb + i < KB) {
+            tma_load_2d(st + i * a.block_bytes, &tmW, &full_bar[stage], (kb0 + kb + i) * (LR_KBYTES / 2), n0);
+            tma_load_2d(st + i * a.block_bytes + W_BYTES, &tmA, &full_bar[stage], (kb0 + kb + i) * (LR_KBYTES / 2), m0);
+          }
       }
       if (++stage == a.stages) { stage = 0; phase ^= 1; }
     }
@@ -167,61 +272,72 @@ linear_residual_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_con
     // ------------------------------ MMA issuer (a converged warp, one lane issues) ------
     const bool issuer = elect_one();
     const uint64_t desc0 = make_smem_desc_sw128(smem_u32(smem), 16, 1024);
-    int stage = 0;
-    uint32_t phase = 0;
-    for (int kb = 0; kb < KB; ++kb) {
+    int stage = 0, in_chunk = 0;
+    uint32_t phase = 0, d_tmem = tmem_base;
+    for (int kb = 0; kb < KB; kb += LR_SLOT) {
       if (!mbar_wait_all(&full_bar[stage], phase, wc, DEV_TIMEOUT_FULL)) break;
       tc_fence_after_sync();
-      if (issuer) {
-        const uint64_t w_desc = desc0 + static_cast<uint32_t>(stage * (a.stage_bytes >> 4));
-        const uint64_t a_desc = w_desc + (W_BYTES >> 4);
 #pragma unroll
-        for (int k = 0; k < LR_KBYTES / 32; ++k)
-          mma_f16_ss(tmem_base, a_desc + 2 * k, w_desc + 2 * k, IDESC, (kb | k) != 0);
+      for (int i = 0; i < LR_SLOT; ++i)
+        if (kb + i < KB) {
+          if (issuer) {
+            const uint64_t w_desc = desc0 + static_cast<uint32_t>((stage * a.stage_bytes + i * a.block_bytes) >> 4);
+            const uint64_t a_desc = w_desc + (W_BYTES >> 4);
+#pragma unroll
+            for (int k = 0; k < LR_KBYTES / 32; ++k)
+              mma_f16_ss(d_tmem, a_desc + 2 * k, w_desc + 2 * k, IDESC, (in_chunk | k) != 0);
+          }
+          if (++in_chunk == a.chunk) { in_chunk = 0; d_tmem += BN; }
+        }
+      if (issuer) {
         mma_commit(&empty_bar[stage]);
-        if (kb == KB - 1) mma_commit(tfull_bar);
+        if (kb + LR_SLOT >= KB) mma_commit(tfull_bar);
       }
       if (++stage == a.stages) { stage = 0; phase ^= 1; }
     }
   } else {
     // ------------------------------ accumulator -> partial sums of the cluster's CTAs ------
-    // warp w may read TMEM lanes [32 (w % 4), +32); warps 2-5 take the first half of the columns, warps 6-9 the second
-    const int quad = warp & 3, half = (warp - 2) >> 2;
+    // warp w may read TMEM lanes [32 (w % 4), +32); two warps share the columns of a quarter of the rows
+    const int quad = warp & 3, part = (warp - 2) >> 2;
+    constexpr int PART = BN / (EPI_WARPS / 4);
     const int row = quad * 32 + lane;
-    // bring this CTA's columns of add into L2 while the products run
-    if (a.epi.add) {
-      const int threads = 32 * EPI_WARPS, t = threadIdx.x - 64, esz = OUT_F32 ? 4 : 2;
-      const int m = m0 + t % LR_BM;
-      if (m < a.M)
-        for (int c = (t / LR_BM) * 32; c < a.cols; c += threads / LR_BM * 32) {
-          const int n = n0 + rank * a.cols + c;
-          if (n < a.N && rank * a.cols + c < BN)
-            asm volatile("prefetch.global.L2 [%0];" ::"l"(static_cast<const uint8_t*>(a.epi.add) +
-                                                           (static_cast<long>(m) * a.epi.ld_add + n) * esz));
-        }
+    if (works) {
+      if (whole) vec.begin(a.epi.bias, addend, ld_add, m0, n, r0, rstep, rows, last);
+      else odd.begin(a.epi.bias, addend, ld_add, m0, n, r0, rstep, rows, last);
     }
-    if (m0 + quad * 32 < a.M && mbar_wait_warp(tfull_bar, 0, wc, DEV_TIMEOUT_TMEM_FULL)) {
+    __syncwarp();
+    bool ok = m0 + quad * 32 < a.M && mbar_wait_warp(tfull_bar, 0, wc, DEV_TIMEOUT_TMEM_FULL);
+    if (split > 1) cluster_wait();
+    if (ok) {
       tc_fence_after_sync();
       const uint32_t t_row = tmem_base + (static_cast<uint32_t>(quad * 32) << 16);
       const bool live = m0 + row < a.M;
 #pragma unroll 1
-      for (int c = half * (BN / 2); c < (half + 1) * (BN / 2); c += 32) {
-        uint32_t r[32];
-        tmem_ld_32x32b_x32(t_row + c, r);
+      for (int c = part * PART; c < (part + 1) * PART; c += 16) {
+        uint32_t r[16];
+        tmem_ld_32x32b_x16(t_row + c, r);
         tmem_wait_ld();
-        if (live) {
-          int owner = c / a.cols, col = c - owner * a.cols;
+#pragma unroll 1
+        for (int i = 1; i * a.chunk < KB; ++i) {  // the accumulators that this CTA's K blocks reached
+          uint32_t u[16];
+          tmem_ld_32x32b_x16(t_row + i * BN + c, u);
+          tmem_wait_ld();
 #pragma unroll
-          for (int j = 0; j < 32; j += 4) {
-            float* dst = partial + (rank * LR_BM + row) * (a.cols + 4) + col;
-            if (a.split > 1)
+          for (int j = 0; j < 16; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) + __uint_as_float(u[j]));
+        }
+        if (live) {
+          int owner = c / cols, at = c - owner * cols;
+#pragma unroll
+          for (int j = 0; j < 16; j += 4) {
+            float* dst = partial + (rank * a_rows + row) * (cols + 4) + at;
+            if (split > 1)
               st_cluster_v4(map_to_cta(smem_u32(dst), owner), __uint_as_float(r[j]), __uint_as_float(r[j + 1]),
                             __uint_as_float(r[j + 2]), __uint_as_float(r[j + 3]));
             else
               *reinterpret_cast<float4*>(dst) = make_float4(__uint_as_float(r[j]), __uint_as_float(r[j + 1]),
                                                             __uint_as_float(r[j + 2]), __uint_as_float(r[j + 3]));
-            col += 4;
-            if (col == a.cols) { col = 0; ++owner; }
+            at += 4;
+            if (at == cols) { at = 0; ++owner; }
           }
         }
       }
@@ -230,28 +346,23 @@ linear_residual_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_con
 
   tc_fence_before_sync();
   __syncwarp();
-  if (a.split > 1) cluster_sync_all();  // the partial sums are complete; no CTA is written to after this
-  else __syncthreads();
+  if (split > 1) {
+    if (warp < 2) cluster_wait();
+    cluster_sync_all();  // the partial sums are complete; no CTA is written to after this
+  } else {
+    __syncthreads();
+  }
   if (*s_abort) drain_after_abort();
-  // ------------------------------ sum, bias, activation, residual, store: all threads ------
-  const int rows = min(LR_BM, a.M - m0);
-  const int quads = max(0, min(a.cols, BN - rank * a.cols)) / 4;
-  const int pitch = (a.cols + 4) / 4;
-  const float4* p4 = reinterpret_cast<const float4*>(partial);
-  for (int i = threadIdx.x; i < rows * quads; i += LR_THREADS) {
-    const int r = i / quads, q = i - r * quads;
-    const int n = n0 + rank * a.cols + 4 * q;
-    if (n >= a.N) continue;
-    float4 v = p4[r * pitch + q];
-    for (int s = 1; s < a.split; ++s) {
-      const float4 u = p4[(s * LR_BM + r) * pitch + q];
-      v.x += u.x; v.y += u.y; v.z += u.z; v.w += u.w;
-    }
-    finish4<OUT_F32>(a, m0 + r, n, v);
+  // ------------------------------ sum, bias, activation, residual, store ------
+  if (works) {
+    float4* p4 = reinterpret_cast<float4*>(partial) + col / 4;
+    const int pitch = (cols + 4) / 4;
+    if (whole) vec.run(p4, pitch, split, a_rows, act_of, addend, ld_add, out, ldo, m0, n, r0, rstep, rows, last);
+    else odd.run(p4, pitch, split, a_rows, act_of, addend, ld_add, out, ldo, m0, n, r0, rstep, rows, last);
   }
   if (warp == 1) {
     tc_fence_after_sync();
-    tmem_dealloc(tmem_base, BN);
+    tmem_dealloc(tmem_base, tmem_columns(a.accs * BN));
   }
 }
 
@@ -270,8 +381,9 @@ int launch_inst(const CUtensorMap& tmA, const CUtensorMap& tmW, const LinearArgs
       attr_done[dev] = true;
     }
   }
-  launch_dependent_cluster(kern, static_cast<unsigned>(a.tiles_m) * a.tiles_n * a.split, a.split, LR_THREADS, smem, stream,
-                           tmA, tmW, a);
+  const unsigned grid = static_cast<unsigned>(a.tiles_m) * a.tiles_n * a.split;
+  if (a.split > 1) launch_dependent_cluster(kern, grid, a.split, LR_THREADS, smem, stream, tmA, tmW, a);
+  else launch_dependent(kern, grid, LR_THREADS, smem, stream, tmA, tmW, a);
   return after_launch("linear_residual_kernel");
 }
 
@@ -284,7 +396,7 @@ int launch_linear_residual(const bf16* x, long lda, const bf16* w, long ldw, int
                        (!epi.add || ((epi.ld_add * esz) % 16 == 0 && (reinterpret_cast<uintptr_t>(epi.add) & 15) == 0));
   const int sms = device_sm_count();
   const int k_blocks = (K + 63) / 64;
-  const LinearPlan plan = linear_plan(M, N, k_blocks, tma_out, sms);
+  const LinearPlan plan = linear_plan(M, N, k_blocks, tma_out, epi.out_f32 != 0, sms);
   if (plan.pair) {
     GemmProblem q;
     q.A = x; q.lda = lda; q.W = w; q.ldw = ldw; q.M = M; q.epi = epi;
@@ -298,13 +410,18 @@ int launch_linear_residual(const bf16* x, long lda, const bf16* w, long ldw, int
   a.split = plan.split;
   a.cols = (plan.bn / 4 + a.split - 1) / a.split * 4;
   a.a_rows = M < LR_BM ? (M + 7) / 8 * 8 : LR_BM;
-  a.stage_bytes = (plan.bn + a.a_rows) * LR_KBYTES;
+  a.block_bytes = (plan.bn + a.a_rows) * LR_KBYTES;
+  a.stage_bytes = LR_SLOT * a.block_bytes;
   const int bars = (2 * LR_MAX_STAGES + 1) * 8 + 8;
-  const int room = LR_SMEM - 1024 - bars - partial_bytes(a.split, a.cols);
+  const int room = LR_SMEM - 1024 - bars - partial_bytes(a.split, a.a_rows, a.cols);
   a.stages = room / a.stage_bytes;
   if (a.stages > LR_MAX_STAGES) a.stages = LR_MAX_STAGES;
   const int most = (k_blocks + a.split - 1) / a.split;
-  if (a.stages > most) a.stages = most;
+  if (a.stages > (most + LR_SLOT - 1) / LR_SLOT) a.stages = (most + LR_SLOT - 1) / LR_SLOT;
+  // fp32 outputs: at most 8 K blocks an accumulator where tensor memory has room (launch_rules.h)
+  a.accs = epi.out_f32 ? (most + 7) / 8 : 1;
+  if (a.accs > 512 / plan.bn) a.accs = 512 / plan.bn;
+  a.chunk = (most + a.accs - 1) / a.accs;
   a.vec_store = (epi.ldo * esz) % (4 * esz) == 0 && (reinterpret_cast<uintptr_t>(epi.out) % (4 * esz)) == 0 &&
                 (!epi.add || ((epi.ld_add * esz) % (4 * esz) == 0 && (reinterpret_cast<uintptr_t>(epi.add) % (4 * esz)) == 0));
   a.epi = epi;
@@ -314,7 +431,7 @@ int launch_linear_residual(const bf16* x, long lda, const bf16* w, long ldw, int
   if (rc) return rc;
   rc = encode_tmap_2d(&tmW, w, 2, (uint64_t)K, (uint64_t)N, (uint64_t)ldw * 2, 64, plan.bn);
   if (rc) return rc;
-  const int smem = 1024 + a.stages * a.stage_bytes + partial_bytes(a.split, a.cols) + bars;
+  const int smem = 1024 + a.stages * a.stage_bytes + partial_bytes(a.split, a.a_rows, a.cols) + bars;
   if (plan.bn == 64)
     return epi.out_f32 ? launch_inst<64, true>(tmA, tmW, a, smem, stream) : launch_inst<64, false>(tmA, tmW, a, smem, stream);
   return epi.out_f32 ? launch_inst<128, true>(tmA, tmW, a, smem, stream) : launch_inst<128, false>(tmA, tmW, a, smem, stream);

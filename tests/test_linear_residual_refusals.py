@@ -37,16 +37,17 @@ def test_plan(tmp_path):
 #include <cstdio>
 int main() {
   const int sizes[] = {1, 2, 7, 8, 63, 64, 65, 127, 128, 129, 255, 256, 257, 700, 1536, 4096, 16384, 100000};
-  for (int M : sizes) for (int N : sizes) for (int K : sizes) for (int out = 0; out < 2; ++out) {
+  for (int M : sizes) for (int N : sizes) for (int K : sizes) for (int out = 0; out < 4; ++out) {
     const int kb = (K + 63) / 64;
-    const sd3::LinearPlan p = sd3::linear_plan(M, N, kb, out != 0, 148);
-    if (p.pair) { if (!out) return 1; continue; }
+    const sd3::LinearPlan p = sd3::linear_plan(M, N, kb, out % 2 != 0, out / 2 != 0, 148);
+    if (p.pair) { if (out % 2 == 0) return 1; continue; }
     if ((p.bn != 64 && p.bn != 128) || p.split < 1 || p.split > 8 || p.split > kb) return 2;
     const int cols = (p.bn / 4 + p.split - 1) / p.split * 4, a_rows = M < 128 ? (M + 7) / 8 * 8 : 128;
     if (cols * p.split < p.bn) return 3;
-    const int partial = p.split * 128 * (cols + 4) * 4, room = 227 * 1024 - 1024 - 208 - partial;
-    // two stages at least, and behind the last one the 16 KiB that an MMA may read
-    if (room / ((p.bn + a_rows) * 128) < 2 || partial < 16384) return 4;
+    int partial = p.split * a_rows * (cols + 4) * 4;
+    if (partial < 16384) partial = 16384;  // what an MMA may read behind the last stage
+    const int room = 227 * 1024 - 1024 - 208 - partial;
+    if (room / (2 * (p.bn + a_rows) * 128) < 2) return 4;  // two stages of two K blocks at least
   }
   std::puts("ok");
 }
