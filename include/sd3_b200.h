@@ -191,6 +191,22 @@ SD3_API int sd3_attention_bounded(const void* qkv_bf16, int B, int T, int num_he
                                   void* out_x_bf16, float scale, float score_bound, void* scratch,
                                   long scratch_bytes, void* stream);
 
+/* Attention over packed sequences of different lengths: row t of q, k, v and out is one token; sequence s owns the rows
+ * offsets[s] <= t < offsets[s + 1], offsets being count + 1 non-decreasing int32 row numbers in DEVICE memory, read by the kernel
+ * (they may be written by earlier work of the stream and change between replays of a captured graph).  A query sees the keys
+ * of its own sequence, with causal != 0 those up to its own place.  kv_heads divides heads; query head h uses key / value head
+ * h / (heads / kv_heads).  head_dim 64 or 128.  Head h of row t of q lies at q + t * ldq + h * head_dim, and so on: bf16, 16-byte
+ * aligned pointers, row strides multiples of 8 elements and at least heads * head_dim (kv_heads * head_dim), so that q, k and v may
+ * be slices of one buffer.  out overlaps none of them.  Sequences may be empty.  Rows of out that belong to no sequence (behind the
+ * last one of a padded batch) are left as they were.  Offsets outside [0, rows] are taken as the nearest row; sequences that
+ * overlap give undefined values.  What lies in other sequences' rows of q, k and v reaches no output, infinities and NaN included;
+ * within a sequence a value row that is not finite may also reach up to 127 earlier queries of a causal call.  rows or count may
+ * be 0.  Softmax and sums in fp32, the exponentials enter the second product as bf16.  Extends multihead_attention
+ * (modules.cpp:766-831), which has one length, as many key heads as query heads and no mask. */
+SD3_API int sd3_attention_packed(const void* q_bf16, long ldq, const void* k_bf16, long ldk, const void* v_bf16, long ldv,
+                                 void* out_bf16, long ldo, const int* offsets, int count, int rows, int heads, int kv_heads,
+                                 int head_dim, int causal, float scale, void* stream);
+
 /* Generic attention in fp32 arithmetic for any head_dim <= 128: q, k, v are
  * (B, Tq|Tk, num_heads*head_dim) row-major with leading dimension ld elements,
  * dtype in_dtype; out (B, Tq, num_heads*head_dim) of out_dtype.  Stand-in for

@@ -315,6 +315,44 @@ int sd3_attention_bounded(const void* qkv, int B, int T, int num_heads, int Tc, 
                                scratch_bytes > 0 ? static_cast<size_t>(scratch_bytes) : 0, score_bound);
 }
 
+int sd3_attention_packed(const void* q, long ldq, const void* k, long ldk, const void* v, long ldv, void* out, long ldo,
+                         const int* offsets, int count, int rows, int heads, int kv_heads, int head_dim, int causal, float scale,
+                         void* stream) {
+  if (count < 0 || rows < 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || heads > (1 << 16) ||
+      !(scale > 0.f && scale < 1e30f)) {
+    set_last_error("sd3_attention_packed: invalid argument (count %d rows %d heads %d kv_heads %d scale %g)", count, rows, heads,
+                   kv_heads, static_cast<double>(scale));
+    return SD3_ERR_INVALID_ARG;
+  }
+  if (head_dim != 64 && head_dim != 128) {
+    set_last_error("sd3_attention_packed: head_dim 64 or 128 expected, got %d", head_dim);
+    return SD3_ERR_UNSUPPORTED;
+  }
+  if (count == 0 || rows == 0) return SD3_OK;
+  const long wq = static_cast<long>(heads) * head_dim, wk = static_cast<long>(kv_heads) * head_dim;
+  if (!q || !k || !v || !out || !offsets || (reinterpret_cast<uintptr_t>(offsets) & 3) || ldq < wq || ldk < wk || ldv < wk ||
+      ldo < wq || out == q || out == k || out == v) {
+    set_last_error("sd3_attention_packed: null or misaligned pointer, or rows that overlap (ldq %ld ldk %ld ldv %ld ldo %ld)", ldq,
+                   ldk, ldv, ldo);
+    return SD3_ERR_INVALID_ARG;
+  }
+  if (((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) |
+        reinterpret_cast<uintptr_t>(out)) & 15) || ldq % 8 || ldk % 8 || ldv % 8 || ldo % 8) {
+    set_last_error("sd3_attention_packed: rows must be 16-byte aligned (ldq %ld ldk %ld ldv %ld ldo %ld)", ldq, ldk, ldv, ldo);
+    return SD3_ERR_UNSUPPORTED;
+  }
+  PackedAttention p;
+  p.q = static_cast<const bf16*>(q); p.k = static_cast<const bf16*>(k); p.v = static_cast<const bf16*>(v);
+  p.out = static_cast<bf16*>(out);
+  p.ldq = ldq; p.ldk = ldk; p.ldv = ldv; p.ldo = ldo;
+  p.offsets = offsets;
+  p.count = count; p.rows = rows;
+  p.heads = heads; p.kv_heads = kv_heads; p.head_dim = head_dim;
+  p.causal = causal != 0;
+  p.scale = scale;
+  return launch_attention_packed(p, status_word_for(S(stream)), S(stream));
+}
+
 int sd3_attention_generic(const void* q, const void* k, const void* v, long ld, int in_dtype,
                           int B, int T, int num_heads, int head_dim, void* out, long ldo,
                           int out_dtype, float scale, void* stream) {

@@ -1,0 +1,478 @@
+// Attention over packed sequences: the rows of q, k and v are the tokens of one sequence after the other, `offsets`
+// (count + 1 numbers in device memory) says where each begins; a query sees the keys of its own sequence, with `causal` those up
+// to its own place.  Several query heads may share a key / value head.  head_dim 64 and 128, bf16.
+//
+//   out[t, h] = sum_j p_j v[j, g],  p = softmax_j(scale q[t, h] . k[j, g]),  g = h / (heads / kv_heads)
+//
+// One CTA owns 128 queries of one (sequence, head), two CTAs share an SM and fill each other's waits: warp 0 streams K and V
+// tiles of 128 keys by TMA, warp 1 issues the MMAs, four softmax warps own a query row per thread.  As in
+// attention_tcgen05.cu the softmax is online per 64 keys, exponentials go to the MUFU unit and, one of eight, to the FMA pipe,
+// O is rescaled only when the maximum has moved by more than 2^8.
+//
+// Which tile a CTA takes is found on the device, from the offsets: their values may come from an earlier kernel and may change
+// between replays of a captured graph.  The grid has room for every way in which the rows can be cut into `count` sequences.
+// Tiles run in the order of their place in their sequence, the last first: with `causal` those are the long ones, and the
+// short ones fill the end.
+//
+// Only the last key tile of a query tile is masked: it holds the diagonal or the end of the sequence.  Keys behind the end are the
+// next sequence's: their scores become -inf, and their rows of V zeros, because 0 * inf is not 0.
+#include <cuda.h>
+
+#include <mutex>
+
+#include "attention_softmax.cuh"
+#include "kernels.h"
+#include "ptx.cuh"
+
+namespace sd3 {
+
+int device_sm_count();
+int encode_tmap_3d(CUtensorMap* map, const void* base, int elem_bytes, uint64_t d0, uint64_t d1, uint64_t d2,
+                   uint64_t stride1_bytes, uint64_t stride2_bytes, uint32_t box0, uint32_t box1, uint32_t box2);
+
+namespace {
+
+using namespace softmax_detail;
+
+constexpr int AP_BM = 128;                    // queries per CTA
+constexpr int AP_BN = 128;                    // keys per tile
+constexpr int AP_SUB_BYTES = AP_BN * 64 * 2;  // 128 rows x 64 values in the 128-byte swizzle: 16 KiB
+constexpr int AP_THREADS = 192;
+constexpr int AP_TMEM_COLS = 256;
+constexpr int AP_SCAN_CHUNKS = 8;  // up to 256 sequences are put in order of length
+// head_dim 64: scores, P and O side by side (128 + 64 + 64 columns), K and V rings of two tiles.  head_dim 128: O takes 128
+// columns, P lies over the scores it was made from, and one tile each of K and V leaves room for two CTAs an SM.
+template <int D>
+struct ApCfg {
+  static constexpr int SUBS = D / 64;
+  static constexpr int TILE_BYTES = SUBS * AP_SUB_BYTES;
+  static constexpr int STAGES = D == 64 ? 2 : 1;
+  static constexpr bool P_OVER_S = D == 128;
+  static constexpr int P_COL = P_OVER_S ? 0 : 128;
+  static constexpr int O_COL = D == 64 ? 192 : 128;
+  static constexpr int SMEM_BYTES = (1 + 2 * STAGES) * TILE_BYTES + 256 + 1024;
+};
+
+struct PackedArgs {
+  const int* offsets;
+  int count, rows;  // sequences; rows of q, k, v and out
+  int heads, group;
+  long ldo;
+  bf16* out;
+  float scale_log2e;
+  int causal;
+  int* status;
+};
+
+struct Unit {
+  int begin, len, q0;  // the sequence's first row and length; the tile's first query in it (q0 < 0: nothing to do)
+};
+
+__device__ __forceinline__ Unit sequence_at(const PackedArgs& a, int s) {
+  Unit u;
+  u.begin = min(max(a.offsets[s], 0), a.rows);
+  u.len = min(max(a.offsets[s + 1], u.begin), a.rows) - u.begin;
+  u.q0 = -1;
+  return u;
+}
+__device__ __forceinline__ int tiles_of(const PackedArgs& a, int s) {
+  return s < a.count ? (sequence_at(a, s).len + AP_BM - 1) / AP_BM : 0;
+}
+
+// The tile of rank `rank`, for a converged warp.
+__device__ Unit find_unit(const PackedArgs& a, int rank) {
+  const int lane = threadIdx.x & 31;
+  Unit none;
+  none.begin = none.len = 0;
+  none.q0 = -1;
+  if (a.count <= 32 * AP_SCAN_CHUNKS) {
+    // by place in the sequence, the highest first, then by sequence: tiles at place >= p number cnt(p) = sum max(0, n_s - p)
+    const int chunks = (a.count + 31) / 32;
+    int n[AP_SCAN_CHUNKS], most = 0;
+#pragma unroll
+    for (int i = 0; i < AP_SCAN_CHUNKS; ++i) {
+      n[i] = i < chunks ? tiles_of(a, 32 * i + lane) : 0;
+      most = max(most, n[i]);
+    }
+    auto cnt = [&](int p) {
+      int c = 0;
+#pragma unroll
+      for (int i = 0; i < AP_SCAN_CHUNKS; ++i) c += max(0, n[i] - p);
+      return __reduce_add_sync(0xffffffffu, c);
+    };
+    int lo = 0, hi = __reduce_max_sync(0xffffffffu, most);
+    if (rank >= cnt(0)) return none;
+    while (hi - lo > 1) {  // cnt(lo) > rank >= cnt(hi)
+      const int mid = (lo + hi) >> 1;
+      if (cnt(mid) > rank) lo = mid;
+      else hi = mid;
+    }
+    int r = rank - cnt(lo + 1);
+#pragma unroll
+    for (int i = 0; i < AP_SCAN_CHUNKS; ++i) {
+      const unsigned has = __ballot_sync(0xffffffffu, n[i] > lo);
+      if (r < __popc(has)) {
+        Unit u = sequence_at(a, 32 * i + static_cast<int>(__fns(has, 0, r + 1)));
+        u.q0 = lo * AP_BM;
+        return u;
+      }
+      r -= __popc(has);
+    }
+    return none;
+  }
+  // many sequences: one after the other, each from its last tile on
+  int before = 0;
+  for (int s0 = 0; s0 < a.count; s0 += 32) {
+    const int n = tiles_of(a, s0 + lane);
+    int upto = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int t = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += t;
+    }
+    const int all = __shfl_sync(0xffffffffu, upto, 31);
+    if (rank < before + all) {
+      const int src = __popc(__ballot_sync(0xffffffffu, before + upto <= rank));  // the first lane past rank
+      Unit u = sequence_at(a, s0 + src);
+      u.q0 = (before + __shfl_sync(0xffffffffu, upto, src) - 1 - rank) * AP_BM;
+      return u;
+    }
+    before += all;
+  }
+  return none;
+}
+
+// O *= alpha for this thread's query row.  Rare, so it is kept out of line.
+template <int D>
+__device__ __noinline__ void rescale_row(uint32_t o_tmem, float alpha) {
+  tc_fence_after_sync();
+  uint32_t o0[16];
+#pragma unroll 1
+  for (int part = 0; part < D / 16; ++part) {
+    tmem_ld_32x32b_x16(o_tmem + 16 * part, o0);
+    tmem_wait_ld();
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o0[i] = __float_as_uint(__uint_as_float(o0[i]) * alpha);
+    tmem_st_32x32b_x16(o_tmem + 16 * part, o0);
+  }
+  tmem_wait_st();
+}
+
+template <int D>
+__global__ void __launch_bounds__(AP_THREADS, 2)
+attention_packed_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+                        const __grid_constant__ CUtensorMap tmV, const __grid_constant__ PackedArgs a) {
+  using Cfg = ApCfg<D>;
+  constexpr int STAGES = Cfg::STAGES, SUBS = Cfg::SUBS, TILE = Cfg::TILE_BYTES;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint8_t* q_smem = smem;
+  uint8_t* k_smem = smem + TILE;
+  uint8_t* v_smem = k_smem + STAGES * TILE;
+  uint64_t* q_full = reinterpret_cast<uint64_t*>(v_smem + STAGES * TILE);
+  uint64_t* k_full = q_full + 1;          // STAGES
+  uint64_t* v_full = k_full + STAGES;     // STAGES
+  uint64_t* s_full = v_full + STAGES;     // STAGES: scores of the tile in this stage complete (its K is free)
+  uint64_t* pv_done = s_full + STAGES;    // STAGES: products of the tile in this stage complete (V and P free, O quiescent)
+  uint64_t* s_free = pv_done + STAGES;    // 1: scores pulled into registers (4 arrivals); not used with P over S
+  uint64_t* p_ready = s_free + 1;         // 1: P of the tile stored (4 arrivals)
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(p_ready + 1);
+  int* s_abort = reinterpret_cast<int*>(tmem_slot + 1);
+  int* s_unit = s_abort + 1;  // 3
+
+  const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0);  // known uniform
+  const int lane = threadIdx.x & 31;
+  const int h = static_cast<int>(blockIdx.x) % a.heads;
+
+  if (threadIdx.x == 32) {
+    mbar_init(q_full, 1);
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(&k_full[s], 1);
+      mbar_init(&v_full[s], 1);
+      mbar_init(&s_full[s], 1);
+      mbar_init(&pv_done[s], 1);
+    }
+    mbar_init(s_free, 4);
+    mbar_init(p_ready, 4);
+    *s_abort = 0;
+    fence_barrier_init();
+    prefetch_tmap(&tmQ);
+    prefetch_tmap(&tmK);
+    prefetch_tmap(&tmV);
+  }
+  __syncwarp();
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, AP_TMEM_COLS);
+    tmem_relinquish();
+  }
+  grid_dep_wait();  // the offsets may be the work of the preceding kernel
+  grid_dep_launch();
+  if (warp == 0) {
+    const Unit u = find_unit(a, static_cast<int>(blockIdx.x) / a.heads);
+    if (lane == 0) {
+      s_unit[0] = u.begin;
+      s_unit[1] = u.len;
+      s_unit[2] = u.q0;
+    }
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_slot, 0);
+  const WaitCtx wc{s_abort, a.status};
+  const int begin = __shfl_sync(0xffffffffu, s_unit[0], 0), len = __shfl_sync(0xffffffffu, s_unit[1], 0);
+  const int q0 = __shfl_sync(0xffffffffu, s_unit[2], 0);
+  const int keys = a.causal ? min(len, q0 + AP_BM) : len;  // that this tile's queries see
+  const int nkv = q0 < 0 ? 0 : (keys + AP_BN - 1) / AP_BN;  // at least one for a tile that exists
+
+  if (nkv == 0) {
+    // no such tile: the rows hold fewer than the grid has room for
+  } else if (warp == 0) {
+    // ------------------------------ TMA producer (a converged warp, one lane issues) ------
+    const bool issuer = elect_one();
+    const int g = h / a.group;
+    auto load = [&](const CUtensorMap* tm, uint8_t* to, uint64_t* bar, int head, int row) {
+      mbar_expect_tx(bar, TILE);
+#pragma unroll
+      for (int s = 0; s < SUBS; ++s) tma_load_3d(to + s * AP_SUB_BYTES, tm, bar, 64 * s, head, row);
+    };
+    if (issuer) load(&tmQ, q_smem, q_full, h, begin + q0);
+    for (int j = 0; j < nkv; ++j) {
+      const int st = j % STAGES;
+      const uint32_t prev = ((j / STAGES) + 1) & 1;  // parity of this stage's previous use
+      if (j >= STAGES && !mbar_wait_all(&s_full[st], prev, wc, DEV_TIMEOUT_ATTN_KV)) break;
+      if (issuer) load(&tmK, k_smem + st * TILE, &k_full[st], g, begin + j * AP_BN);
+      if (j >= STAGES && !mbar_wait_all(&pv_done[st], prev, wc, DEV_TIMEOUT_ATTN_KV)) break;
+      if (issuer) load(&tmV, v_smem + st * TILE, &v_full[st], g, begin + j * AP_BN);
+    }
+  } else if (warp == 1) {
+    // ------------------------------ MMA issuer (a converged warp, one lane issues) ------
+    constexpr uint32_t IDESC_S = make_idesc(1, 1, AP_BM, AP_BN, 0, 0);  // Q K^T, both K-major
+    constexpr uint32_t IDESC_O = make_idesc(1, 1, AP_BM, D, 0, 1);      // P V, V is MN-major
+    const uint64_t q_desc = make_smem_desc_sw128(smem_u32(q_smem), 16, 1024);
+    const uint64_t k_desc0 = make_smem_desc_sw128(smem_u32(k_smem), 16, 1024);
+    const uint64_t v_desc0 = make_smem_desc_sw128(smem_u32(v_smem), AP_SUB_BYTES, 1024);
+    const bool issuer = elect_one();
+    auto issue_s = [&](int j) {
+      const int st = j % STAGES;
+      if (!mbar_wait_all(&k_full[st], (j / STAGES) & 1, wc, DEV_TIMEOUT_ATTN_KV)) return false;
+      tc_fence_after_sync();
+      if (issuer) {
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) {  // 16 of head_dim: 32 bytes of a 128-byte row, four to a 64-wide subtile
+          const uint64_t adv = static_cast<uint64_t>(((k / 4) * AP_SUB_BYTES + (k % 4) * 32) >> 4);
+          mma_f16_ss(tmem_base, q_desc + adv, k_desc0 + static_cast<uint32_t>(st * (TILE >> 4)) + adv, IDESC_S, k != 0);
+        }
+        mma_commit(&s_full[st]);
+      }
+      return true;
+    };
+    auto issue_pv = [&](int j) {
+      const int st = j % STAGES;
+      if (!mbar_wait_all(&v_full[st], (j / STAGES) & 1, wc, DEV_TIMEOUT_ATTN_KV)) return false;
+      if (!mbar_wait_all(p_ready, j & 1, wc, DEV_TIMEOUT_ATTN_P)) return false;
+      tc_fence_after_sync();
+      if (issuer) {
+#pragma unroll
+        for (int k = 0; k < AP_BN / 16; ++k)  // 16 keys: 8 columns of bf16 pairs, 16 rows of V (128 bytes each)
+          mma_f16_ts(tmem_base + Cfg::O_COL, tmem_base + Cfg::P_COL + 8 * k,
+                     v_desc0 + static_cast<uint32_t>(st * (TILE >> 4)) + static_cast<uint64_t>((k * 16 * 128) >> 4), IDESC_O,
+                     (j != 0 || k != 0));
+        mma_commit(&pv_done[st]);
+      }
+      return true;
+    };
+    bool ok = mbar_wait_all(q_full, 0, wc, DEV_TIMEOUT_ATTN_Q);
+    for (int j = 0; j <= nkv && ok; ++j) {
+      if constexpr (Cfg::P_OVER_S) {
+        // the scores of tile j take the place of P of tile j - 1
+        if (j >= 1) ok = issue_pv(j - 1);
+        if (ok && j >= 1 && j < nkv)
+          ok = mbar_wait_all(&pv_done[(j - 1) % STAGES], ((j - 1) / STAGES) & 1, wc, DEV_TIMEOUT_ATTN_O);
+        if (ok && j < nkv) ok = issue_s(j);
+      } else {
+        // the softmax warps have pulled the scores of tile j - 1 into registers
+        if (j >= 1 && j < nkv) ok = mbar_wait_all(s_free, (j - 1) & 1, wc, DEV_TIMEOUT_ATTN_S);
+        if (ok && j < nkv) ok = issue_s(j);
+        if (ok && j >= 1) ok = issue_pv(j - 1);
+      }
+    }
+  } else {
+    // ------------------------------ softmax + epilogue ------------------------
+    const int quad = warp & 3;
+    const int row = quad * 32 + lane;
+    const uint32_t lane_base = tmem_base + (static_cast<uint32_t>(quad * 32) << 16);
+    const uint32_t s_tmem = lane_base, p_tmem = lane_base + Cfg::P_COL, o_tmem = lane_base + Cfg::O_COL;
+    const float c = a.scale_log2e;
+    const int seen = a.causal ? min(len, q0 + row + 1) : len;  // keys that this row sees, at least one
+    float m_used = -INFINITY;  // running maximum (raw score units) that the exponentials refer to
+    float2 l2 = make_float2(0.f, 0.f);
+    bool ok = true;
+    uint32_t pre_s = 0;  // early test of s_full for the coming tile
+    uint32_t ra[32], rb[32], rc[32], rd[32];
+    for (int j = 0; j < nkv; ++j) {
+      const int st = j % STAGES;
+      const int kv0 = j * AP_BN;
+      const bool masked = j == nkv - 1;
+      const int stp = (j + STAGES - 1) % STAGES;                      // stage and parity of the
+      const uint32_t parp = j >= 1 ? ((j - 1) / STAGES) & 1 : 0;      // previous tile's products
+      if (!mbar_wait_pre(pre_s, &s_full[st], (j / STAGES) & 1, wc, DEV_TIMEOUT_ATTN_S)) { ok = false; break; }
+      tc_fence_after_sync();
+      auto half_step = [&](uint32_t (&r0)[32], uint32_t (&r1)[32], bool second) {
+        const float mx = max_of2(r0, r1);
+        const bool need = (mx - m_used) * c > 8.0f;  // always true in the very first half (m_used = -inf)
+        if (__any_sync(0xffffffffu, need)) {
+          float alpha = 1.0f;
+          if (need) {
+            alpha = ex2_approx((m_used - mx) * c);
+            m_used = mx;
+            l2.x *= alpha;
+            l2.y *= alpha;
+          }
+          if (j >= 1 && ok) {
+            // with P over S the scores of this tile were issued after these products were complete
+            if (!Cfg::P_OVER_S) ok = mbar_wait_warp(&pv_done[stp], parp, wc, DEV_TIMEOUT_ATTN_O);
+            if (ok) rescale_row<D>(o_tmem, alpha);
+          }
+          if (second) {  // the first half of P was formed against the older maximum
+            scale_packed(ra, alpha);
+            scale_packed(rb, alpha);
+          }
+        }
+        const float nmc = -m_used * c;
+        if (masked) {
+          exp_pack<false>(r0, c, nmc, l2);
+          exp_pack<false>(r1, c, nmc, l2);
+        } else {
+          exp_pack(r0, c, nmc, l2);
+          exp_pack(r1, c, nmc, l2);
+        }
+      };
+      tmem_ld_32x32b_x32(s_tmem, ra);
+      tmem_ld_32x32b_x32(s_tmem + 32, rb);
+      tmem_wait_ld();
+      if (masked) { mask_cols(ra, kv0, seen); mask_cols(rb, kv0 + 32, seen); }
+      half_step(ra, rb, false);
+      // the second half is only loaded now: with all 128 scores live the kernel spills
+      tmem_ld_32x32b_x32(s_tmem + 64, rc);
+      tmem_ld_32x32b_x32(s_tmem + 96, rd);
+      tmem_wait_ld();
+      __syncwarp();
+      if (!Cfg::P_OVER_S) mbar_arrive_lane0(s_free, lane);  // the score buffer can take the next tile
+      if (masked) { mask_cols(rc, kv0 + 64, seen); mask_cols(rd, kv0 + 96, seen); }
+      uint32_t pre_pv = 1;
+      if (!Cfg::P_OVER_S && j >= 1) pre_pv = mbar_test_wait(&pv_done[stp], parp);
+      half_step(rc, rd, true);
+      // P is free once the products of the previous tile are complete (tested half a tile ago)
+      if (!Cfg::P_OVER_S && j >= 1 && ok) ok = mbar_wait_pre(pre_pv, &pv_done[stp], parp, wc, DEV_TIMEOUT_ATTN_O);
+      if (!ok) break;
+      tmem_st_32x32b_x16(p_tmem, reinterpret_cast<uint32_t(&)[16]>(ra));
+      tmem_st_32x32b_x16(p_tmem + 16, reinterpret_cast<uint32_t(&)[16]>(rb));
+      tmem_st_32x32b_x16(p_tmem + 32, reinterpret_cast<uint32_t(&)[16]>(rc));
+      tmem_st_32x32b_x16(p_tmem + 48, reinterpret_cast<uint32_t(&)[16]>(rd));
+      if (masked && kv0 + AP_BN > len) {
+        // rows of V behind the sequence's end become zeros, whatever they are
+        ok = mbar_wait_warp(&v_full[st], (j / STAGES) & 1, wc, DEV_TIMEOUT_ATTN_KV);
+        if (ok && kv0 + row >= len) {
+#pragma unroll
+          for (int s = 0; s < SUBS; ++s)
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              *reinterpret_cast<uint4*>(v_smem + st * TILE + s * AP_SUB_BYTES + row * 128 + i * 16) = make_uint4(0, 0, 0, 0);
+        }
+        fence_proxy_async_smem();
+      }
+      pre_s = 0;
+      if (j + 1 < nkv) pre_s = mbar_test_wait(&s_full[(j + 1) % STAGES], ((j + 1) / STAGES) & 1);
+      tmem_wait_st();
+      tc_fence_before_sync();
+      __syncwarp();
+      mbar_arrive_lane0(p_ready, lane);
+    }
+    const float l = l2.x + l2.y;
+    if (ok && mbar_wait_warp(&pv_done[(nkv - 1) % STAGES], ((nkv - 1) / STAGES) & 1, wc, DEV_TIMEOUT_ATTN_O)) {
+      tc_fence_after_sync();
+      const float inv = 1.0f / l;
+      uint4* to = reinterpret_cast<uint4*>(a.out + static_cast<long>(begin + q0 + row) * a.ldo + h * D);
+#pragma unroll 1
+      for (int part = 0; part < D / 32; ++part) {
+        uint32_t o[32];
+        tmem_ld_32x32b_x32(o_tmem + 32 * part, o);
+        tmem_wait_ld();
+        if (q0 + row < len) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            uint4 u;
+            u.x = pack_bf16x2(__uint_as_float(o[8 * i]) * inv, __uint_as_float(o[8 * i + 1]) * inv);
+            u.y = pack_bf16x2(__uint_as_float(o[8 * i + 2]) * inv, __uint_as_float(o[8 * i + 3]) * inv);
+            u.z = pack_bf16x2(__uint_as_float(o[8 * i + 4]) * inv, __uint_as_float(o[8 * i + 5]) * inv);
+            u.w = pack_bf16x2(__uint_as_float(o[8 * i + 6]) * inv, __uint_as_float(o[8 * i + 7]) * inv);
+            to[4 * part + i] = u;
+          }
+        }
+      }
+    }
+  }
+
+  // ------------------------------ teardown ------------------------------------
+  tc_fence_before_sync();
+  __syncthreads();
+  if (*s_abort) drain_after_abort();
+  if (warp == 1) {
+    tc_fence_after_sync();
+    tmem_dealloc(tmem_base, AP_TMEM_COLS);
+  }
+}
+
+template <int D>
+int launch_inst(const CUtensorMap* tm, const PackedArgs& a, long units, cudaStream_t stream) {
+  auto kern = attention_packed_kernel<D>;
+  static std::mutex attr_mutex;
+  static bool attr_done[64] = {false};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev >= 0 && dev < 64) {
+    std::lock_guard<std::mutex> lock(attr_mutex);
+    if (!attr_done[dev]) {
+      cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, ApCfg<D>::SMEM_BYTES);
+      if (e != cudaSuccess) return check_cuda(e, "cudaFuncSetAttribute(attention_packed)");
+      attr_done[dev] = true;
+    }
+  }
+  launch_dependent(kern, static_cast<unsigned>(units * a.heads), AP_THREADS, ApCfg<D>::SMEM_BYTES, stream, tm[0], tm[1], tm[2], a);
+  return after_launch("attention_packed_kernel");
+}
+
+}  // namespace
+
+int launch_attention_packed(const PackedAttention& p, int* dev_status, cudaStream_t stream) {
+  // every way to cut `rows` rows into `count` sequences has at most this many tiles
+  const long units = (static_cast<long>(p.rows) + static_cast<long>(AP_BM - 1) * p.count) / AP_BM;
+  if (units * p.heads > 0x7fffffffL) {
+    set_last_error("attention_packed: %ld tiles of %d heads are too many for one launch", units, p.heads);
+    return ST_UNSUPPORTED;
+  }
+  CUtensorMap tm[3];
+  const bf16* base[3] = {p.q, p.k, p.v};
+  const long ld[3] = {p.ldq, p.ldk, p.ldv};
+  for (int i = 0; i < 3; ++i) {
+    int rc = encode_tmap_3d(&tm[i], base[i], 2, static_cast<uint64_t>(p.head_dim),
+                            static_cast<uint64_t>(i == 0 ? p.heads : p.kv_heads), static_cast<uint64_t>(p.rows),
+                            static_cast<uint64_t>(p.head_dim) * 2, static_cast<uint64_t>(ld[i]) * 2, 64, 1, AP_BM);
+    if (rc) return rc;
+  }
+  PackedArgs a;
+  a.offsets = p.offsets;
+  a.count = p.count;
+  a.rows = p.rows;
+  a.heads = p.heads;
+  a.group = p.heads / p.kv_heads;
+  a.ldo = p.ldo;
+  a.out = p.out;
+  a.scale_log2e = p.scale * 1.4426950408889634f;
+  a.causal = p.causal;
+  a.status = dev_status;
+  return p.head_dim == 64 ? launch_inst<64>(tm, a, units, stream) : launch_inst<128>(tm, a, units, stream);
+}
+
+}  // namespace sd3

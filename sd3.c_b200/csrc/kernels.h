@@ -214,6 +214,20 @@ struct AttnProblem {
 };
 int launch_attention_group(const AttnProblem* p, int n, int B, int NH, int* dev_status, cudaStream_t stream);
 
+// Attention over packed sequences (attention_packed.cu): row t, head h of q at q + t * ldq + h * head_dim, and so on; out like q.
+// offsets: count + 1 row numbers in device memory.  head_dim 64 or 128; heads a multiple of kv_heads.
+struct PackedAttention {
+  const bf16 *q, *k, *v;
+  bf16* out;
+  long ldq, ldk, ldv, ldo;
+  const int* offsets;
+  int count, rows;
+  int heads, kv_heads, head_dim;
+  int causal;
+  float scale;
+};
+int launch_attention_packed(const PackedAttention& p, int* dev_status, cudaStream_t stream);
+
 // fp32 attention for head_dim 64 on the tensor cores.  qkv: three bf16 planes (split3.cuh) of
 // (B, T, 3E), B * T * 3E elements apart; outputs split by rows like above, as three planes of
 // B * Tc * E (out_c, may be null) and B * (T - Tc) * E (out_x) elements.

@@ -490,6 +490,48 @@ Tensor mha(Tensor& Q, Tensor& K, Tensor& V, int num_heads) {
   return out;
 }
 
+// (tokens, heads, head_dim) with the heads of a token next to each other: its row stride; anything else is copied
+Tensor tokens_of(const Tensor& t, const char* name) {
+  TORCH_CHECK(t.is_cuda(), "custom_modules: '", name, "' must be a CUDA tensor (this build has no CPU path)");
+  TORCH_CHECK(t.dim() == 3 && t.scalar_type() == torch::kBFloat16, "mha_packed: bfloat16 ", name,
+              " (tokens, heads, head_dim) expected");
+  const int64_t H = t.size(1), D = t.size(2);
+  const bool rows = t.stride(2) == 1 && (H == 1 || t.stride(1) == D) &&
+                    (t.size(0) <= 1 || (t.stride(0) >= H * D && t.stride(0) % 8 == 0)) &&
+                    reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+  return rows ? t : t.clone(at::MemoryFormat::Contiguous);
+}
+long token_stride(const Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(1) * t.size(2); }
+
+// mha_packed(q (T, heads, D), k, v (T, kv_heads, D) bf16, offsets (count + 1) int32 on the device, causal, scale, out)
+//   -> (T, heads, D).  scale: None for D^-0.5.  out: optional; rows of no sequence are left as they were in it (in an output
+// of the call's own they hold nothing in particular).
+Tensor mha_packed(const Tensor& q_in, const Tensor& k_in, const Tensor& v_in, const Tensor& offsets, bool causal,
+                  c10::optional<double> scale, const c10::optional<Tensor>& out_in) {
+  TORCH_CHECK(q_in.is_cuda(), "custom_modules: 'q' must be a CUDA tensor (this build has no CPU path)");
+  c10::cuda::CUDAGuard guard(q_in.device());
+  Tensor q = tokens_of(q_in, "q"), k = tokens_of(k_in, "k"), v = tokens_of(v_in, "v");
+  TORCH_CHECK(k.device() == q.device() && v.device() == q.device() && k.sizes() == v.sizes() && k.size(0) == q.size(0) &&
+                  k.size(2) == q.size(2) && k.size(1) > 0 && q.size(1) > 0 && q.size(1) % k.size(1) == 0,
+              "mha_packed: k and v (T, kv_heads, D) next to q (T, heads, D) expected, heads a multiple of kv_heads");
+  TORCH_CHECK(offsets.device() == q.device() && offsets.scalar_type() == torch::kInt32 && offsets.dim() == 1 &&
+                  offsets.numel() >= 1 && offsets.is_contiguous(),
+              "mha_packed: offsets must be contiguous int32 row numbers on q's device, one more than there are sequences");
+  TORCH_CHECK(q.size(0) < (1ll << 31) && q.size(1) <= 65536, "mha_packed: fewer than 2^31 rows and at most 65536 heads expected");
+  Tensor out = out_in ? *out_in : torch::empty({q.size(0), q.size(1), q.size(2)}, q.options());
+  if (out_in) {
+    TORCH_CHECK(out.device() == q.device() && out.sizes() == q.sizes() && out.scalar_type() == torch::kBFloat16,
+                "mha_packed: out must be bfloat16 of q's shape on its device");
+    TORCH_CHECK(tokens_of(out, "out").data_ptr() == out.data_ptr(), "mha_packed: out must have 16-byte aligned rows of whole heads");
+  }
+  const int D = (int)q.size(2);
+  ok(sd3_attention_packed(q.data_ptr(), token_stride(q), k.data_ptr(), token_stride(k), v.data_ptr(), token_stride(v), out.data_ptr(),
+                          token_stride(out), offsets.data_ptr<int>(), (int)offsets.numel() - 1, (int)q.size(0), (int)q.size(1),
+                          (int)k.size(1), D, causal, scale ? (float)*scale : 1.0f / std::sqrt((float)D), stream()),
+     "sd3_attention_packed");
+  return out;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -505,6 +547,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("sinusoidal_embedding", &sinusoidal_embedding, "Temporal sinusoidal embeddings");
   m.def("positional_embedding", &positional_embedding2D_forward, "2D positional embeddings");
   m.def("mha", &mha, "multi-head self attention");
+  m.def("mha_packed", &mha_packed, "attention over packed sequences, causal or not, with grouped heads", pybind11::arg("q"),
+        pybind11::arg("k"), pybind11::arg("v"), pybind11::arg("offsets"), pybind11::arg("causal") = false,
+        pybind11::arg("scale") = pybind11::none(), pybind11::arg("out") = pybind11::none());
   m.def("mlp", &MLP, "MLP");
   m.def("Dit_block", &DiT_block_forward_cuda, "Stable diffusion's DiT block");
   m.def("DiT", &DiT_forward, "SD3.5 medium");

@@ -73,6 +73,7 @@ PROTOTYPES = {
     "sd3_attention_scratch_bytes": (c_long, [c_int, c_int, c_int]),
     "sd3_attention_ws": (c_int, [c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_float, c_void_p, c_long, c_void_p]),
     "sd3_attention_bounded": (c_int, [c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_float, c_float, c_void_p, c_long, c_void_p]),
+    "sd3_attention_packed": (c_int, [c_void_p, c_long, c_void_p, c_long, c_void_p, c_long, c_void_p, c_long, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_void_p]),
     "sd3_attention_generic": (c_int, [c_void_p, c_void_p, c_void_p, c_long, c_int, c_int, c_int, c_int, c_int, c_void_p, c_long, c_int, c_float, c_void_p]),
     "sd3_cross_attention": (c_int, [c_void_p, c_void_p, c_void_p, c_long, c_long, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p, c_long, c_int, c_float, c_void_p]),
     "sd3_conv2d": (c_int, [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p]),
@@ -326,6 +327,41 @@ def attention_generic(q, k, v, num_heads, scale=None, out_dtype=None):
     check(lib().sd3_attention_generic(ptr(q), ptr(k), ptr(v), C, dtype_tag(q), B, T, num_heads, D,
                                       ptr(out), C, dtype_tag(out), scale, stream_ptr()),
           "sd3_attention_generic")
+    return out
+
+
+def _tokens(t, what):
+    """Row stride of a (tokens, heads, head_dim) tensor whose tokens hold their heads one after the other."""
+    torch = _torch()
+    if t.dim() != 3 or not t.is_cuda or t.dtype != torch.bfloat16:
+        raise Sd3Error("attention_packed: bfloat16 CUDA tensor %s (tokens, heads, head_dim) expected" % what)
+    T, H, D = t.shape
+    if t.numel() and (t.stride(2) != 1 or (H > 1 and t.stride(1) != D)):
+        raise Sd3Error("attention_packed: the heads of a token of %s must lie next to each other" % what)
+    return t.stride(0) if T > 1 else H * D
+
+
+def attention_packed(q, k, v, offsets, causal=False, scale=None, out=None):
+    """Attention over packed sequences: q (T, heads, head_dim), k and v (T, kv_heads, head_dim) bf16, each may be a slice of wider
+    rows; offsets: int32 row numbers on the device, sequence s owns rows offsets[s] to offsets[s + 1] (sd3_attention_packed).
+    scale: None for head_dim ** -0.5.  Rows of no sequence are left as they were in `out`."""
+    torch = _torch()
+    ldq, ldk, ldv = _tokens(q, "q"), _tokens(k, "k"), _tokens(v, "v")
+    T, H, D = q.shape
+    if k.shape != v.shape or k.shape[0] != T or k.shape[2] != D or k.device != q.device or v.device != q.device:
+        raise Sd3Error("attention_packed: k and v (T, kv_heads, head_dim) next to q (T, heads, head_dim) expected")
+    if (offsets.dtype != torch.int32 or offsets.dim() != 1 or offsets.numel() < 1 or not offsets.is_contiguous()
+            or offsets.device != q.device):
+        raise Sd3Error("attention_packed: offsets must be contiguous int32 row numbers on q's device")
+    if out is None:
+        out = torch.empty((T, H, D), device=q.device, dtype=q.dtype)
+    if out.shape != q.shape or out.device != q.device:
+        raise Sd3Error("attention_packed: out must have q's shape and device")
+    with torch.cuda.device(q.device):
+        check(lib().sd3_attention_packed(c_void_p(q.data_ptr()), ldq, c_void_p(k.data_ptr()), ldk, c_void_p(v.data_ptr()), ldv,
+                                         c_void_p(out.data_ptr()), _tokens(out, "out"), c_void_p(offsets.data_ptr()),
+                                         offsets.numel() - 1, T, H, k.shape[1], D, int(bool(causal)),
+                                         D ** -0.5 if scale is None else scale, stream_ptr()), "sd3_attention_packed")
     return out
 
 
