@@ -5,7 +5,7 @@
 //   out[t, h] = sum_j p_j v[j, g],  p = softmax_j(scale q[t, h] . k[j, g]),  g = h / (heads / kv_heads)
 //
 // One CTA owns 128 queries of one (sequence, head), two CTAs share an SM and fill each other's waits: warp 0 streams K and V
-// tiles of 128 keys by TMA, warp 1 issues the MMAs, four softmax warps own a query row per thread.  As in
+// tiles by TMA, warp 1 issues the MMAs, four softmax warps own a query row per thread.  As in
 // attention_tcgen05.cu the softmax is online per 64 keys, exponentials go to the MUFU unit and, one of eight, to the FMA pipe,
 // O is rescaled only when the maximum has moved by more than 2^8.
 //
@@ -14,8 +14,8 @@
 // Tiles run in the order of their place in their sequence, the last first: with `causal` those are the long ones, and the
 // short ones fill the end.
 //
-// Only the last key tile of a query tile is masked: it holds the diagonal or the end of the sequence.  Keys behind the end are the
-// next sequence's: their scores become -inf, and their rows of V zeros, because 0 * inf is not 0.
+// Only key tiles that hold the diagonal or the end of the sequence are masked.  Keys behind the end are the next sequence's: their
+// scores become -inf, and their rows of V zeros, because 0 * inf is not 0.
 #include <cuda.h>
 
 #include <mutex>
@@ -35,22 +35,25 @@ namespace {
 using namespace softmax_detail;
 
 constexpr int AP_BM = 128;                    // queries per CTA
-constexpr int AP_BN = 128;                    // keys per tile
-constexpr int AP_SUB_BYTES = AP_BN * 64 * 2;  // 128 rows x 64 values in the 128-byte swizzle: 16 KiB
 constexpr int AP_THREADS = 192;
 constexpr int AP_TMEM_COLS = 256;
 constexpr int AP_SCAN_CHUNKS = 8;  // up to 256 sequences are put in order of length
-// head_dim 64: scores, P and O side by side (128 + 64 + 64 columns), K and V rings of two tiles.  head_dim 128: O takes 128
-// columns, P lies over the scores it was made from, and one tile each of K and V leaves room for two CTAs an SM.
+// Tensor memory, 256 columns for each of the two CTAs of an SM: the scores of one tile of keys, P of one or two, O.  The score
+// buffer takes the next tile as soon as the softmax warps have pulled this one into registers, and P has columns of its own, so
+// that scores, softmax and products of neighbouring tiles overlap.  head_dim 128 leaves 128 columns beside O: tiles of 64
+// keys, P of two.  (With 128 keys, P over the scores it was made from, everything waits for everything: a tile took 4600 cycles a
+// CTA, softmax 2200, products 850, scores 1150; 8192 causal tokens, 32 heads: 641 us.)
 template <int D>
 struct ApCfg {
+  static constexpr int BN = D == 64 ? 128 : 64;  // keys per tile
   static constexpr int SUBS = D / 64;
-  static constexpr int TILE_BYTES = SUBS * AP_SUB_BYTES;
-  static constexpr int STAGES = D == 64 ? 2 : 1;
-  static constexpr bool P_OVER_S = D == 128;
-  static constexpr int P_COL = P_OVER_S ? 0 : 128;
-  static constexpr int O_COL = D == 64 ? 192 : 128;
-  static constexpr int SMEM_BYTES = (1 + 2 * STAGES) * TILE_BYTES + 256 + 1024;
+  static constexpr int Q_SUB = AP_BM * 128, KV_SUB = BN * 128;  // rows x 64 values in the 128-byte swizzle
+  static constexpr int Q_BYTES = SUBS * Q_SUB, KV_BYTES = SUBS * KV_SUB;
+  static constexpr int STAGES = 2;
+  static constexpr int P_BUFS = D == 64 ? 1 : 2, P_COLS = BN / 2;
+  static constexpr int P_COL = BN, O_COL = P_COL + P_BUFS * P_COLS;
+  static constexpr int SMEM_BYTES = Q_BYTES + 2 * STAGES * KV_BYTES + 256 + 1024;
+  static_assert(O_COL + D <= AP_TMEM_COLS, "fits the columns of one CTA");
 };
 
 struct PackedArgs {
@@ -163,18 +166,18 @@ __global__ void __launch_bounds__(AP_THREADS, 2)
 attention_packed_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                         const __grid_constant__ CUtensorMap tmV, const __grid_constant__ PackedArgs a) {
   using Cfg = ApCfg<D>;
-  constexpr int STAGES = Cfg::STAGES, SUBS = Cfg::SUBS, TILE = Cfg::TILE_BYTES;
+  constexpr int BN = Cfg::BN, STAGES = Cfg::STAGES, SUBS = Cfg::SUBS, TILE = Cfg::KV_BYTES, P_BUFS = Cfg::P_BUFS;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   uint8_t* q_smem = smem;
-  uint8_t* k_smem = smem + TILE;
+  uint8_t* k_smem = smem + Cfg::Q_BYTES;
   uint8_t* v_smem = k_smem + STAGES * TILE;
   uint64_t* q_full = reinterpret_cast<uint64_t*>(v_smem + STAGES * TILE);
   uint64_t* k_full = q_full + 1;          // STAGES
   uint64_t* v_full = k_full + STAGES;     // STAGES
   uint64_t* s_full = v_full + STAGES;     // STAGES: scores of the tile in this stage complete (its K is free)
   uint64_t* pv_done = s_full + STAGES;    // STAGES: products of the tile in this stage complete (V and P free, O quiescent)
-  uint64_t* s_free = pv_done + STAGES;    // 1: scores pulled into registers (4 arrivals); not used with P over S
+  uint64_t* s_free = pv_done + STAGES;    // 1: scores pulled into registers (4 arrivals)
   uint64_t* p_ready = s_free + 1;         // 1: P of the tile stored (4 arrivals)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(p_ready + 1);
   int* s_abort = reinterpret_cast<int*>(tmem_slot + 1);
@@ -223,7 +226,7 @@ attention_packed_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
   const int begin = __shfl_sync(0xffffffffu, s_unit[0], 0), len = __shfl_sync(0xffffffffu, s_unit[1], 0);
   const int q0 = __shfl_sync(0xffffffffu, s_unit[2], 0);
   const int keys = a.causal ? min(len, q0 + AP_BM) : len;  // that this tile's queries see
-  const int nkv = q0 < 0 ? 0 : (keys + AP_BN - 1) / AP_BN;  // at least one for a tile that exists
+  const int nkv = q0 < 0 ? 0 : (keys + BN - 1) / BN;  // at least one for a tile that exists
 
   if (nkv == 0) {
     // no such tile: the rows hold fewer than the grid has room for
@@ -231,27 +234,27 @@ attention_packed_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
     // ------------------------------ TMA producer (a converged warp, one lane issues) ------
     const bool issuer = elect_one();
     const int g = h / a.group;
-    auto load = [&](const CUtensorMap* tm, uint8_t* to, uint64_t* bar, int head, int row) {
-      mbar_expect_tx(bar, TILE);
+    auto load = [&](const CUtensorMap* tm, uint8_t* to, int sub_bytes, uint64_t* bar, int head, int row) {
+      mbar_expect_tx(bar, SUBS * sub_bytes);
 #pragma unroll
-      for (int s = 0; s < SUBS; ++s) tma_load_3d(to + s * AP_SUB_BYTES, tm, bar, 64 * s, head, row);
+      for (int s = 0; s < SUBS; ++s) tma_load_3d(to + s * sub_bytes, tm, bar, 64 * s, head, row);
     };
-    if (issuer) load(&tmQ, q_smem, q_full, h, begin + q0);
+    if (issuer) load(&tmQ, q_smem, Cfg::Q_SUB, q_full, h, begin + q0);
     for (int j = 0; j < nkv; ++j) {
       const int st = j % STAGES;
       const uint32_t prev = ((j / STAGES) + 1) & 1;  // parity of this stage's previous use
       if (j >= STAGES && !mbar_wait_all(&s_full[st], prev, wc, DEV_TIMEOUT_ATTN_KV)) break;
-      if (issuer) load(&tmK, k_smem + st * TILE, &k_full[st], g, begin + j * AP_BN);
+      if (issuer) load(&tmK, k_smem + st * TILE, Cfg::KV_SUB, &k_full[st], g, begin + j * BN);
       if (j >= STAGES && !mbar_wait_all(&pv_done[st], prev, wc, DEV_TIMEOUT_ATTN_KV)) break;
-      if (issuer) load(&tmV, v_smem + st * TILE, &v_full[st], g, begin + j * AP_BN);
+      if (issuer) load(&tmV, v_smem + st * TILE, Cfg::KV_SUB, &v_full[st], g, begin + j * BN);
     }
   } else if (warp == 1) {
     // ------------------------------ MMA issuer (a converged warp, one lane issues) ------
-    constexpr uint32_t IDESC_S = make_idesc(1, 1, AP_BM, AP_BN, 0, 0);  // Q K^T, both K-major
+    constexpr uint32_t IDESC_S = make_idesc(1, 1, AP_BM, BN, 0, 0);  // Q K^T, both K-major
     constexpr uint32_t IDESC_O = make_idesc(1, 1, AP_BM, D, 0, 1);      // P V, V is MN-major
     const uint64_t q_desc = make_smem_desc_sw128(smem_u32(q_smem), 16, 1024);
     const uint64_t k_desc0 = make_smem_desc_sw128(smem_u32(k_smem), 16, 1024);
-    const uint64_t v_desc0 = make_smem_desc_sw128(smem_u32(v_smem), AP_SUB_BYTES, 1024);
+    const uint64_t v_desc0 = make_smem_desc_sw128(smem_u32(v_smem), Cfg::KV_SUB, 1024);
     const bool issuer = elect_one();
     auto issue_s = [&](int j) {
       const int st = j % STAGES;
@@ -260,8 +263,9 @@ attention_packed_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
       if (issuer) {
 #pragma unroll
         for (int k = 0; k < D / 16; ++k) {  // 16 of head_dim: 32 bytes of a 128-byte row, four to a 64-wide subtile
-          const uint64_t adv = static_cast<uint64_t>(((k / 4) * AP_SUB_BYTES + (k % 4) * 32) >> 4);
-          mma_f16_ss(tmem_base, q_desc + adv, k_desc0 + static_cast<uint32_t>(st * (TILE >> 4)) + adv, IDESC_S, k != 0);
+          const uint64_t q_adv = static_cast<uint64_t>(((k / 4) * Cfg::Q_SUB + (k % 4) * 32) >> 4);
+          const uint64_t k_adv = static_cast<uint64_t>(((k / 4) * Cfg::KV_SUB + (k % 4) * 32) >> 4);
+          mma_f16_ss(tmem_base, q_desc + q_adv, k_desc0 + static_cast<uint32_t>(st * (TILE >> 4)) + k_adv, IDESC_S, k != 0);
         }
         mma_commit(&s_full[st]);
       }
@@ -274,8 +278,8 @@ attention_packed_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
       tc_fence_after_sync();
       if (issuer) {
 #pragma unroll
-        for (int k = 0; k < AP_BN / 16; ++k)  // 16 keys: 8 columns of bf16 pairs, 16 rows of V (128 bytes each)
-          mma_f16_ts(tmem_base + Cfg::O_COL, tmem_base + Cfg::P_COL + 8 * k,
+        for (int k = 0; k < BN / 16; ++k)  // 16 keys: 8 columns of bf16 pairs, 16 rows of V (128 bytes each)
+          mma_f16_ts(tmem_base + Cfg::O_COL, tmem_base + Cfg::P_COL + (j % P_BUFS) * Cfg::P_COLS + 8 * k,
                      v_desc0 + static_cast<uint32_t>(st * (TILE >> 4)) + static_cast<uint64_t>((k * 16 * 128) >> 4), IDESC_O,
                      (j != 0 || k != 0));
         mma_commit(&pv_done[st]);
@@ -284,36 +288,29 @@ attention_packed_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
     };
     bool ok = mbar_wait_all(q_full, 0, wc, DEV_TIMEOUT_ATTN_Q);
     for (int j = 0; j <= nkv && ok; ++j) {
-      if constexpr (Cfg::P_OVER_S) {
-        // the scores of tile j take the place of P of tile j - 1
-        if (j >= 1) ok = issue_pv(j - 1);
-        if (ok && j >= 1 && j < nkv)
-          ok = mbar_wait_all(&pv_done[(j - 1) % STAGES], ((j - 1) / STAGES) & 1, wc, DEV_TIMEOUT_ATTN_O);
-        if (ok && j < nkv) ok = issue_s(j);
-      } else {
-        // the softmax warps have pulled the scores of tile j - 1 into registers
-        if (j >= 1 && j < nkv) ok = mbar_wait_all(s_free, (j - 1) & 1, wc, DEV_TIMEOUT_ATTN_S);
-        if (ok && j < nkv) ok = issue_s(j);
-        if (ok && j >= 1) ok = issue_pv(j - 1);
-      }
+      // the softmax warps have pulled the scores of tile j - 1 into registers
+      if (j >= 1 && j < nkv) ok = mbar_wait_all(s_free, (j - 1) & 1, wc, DEV_TIMEOUT_ATTN_S);
+      if (ok && j < nkv) ok = issue_s(j);
+      if (ok && j >= 1) ok = issue_pv(j - 1);
     }
   } else {
     // ------------------------------ softmax + epilogue ------------------------
     const int quad = warp & 3;
     const int row = quad * 32 + lane;
     const uint32_t lane_base = tmem_base + (static_cast<uint32_t>(quad * 32) << 16);
-    const uint32_t s_tmem = lane_base, p_tmem = lane_base + Cfg::P_COL, o_tmem = lane_base + Cfg::O_COL;
+    const uint32_t s_tmem = lane_base, o_tmem = lane_base + Cfg::O_COL;
     const float c = a.scale_log2e;
     const int seen = a.causal ? min(len, q0 + row + 1) : len;  // keys that this row sees, at least one
     float m_used = -INFINITY;  // running maximum (raw score units) that the exponentials refer to
     float2 l2 = make_float2(0.f, 0.f);
     bool ok = true;
     uint32_t pre_s = 0;  // early test of s_full for the coming tile
-    uint32_t ra[32], rb[32], rc[32], rd[32];
+    uint32_t ra[32], rb[32], rc[32], rd[32];  // scores of a tile, then packed P (the last two: of 128 keys)
     for (int j = 0; j < nkv; ++j) {
       const int st = j % STAGES;
-      const int kv0 = j * AP_BN;
-      const bool masked = j == nkv - 1;
+      const int kv0 = j * BN;
+      const bool masked = kv0 + BN > len || (a.causal && kv0 + BN > q0 + 1);  // some row does not see all of its keys
+      const uint32_t p_tmem = lane_base + Cfg::P_COL + (j % P_BUFS) * Cfg::P_COLS;
       const int stp = (j + STAGES - 1) % STAGES;                      // stage and parity of the
       const uint32_t parp = j >= 1 ? ((j - 1) / STAGES) & 1 : 0;      // previous tile's products
       if (!mbar_wait_pre(pre_s, &s_full[st], (j / STAGES) & 1, wc, DEV_TIMEOUT_ATTN_S)) { ok = false; break; }
@@ -330,8 +327,7 @@ attention_packed_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
             l2.y *= alpha;
           }
           if (j >= 1 && ok) {
-            // with P over S the scores of this tile were issued after these products were complete
-            if (!Cfg::P_OVER_S) ok = mbar_wait_warp(&pv_done[stp], parp, wc, DEV_TIMEOUT_ATTN_O);
+            ok = mbar_wait_warp(&pv_done[stp], parp, wc, DEV_TIMEOUT_ATTN_O);
             if (ok) rescale_row<D>(o_tmem, alpha);
           }
           if (second) {  // the first half of P was formed against the older maximum
@@ -351,34 +347,47 @@ attention_packed_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
       tmem_ld_32x32b_x32(s_tmem, ra);
       tmem_ld_32x32b_x32(s_tmem + 32, rb);
       tmem_wait_ld();
+      if constexpr (BN == 64) {
+        tc_fence_before_sync();
+        __syncwarp();
+        mbar_arrive_lane0(s_free, lane);  // the score buffer can take the next tile
+      }
       if (masked) { mask_cols(ra, kv0, seen); mask_cols(rb, kv0 + 32, seen); }
       half_step(ra, rb, false);
-      // the second half is only loaded now: with all 128 scores live the kernel spills
-      tmem_ld_32x32b_x32(s_tmem + 64, rc);
-      tmem_ld_32x32b_x32(s_tmem + 96, rd);
-      tmem_wait_ld();
-      __syncwarp();
-      if (!Cfg::P_OVER_S) mbar_arrive_lane0(s_free, lane);  // the score buffer can take the next tile
-      if (masked) { mask_cols(rc, kv0 + 64, seen); mask_cols(rd, kv0 + 96, seen); }
-      uint32_t pre_pv = 1;
-      if (!Cfg::P_OVER_S && j >= 1) pre_pv = mbar_test_wait(&pv_done[stp], parp);
-      half_step(rc, rd, true);
-      // P is free once the products of the previous tile are complete (tested half a tile ago)
-      if (!Cfg::P_OVER_S && j >= 1 && ok) ok = mbar_wait_pre(pre_pv, &pv_done[stp], parp, wc, DEV_TIMEOUT_ATTN_O);
+      if constexpr (BN == 128) {
+        // the second half is only loaded now: with all 128 scores live the kernel spills
+        tmem_ld_32x32b_x32(s_tmem + 64, rc);
+        tmem_ld_32x32b_x32(s_tmem + 96, rd);
+        tmem_wait_ld();
+        tc_fence_before_sync();
+        __syncwarp();
+        mbar_arrive_lane0(s_free, lane);  // the score buffer can take the next tile
+        if (masked) { mask_cols(rc, kv0 + 64, seen); mask_cols(rd, kv0 + 96, seen); }
+        uint32_t pre_pv = 1;
+        if (j >= 1) pre_pv = mbar_test_wait(&pv_done[stp], parp);
+        half_step(rc, rd, true);
+        // P is free once the products of the previous tile are complete (tested half a tile ago)
+        if (j >= 1 && ok) ok = mbar_wait_pre(pre_pv, &pv_done[stp], parp, wc, DEV_TIMEOUT_ATTN_O);
+      } else {
+        // this buffer of P is free once the products of the tile before the last are complete
+        if (j >= 2 && ok) ok = mbar_wait_warp(&pv_done[st], ((j - 2) / STAGES) & 1, wc, DEV_TIMEOUT_ATTN_O);
+      }
       if (!ok) break;
       tmem_st_32x32b_x16(p_tmem, reinterpret_cast<uint32_t(&)[16]>(ra));
       tmem_st_32x32b_x16(p_tmem + 16, reinterpret_cast<uint32_t(&)[16]>(rb));
-      tmem_st_32x32b_x16(p_tmem + 32, reinterpret_cast<uint32_t(&)[16]>(rc));
-      tmem_st_32x32b_x16(p_tmem + 48, reinterpret_cast<uint32_t(&)[16]>(rd));
-      if (masked && kv0 + AP_BN > len) {
+      if constexpr (BN == 128) {
+        tmem_st_32x32b_x16(p_tmem + 32, reinterpret_cast<uint32_t(&)[16]>(rc));
+        tmem_st_32x32b_x16(p_tmem + 48, reinterpret_cast<uint32_t(&)[16]>(rd));
+      }
+      if (kv0 + BN > len) {
         // rows of V behind the sequence's end become zeros, whatever they are
         ok = mbar_wait_warp(&v_full[st], (j / STAGES) & 1, wc, DEV_TIMEOUT_ATTN_KV);
-        if (ok && kv0 + row >= len) {
+        if (ok && row < BN && kv0 + row >= len) {
 #pragma unroll
           for (int s = 0; s < SUBS; ++s)
 #pragma unroll
             for (int i = 0; i < 8; ++i)
-              *reinterpret_cast<uint4*>(v_smem + st * TILE + s * AP_SUB_BYTES + row * 128 + i * 16) = make_uint4(0, 0, 0, 0);
+              *reinterpret_cast<uint4*>(v_smem + st * TILE + s * Cfg::KV_SUB + row * 128 + i * 16) = make_uint4(0, 0, 0, 0);
         }
         fence_proxy_async_smem();
       }
@@ -458,7 +467,8 @@ int launch_attention_packed(const PackedAttention& p, int* dev_status, cudaStrea
   for (int i = 0; i < 3; ++i) {
     int rc = encode_tmap_3d(&tm[i], base[i], 2, static_cast<uint64_t>(p.head_dim),
                             static_cast<uint64_t>(i == 0 ? p.heads : p.kv_heads), static_cast<uint64_t>(p.rows),
-                            static_cast<uint64_t>(p.head_dim) * 2, static_cast<uint64_t>(ld[i]) * 2, 64, 1, AP_BM);
+                            static_cast<uint64_t>(p.head_dim) * 2, static_cast<uint64_t>(ld[i]) * 2, 64, 1,
+                            i == 0 ? AP_BM : p.head_dim == 64 ? ApCfg<64>::BN : ApCfg<128>::BN);
     if (rc) return rc;
   }
   PackedArgs a;
