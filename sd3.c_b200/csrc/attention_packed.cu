@@ -6,8 +6,8 @@
 //
 // One CTA owns 128 queries of one (sequence, head), two CTAs share an SM and fill each other's waits: warp 0 streams K and V
 // tiles by TMA, warp 1 issues the MMAs, four softmax warps own a query row per thread.  As in
-// attention_tcgen05.cu the softmax is online per 64 keys, exponentials go to the MUFU unit and, one of eight, to the FMA pipe,
-// O is rescaled only when the maximum has moved by more than 2^8.
+// attention_tcgen05.cu the softmax is online per 64 keys and O is rescaled only when the maximum has moved by more than 2^8; every
+// exponential goes to the MUFU unit (a quarter of them as polynomials changes no time: 8192 tokens, head_dim 64, 375 us either way).
 //
 // Which tile a CTA takes is found on the device, from the offsets: their values may come from an earlier kernel and may change
 // between replays of a captured graph.  The grid has room for every way in which the rows can be cut into `count` sequences.
@@ -22,6 +22,7 @@
 
 #include "attention_softmax.cuh"
 #include "kernels.h"
+#include "launch_rules.h"
 #include "ptx.cuh"
 
 namespace sd3 {
@@ -336,13 +337,8 @@ attention_packed_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
           }
         }
         const float nmc = -m_used * c;
-        if (masked) {
-          exp_pack<false>(r0, c, nmc, l2);
-          exp_pack<false>(r1, c, nmc, l2);
-        } else {
-          exp_pack(r0, c, nmc, l2);
-          exp_pack(r1, c, nmc, l2);
-        }
+        exp_pack<false>(r0, c, nmc, l2);
+        exp_pack<false>(r1, c, nmc, l2);
       };
       tmem_ld_32x32b_x32(s_tmem, ra);
       tmem_ld_32x32b_x32(s_tmem + 32, rb);
@@ -433,21 +429,340 @@ attention_packed_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
   }
 }
 
+// ----------------------------------------------------------------------------
+// head_dim 128, long sequences, an even number of query heads to a key / value head: one CTA an SM owns the same 128 queries of
+// two heads, A and B, that share K and V.  512 columns of tensor memory hold O of both (2 x 128), P of both (2 x 64) and the scores
+// of ONE tile of 128 keys, which the heads use in turn: a warpgroup pulls all 128 scores of its row into registers (216 of them,
+// taken over from the first warpgroup), and the other head's next scores are formed while it works.  Scores of 64 keys, all that
+// two CTAs an SM leave room for, cost the tensor cores as much shared-memory bandwidth as 96 (4 KiB of Q for 2 KiB of K an
+// instruction); K and V are read once for both heads.
+// ----------------------------------------------------------------------------
+constexpr int HP_BN = 128, HP_STAGES = 2, HP_D = 128;
+constexpr int HP_SUB = 128 * 128;               // 128 rows x 64 values
+constexpr int HP_TILE = 2 * HP_SUB;             // Q of a head, K or V of a tile
+constexpr int HP_THREADS = 384;                 // TMA, MMA, two idle warps; softmax warpgroups of A and B
+constexpr int HP_REGS_LAUNCH = 168, HP_REGS_ISSUE = 64, HP_REGS_SOFTMAX = 216;
+static_assert(128 * HP_REGS_ISSUE + 256 * HP_REGS_SOFTMAX <= HP_THREADS * HP_REGS_LAUNCH, "the shares fit the launch");
+constexpr int HP_S_COL = 0, HP_P_COL = 128, HP_O_COL = 256;  // P and O of B 64 and 128 columns further
+constexpr int HP_SMEM_BYTES = (2 + 2 * HP_STAGES) * HP_TILE + 256 + 1024;
+
+__global__ void __launch_bounds__(HP_THREADS, 1)
+attention_packed_heads_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+                              const __grid_constant__ CUtensorMap tmV, const __grid_constant__ PackedArgs a) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint8_t* q_smem = smem;  // A, B
+  uint8_t* k_smem = q_smem + 2 * HP_TILE;
+  uint8_t* v_smem = k_smem + HP_STAGES * HP_TILE;
+  uint64_t* q_full = reinterpret_cast<uint64_t*>(v_smem + HP_STAGES * HP_TILE);
+  uint64_t* k_full = q_full + 1;           // HP_STAGES
+  uint64_t* v_full = k_full + HP_STAGES;   // HP_STAGES
+  uint64_t* k_free = v_full + HP_STAGES;   // HP_STAGES: both heads' scores of the tile in this stage complete
+  uint64_t* v_free = k_free + HP_STAGES;   // HP_STAGES: both heads' products complete
+  uint64_t* s_full = v_free + HP_STAGES;   // 2: scores of A, of B
+  uint64_t* s_free = s_full + 2;           // 2: A, B has pulled its scores (4 arrivals)
+  uint64_t* p_ready = s_free + 2;          // 2 (4 arrivals)
+  uint64_t* pv_done = p_ready + 2;         // 2
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(pv_done + 2);
+  int* s_abort = reinterpret_cast<int*>(tmem_slot + 1);
+  int* s_unit = s_abort + 1;  // 3
+
+  const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0);  // known uniform
+  const int lane = threadIdx.x & 31;
+  const int pairs = a.heads / 2;
+  const int h0 = 2 * (static_cast<int>(blockIdx.x) % pairs);
+
+  if (threadIdx.x == 32) {
+    mbar_init(q_full, 1);
+    for (int s = 0; s < HP_STAGES; ++s) {
+      mbar_init(&k_full[s], 1);
+      mbar_init(&v_full[s], 1);
+      mbar_init(&k_free[s], 1);
+      mbar_init(&v_free[s], 1);
+    }
+    for (int x = 0; x < 2; ++x) {
+      mbar_init(&s_full[x], 1);
+      mbar_init(&s_free[x], 4);
+      mbar_init(&p_ready[x], 4);
+      mbar_init(&pv_done[x], 1);
+    }
+    *s_abort = 0;
+    fence_barrier_init();
+    prefetch_tmap(&tmQ);
+    prefetch_tmap(&tmK);
+    prefetch_tmap(&tmV);
+  }
+  __syncwarp();
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  grid_dep_wait();  // the offsets may be the work of the preceding kernel
+  grid_dep_launch();
+  if (warp == 0) {
+    const Unit u = find_unit(a, static_cast<int>(blockIdx.x) / pairs);
+    if (lane == 0) {
+      s_unit[0] = u.begin;
+      s_unit[1] = u.len;
+      s_unit[2] = u.q0;
+    }
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_slot, 0);
+  const WaitCtx wc{s_abort, a.status};
+  const int begin = __shfl_sync(0xffffffffu, s_unit[0], 0), len = __shfl_sync(0xffffffffu, s_unit[1], 0);
+  const int q0 = __shfl_sync(0xffffffffu, s_unit[2], 0);
+  const int keys = a.causal ? min(len, q0 + AP_BM) : len;  // that this tile's queries see
+  const int nkv = q0 < 0 ? 0 : (keys + HP_BN - 1) / HP_BN;
+
+  if (warp < 4) {
+    setmaxnreg_dec<HP_REGS_ISSUE>();
+    if (warp == 0 && nkv > 0) {
+      // ------------------------------ TMA producer (a converged warp, one lane issues) ------
+      const bool issuer = elect_one();
+      const int g = h0 / a.group;
+      auto load = [&](const CUtensorMap* tm, uint8_t* to, uint64_t* bar, int head, int row) {
+        tma_load_3d(to, tm, bar, 0, head, row);
+        tma_load_3d(to + HP_SUB, tm, bar, 64, head, row);
+      };
+      if (issuer) {
+        mbar_expect_tx(q_full, 2 * HP_TILE);
+        load(&tmQ, q_smem, q_full, h0, begin + q0);
+        load(&tmQ, q_smem + HP_TILE, q_full, h0 + 1, begin + q0);
+      }
+      for (int j = 0; j < nkv; ++j) {
+        const int st = j % HP_STAGES;
+        const uint32_t prev = ((j / HP_STAGES) + 1) & 1;  // parity of this stage's previous use
+        if (j >= HP_STAGES && !mbar_wait_vote(&k_free[st], prev, wc, DEV_TIMEOUT_ATTN_KV)) break;
+        if (issuer) {
+          mbar_expect_tx(&k_full[st], HP_TILE);
+          load(&tmK, k_smem + st * HP_TILE, &k_full[st], g, begin + j * HP_BN);
+        }
+        if (j >= HP_STAGES && !mbar_wait_vote(&v_free[st], prev, wc, DEV_TIMEOUT_ATTN_KV)) break;
+        if (issuer) {
+          mbar_expect_tx(&v_full[st], HP_TILE);
+          load(&tmV, v_smem + st * HP_TILE, &v_full[st], g, begin + j * HP_BN);
+        }
+      }
+    } else if (warp == 1 && nkv > 0) {
+      // ------------------------------ MMA issuer (a converged warp, one lane issues) ------
+      constexpr uint32_t IDESC_S = make_idesc(1, 1, AP_BM, HP_BN, 0, 0);  // Q K^T, both K-major
+      constexpr uint32_t IDESC_O = make_idesc(1, 1, AP_BM, HP_D, 0, 1);   // P V, V is MN-major
+      const uint64_t q_desc = make_smem_desc_sw128(smem_u32(q_smem), 16, 1024);
+      const uint64_t k_desc0 = make_smem_desc_sw128(smem_u32(k_smem), 16, 1024);
+      const uint64_t v_desc0 = make_smem_desc_sw128(smem_u32(v_smem), HP_SUB, 1024);
+      const bool issuer = elect_one();
+      auto issue_s = [&](int x, int j) {
+        const int st = j % HP_STAGES;
+        if (issuer) {
+#pragma unroll
+          for (int k = 0; k < HP_D / 16; ++k) {  // 16 of head_dim: 32 bytes of a 128-byte row, four to a 64-wide half
+            const uint64_t adv = static_cast<uint64_t>(((k / 4) * HP_SUB + (k % 4) * 32) >> 4);
+            mma_f16_ss(tmem_base + HP_S_COL, q_desc + static_cast<uint32_t>(x * (HP_TILE >> 4)) + adv,
+                       k_desc0 + static_cast<uint32_t>(st * (HP_TILE >> 4)) + adv, IDESC_S, k != 0);
+          }
+          mma_commit(&s_full[x]);
+          if (x == 1) mma_commit(&k_free[st]);
+        }
+      };
+      auto issue_pv = [&](int x, int j) {
+        const int st = j % HP_STAGES;
+        if (issuer) {
+#pragma unroll
+          for (int k = 0; k < HP_BN / 16; ++k)  // 16 keys: 8 columns of bf16 pairs, 16 rows of V (128 bytes each)
+            mma_f16_ts(tmem_base + HP_O_COL + x * HP_D, tmem_base + HP_P_COL + x * (HP_BN / 2) + 8 * k,
+                       v_desc0 + static_cast<uint32_t>(st * (HP_TILE >> 4)) + static_cast<uint64_t>((k * 16 * 128) >> 4), IDESC_O,
+                       (j != 0 || k != 0));
+          mma_commit(&pv_done[x]);
+          if (x == 1) mma_commit(&v_free[st]);
+        }
+      };
+      // In the order in which what they wait for comes about: scores A j+1 when B has pulled its scores j from the shared columns,
+      // products A j when P is stored, scores B j+1 when A has pulled its scores j+1, products B j.  (Products before scores: the
+      // scores waited for a whole softmax, 4130 cycles for a tile of both heads.)
+      bool ok = mbar_wait_vote(q_full, 0, wc, DEV_TIMEOUT_ATTN_Q);
+      for (int j = 0; j <= nkv && ok; ++j) {
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          if (ok && j < nkv) {  // scores, once the other head has pulled those before
+            if (x == 0) ok = mbar_wait_vote(&k_full[j % HP_STAGES], (j / HP_STAGES) & 1, wc, DEV_TIMEOUT_ATTN_KV);
+            if (ok && (x == 1 || j > 0)) ok = mbar_wait_vote(&s_free[x ^ 1], (x == 1 ? j : j - 1) & 1, wc, DEV_TIMEOUT_ATTN_S);
+            if (ok) {
+              tc_fence_after_sync();
+              issue_s(x, j);
+            }
+          }
+          if (ok && j > 0) {  // products of the tile before
+            if (x == 0) ok = mbar_wait_vote(&v_full[(j - 1) % HP_STAGES], ((j - 1) / HP_STAGES) & 1, wc, DEV_TIMEOUT_ATTN_KV);
+            if (ok) ok = mbar_wait_vote(&p_ready[x], (j - 1) & 1, wc, DEV_TIMEOUT_ATTN_P);
+            if (ok) {
+              tc_fence_after_sync();
+              issue_pv(x, j - 1);
+            }
+          }
+        }
+      }
+    }
+  } else {
+    setmaxnreg_inc<HP_REGS_SOFTMAX>();
+    if (nkv > 0) {
+      // ------------------------------ softmax + epilogue ------------------------
+      const int x = (warp - 4) >> 2;  // A, B
+      const int quad = warp & 3;
+      const int row = quad * 32 + lane;
+      const uint32_t lane_base = tmem_base + (static_cast<uint32_t>(quad * 32) << 16);
+      const uint32_t s_tmem = lane_base + HP_S_COL, p_tmem = lane_base + HP_P_COL + x * (HP_BN / 2);
+      const uint32_t o_tmem = lane_base + HP_O_COL + x * HP_D;
+      const float c = a.scale_log2e;
+      const int seen = a.causal ? min(len, q0 + row + 1) : len;  // keys that this row sees, at least one
+      float m_used = -INFINITY;  // running maximum (raw score units) that the exponentials refer to
+      float2 l2 = make_float2(0.f, 0.f);
+      bool ok = true;
+      uint32_t r0[32], r1[32], r2[32], r3[32];
+      for (int j = 0; j < nkv; ++j) {
+        const int kv0 = j * HP_BN;
+        const bool masked = j == nkv - 1;
+        if (!mbar_wait_warp(&s_full[x], j & 1, wc, DEV_TIMEOUT_ATTN_S)) { ok = false; break; }
+        tc_fence_after_sync();
+        tmem_ld_32x32b_x32(s_tmem, r0);
+        tmem_ld_32x32b_x32(s_tmem + 32, r1);
+        tmem_ld_32x32b_x32(s_tmem + 64, r2);
+        tmem_ld_32x32b_x32(s_tmem + 96, r3);
+        tmem_wait_ld();
+        tc_fence_before_sync();
+        __syncwarp();
+        mbar_arrive_lane0(&s_free[x], lane);  // the columns can take the other head's scores
+        if (masked) {
+          mask_cols(r0, kv0, seen);
+          mask_cols(r1, kv0 + 32, seen);
+          mask_cols(r2, kv0 + 64, seen);
+          mask_cols(r3, kv0 + 96, seen);
+        }
+        uint32_t pre_pv = 1;
+        if (j >= 1) pre_pv = mbar_test_wait(&pv_done[x], (j - 1) & 1);
+        const float mx = fmaxf(max_of2(r0, r1), max_of2(r2, r3));
+        const bool need = (mx - m_used) * c > 8.0f;  // always true in the first tile (m_used = -inf)
+        if (__any_sync(0xffffffffu, need)) {
+          float alpha = 1.0f;
+          if (need) {
+            alpha = ex2_approx((m_used - mx) * c);
+            m_used = mx;
+            l2.x *= alpha;
+            l2.y *= alpha;
+          }
+          if (j >= 1) {
+            ok = mbar_wait_pre(pre_pv, &pv_done[x], (j - 1) & 1, wc, DEV_TIMEOUT_ATTN_O);
+            pre_pv = 1;
+            if (ok) rescale_row<HP_D>(o_tmem, alpha);
+          }
+        }
+        const float nmc = -m_used * c;
+        exp_pack<false>(r0, c, nmc, l2);
+        exp_pack<false>(r1, c, nmc, l2);
+        // P is free once the products of the previous tile are complete
+        if (j >= 1 && ok) ok = mbar_wait_pre(pre_pv, &pv_done[x], (j - 1) & 1, wc, DEV_TIMEOUT_ATTN_O);
+        if (!ok) break;
+        tmem_st_32x32b_x16(p_tmem, reinterpret_cast<uint32_t(&)[16]>(r0));
+        tmem_st_32x32b_x16(p_tmem + 16, reinterpret_cast<uint32_t(&)[16]>(r1));
+        exp_pack<false>(r2, c, nmc, l2);
+        exp_pack<false>(r3, c, nmc, l2);
+        tmem_st_32x32b_x16(p_tmem + 32, reinterpret_cast<uint32_t(&)[16]>(r2));
+        tmem_st_32x32b_x16(p_tmem + 48, reinterpret_cast<uint32_t(&)[16]>(r3));
+        if (kv0 + HP_BN > len) {
+          // rows of V behind the sequence's end become zeros, whatever they are (both heads' warps write the same zeros)
+          ok = mbar_wait_warp(&v_full[j % HP_STAGES], (j / HP_STAGES) & 1, wc, DEV_TIMEOUT_ATTN_KV);
+          if (ok && kv0 + row >= len) {
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+#pragma unroll
+              for (int i = 0; i < 8; ++i)
+                *reinterpret_cast<uint4*>(v_smem + (j % HP_STAGES) * HP_TILE + s * HP_SUB + row * 128 + i * 16) =
+                    make_uint4(0, 0, 0, 0);
+          }
+          fence_proxy_async_smem();
+        }
+        tmem_wait_st();
+        tc_fence_before_sync();
+        __syncwarp();
+        mbar_arrive_lane0(&p_ready[x], lane);
+      }
+      const float l = l2.x + l2.y;
+      if (ok && mbar_wait_warp(&pv_done[x], (nkv - 1) & 1, wc, DEV_TIMEOUT_ATTN_O)) {
+        tc_fence_after_sync();
+        const float inv = 1.0f / l;
+        uint4* to = reinterpret_cast<uint4*>(a.out + static_cast<long>(begin + q0 + row) * a.ldo + (h0 + x) * HP_D);
+#pragma unroll 1
+        for (int part = 0; part < HP_D / 32; ++part) {
+          uint32_t o[32];
+          tmem_ld_32x32b_x32(o_tmem + 32 * part, o);
+          tmem_wait_ld();
+          if (q0 + row < len) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              uint4 u;
+              u.x = pack_bf16x2(__uint_as_float(o[8 * i]) * inv, __uint_as_float(o[8 * i + 1]) * inv);
+              u.y = pack_bf16x2(__uint_as_float(o[8 * i + 2]) * inv, __uint_as_float(o[8 * i + 3]) * inv);
+              u.z = pack_bf16x2(__uint_as_float(o[8 * i + 4]) * inv, __uint_as_float(o[8 * i + 5]) * inv);
+              u.w = pack_bf16x2(__uint_as_float(o[8 * i + 6]) * inv, __uint_as_float(o[8 * i + 7]) * inv);
+              to[4 * part + i] = u;
+            }
+          }
+        }
+      }
+    }
+  }
+
+  // ------------------------------ teardown ------------------------------------
+  tc_fence_before_sync();
+  __syncthreads();
+  if (*s_abort) drain_after_abort();
+  if (warp == 1) {
+    tc_fence_after_sync();
+    tmem_dealloc(tmem_base, 512);
+  }
+}
+
+// once per device: shared memory, and the registers that the launch of the pair kernel must bring
+template <typename K>
+int prepare_kernel(K kern, int smem, int regs, bool* done) {
+  static std::mutex attr_mutex;
+  std::lock_guard<std::mutex> lock(attr_mutex);
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64 || done[dev]) return ST_OK;
+  int rc = check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem),
+                      "cudaFuncSetAttribute(attention_packed)");
+  if (rc) return rc;
+  if (regs > 0) {
+    cudaFuncAttributes fa;
+    rc = check_cuda(cudaFuncGetAttributes(&fa, kern), "cudaFuncGetAttributes(attention_packed)");
+    if (rc) return rc;
+    if (fa.numRegs != regs) {  // the softmax warps' share would never come together
+      set_last_error("attention_packed: built with %d registers a thread, %d expected", fa.numRegs, regs);
+      return ST_UNSUPPORTED;
+    }
+  }
+  done[dev] = true;
+  return ST_OK;
+}
+
+int launch_heads(const CUtensorMap* tm, const PackedArgs& a, long units, cudaStream_t stream) {
+  static bool done[64] = {false};
+  int rc = prepare_kernel(attention_packed_heads_kernel, HP_SMEM_BYTES, HP_REGS_LAUNCH, done);
+  if (rc) return rc;
+  launch_dependent(attention_packed_heads_kernel, static_cast<unsigned>(units * (a.heads / 2)), HP_THREADS, HP_SMEM_BYTES, stream,
+                   tm[0], tm[1], tm[2], a);
+  return after_launch("attention_packed_heads_kernel");
+}
+
 template <int D>
 int launch_inst(const CUtensorMap* tm, const PackedArgs& a, long units, cudaStream_t stream) {
   auto kern = attention_packed_kernel<D>;
-  static std::mutex attr_mutex;
-  static bool attr_done[64] = {false};
-  int dev = 0;
-  cudaGetDevice(&dev);
-  if (dev >= 0 && dev < 64) {
-    std::lock_guard<std::mutex> lock(attr_mutex);
-    if (!attr_done[dev]) {
-      cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, ApCfg<D>::SMEM_BYTES);
-      if (e != cudaSuccess) return check_cuda(e, "cudaFuncSetAttribute(attention_packed)");
-      attr_done[dev] = true;
-    }
-  }
+  static bool done[64] = {false};
+  int rc = prepare_kernel(kern, ApCfg<D>::SMEM_BYTES, 0, done);
+  if (rc) return rc;
   launch_dependent(kern, static_cast<unsigned>(units * a.heads), AP_THREADS, ApCfg<D>::SMEM_BYTES, stream, tm[0], tm[1], tm[2], a);
   return after_launch("attention_packed_kernel");
 }
@@ -461,6 +776,7 @@ int launch_attention_packed(const PackedAttention& p, int* dev_status, cudaStrea
     set_last_error("attention_packed: %ld tiles of %d heads are too many for one launch", units, p.heads);
     return ST_UNSUPPORTED;
   }
+  const bool two_heads = packed_two_heads(p.head_dim, p.heads / p.kv_heads, p.rows, p.count);
   CUtensorMap tm[3];
   const bf16* base[3] = {p.q, p.k, p.v};
   const long ld[3] = {p.ldq, p.ldk, p.ldv};
@@ -468,7 +784,7 @@ int launch_attention_packed(const PackedAttention& p, int* dev_status, cudaStrea
     int rc = encode_tmap_3d(&tm[i], base[i], 2, static_cast<uint64_t>(p.head_dim),
                             static_cast<uint64_t>(i == 0 ? p.heads : p.kv_heads), static_cast<uint64_t>(p.rows),
                             static_cast<uint64_t>(p.head_dim) * 2, static_cast<uint64_t>(ld[i]) * 2, 64, 1,
-                            i == 0 ? AP_BM : p.head_dim == 64 ? ApCfg<64>::BN : ApCfg<128>::BN);
+                            i == 0 ? AP_BM : two_heads ? HP_BN : p.head_dim == 64 ? ApCfg<64>::BN : ApCfg<128>::BN);
     if (rc) return rc;
   }
   PackedArgs a;
@@ -482,6 +798,7 @@ int launch_attention_packed(const PackedAttention& p, int* dev_status, cudaStrea
   a.scale_log2e = p.scale * 1.4426950408889634f;
   a.causal = p.causal;
   a.status = dev_status;
+  if (two_heads) return launch_heads(tm, a, units, stream);
   return p.head_dim == 64 ? launch_inst<64>(tm, a, units, stream) : launch_inst<128>(tm, a, units, stream);
 }
 

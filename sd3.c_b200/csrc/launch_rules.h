@@ -102,4 +102,9 @@ inline LinearPlan linear_plan(int M, int N, int k_blocks, bool tma_out, bool f32
   return {false, f32 && k_blocks > 32 ? 64 : 128, 1};
 }
 
+// Packed attention: whether two query heads of one key / value head share a CTA.
+inline bool packed_two_heads(int head_dim, int group, int rows, int count) {
+  return head_dim == 128 && group % 2 == 0 && rows >= 256L * count;
+}
+
 }  // namespace sd3

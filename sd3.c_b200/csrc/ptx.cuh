@@ -163,6 +163,27 @@ __device__ __forceinline__ bool mbar_wait_all(uint64_t* bar, uint32_t parity, co
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, w, code)) != 0;
 }
 
+// The same wait as a loop around a warp-wide vote: every branch is uniform to the compiler, so that what lives across it (loop
+// counters, descriptors) stays in uniform registers, and there is little of it: the loops of issuing warps run once in a
+// few thousand cycles, between softmax warps that stream through tens of KiB of instructions, and what the instruction cache has
+// lost by then costs 200 to 300 cycles a line.
+__device__ __forceinline__ bool mbar_wait_vote(uint64_t* bar, uint32_t parity, const WaitCtx& w, int code) {
+  uint64_t t0 = 0;
+  uint32_t it = 0;
+  while (!__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) {
+    if ((++it & 0xffu) == 0) {
+      const uint64_t now = global_timer_ns();
+      if (it == 256) t0 = now;
+      if (__any_sync(0xffffffffu, *w.s_abort != 0 || now - t0 > SD3_WAIT_LIMIT_NS)) {
+        *w.s_abort = 1;
+        if (w.g_status) atomicCAS(w.g_status, 0, code);
+        return false;
+      }
+    }
+  }
+  return true;
+}
+
 // After an abort: give copies and MMAs already in flight a bounded time to
 // land before shared memory and TMEM are released.
 __device__ __forceinline__ void drain_after_abort() {
