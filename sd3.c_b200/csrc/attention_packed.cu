@@ -244,9 +244,9 @@ attention_packed_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
     for (int j = 0; j < nkv; ++j) {
       const int st = j % STAGES;
       const uint32_t prev = ((j / STAGES) + 1) & 1;  // parity of this stage's previous use
-      if (j >= STAGES && !mbar_wait_all(&s_full[st], prev, wc, DEV_TIMEOUT_ATTN_KV)) break;
+      if (j >= STAGES && !mbar_wait_vote(&s_full[st], prev, wc, DEV_TIMEOUT_ATTN_KV)) break;
       if (issuer) load(&tmK, k_smem + st * TILE, Cfg::KV_SUB, &k_full[st], g, begin + j * BN);
-      if (j >= STAGES && !mbar_wait_all(&pv_done[st], prev, wc, DEV_TIMEOUT_ATTN_KV)) break;
+      if (j >= STAGES && !mbar_wait_vote(&pv_done[st], prev, wc, DEV_TIMEOUT_ATTN_KV)) break;
       if (issuer) load(&tmV, v_smem + st * TILE, Cfg::KV_SUB, &v_full[st], g, begin + j * BN);
     }
   } else if (warp == 1) {
@@ -259,7 +259,7 @@ attention_packed_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
     const bool issuer = elect_one();
     auto issue_s = [&](int j) {
       const int st = j % STAGES;
-      if (!mbar_wait_all(&k_full[st], (j / STAGES) & 1, wc, DEV_TIMEOUT_ATTN_KV)) return false;
+      if (!mbar_wait_vote(&k_full[st], (j / STAGES) & 1, wc, DEV_TIMEOUT_ATTN_KV)) return false;
       tc_fence_after_sync();
       if (issuer) {
 #pragma unroll
@@ -274,8 +274,8 @@ attention_packed_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
     };
     auto issue_pv = [&](int j) {
       const int st = j % STAGES;
-      if (!mbar_wait_all(&v_full[st], (j / STAGES) & 1, wc, DEV_TIMEOUT_ATTN_KV)) return false;
-      if (!mbar_wait_all(p_ready, j & 1, wc, DEV_TIMEOUT_ATTN_P)) return false;
+      if (!mbar_wait_vote(&v_full[st], (j / STAGES) & 1, wc, DEV_TIMEOUT_ATTN_KV)) return false;
+      if (!mbar_wait_vote(p_ready, j & 1, wc, DEV_TIMEOUT_ATTN_P)) return false;
       tc_fence_after_sync();
       if (issuer) {
 #pragma unroll
@@ -287,10 +287,10 @@ attention_packed_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
       }
       return true;
     };
-    bool ok = mbar_wait_all(q_full, 0, wc, DEV_TIMEOUT_ATTN_Q);
+    bool ok = mbar_wait_vote(q_full, 0, wc, DEV_TIMEOUT_ATTN_Q);
     for (int j = 0; j <= nkv && ok; ++j) {
       // the softmax warps have pulled the scores of tile j - 1 into registers
-      if (j >= 1 && j < nkv) ok = mbar_wait_all(s_free, (j - 1) & 1, wc, DEV_TIMEOUT_ATTN_S);
+      if (j >= 1 && j < nkv) ok = mbar_wait_vote(s_free, (j - 1) & 1, wc, DEV_TIMEOUT_ATTN_S);
       if (ok && j < nkv) ok = issue_s(j);
       if (ok && j >= 1) ok = issue_pv(j - 1);
     }
