@@ -4,8 +4,9 @@
 //
 //   out[t, h] = sum_j p_j v[j, g],  p = softmax_j(scale q[t, h] . k[j, g]),  g = h / (heads / kv_heads)
 //
-// One CTA owns 128 queries of one (sequence, head), two CTAs share an SM and fill each other's waits: warp 0 streams K and V
-// tiles by TMA, warp 1 issues the MMAs, four softmax warps own a query row per thread.  As in
+// A CTA goes through tiles of 128 queries of one (sequence, head); two CTAs share an SM and fill each other's waits.  Warp 0 finds
+// the tiles and streams Q, K and V by TMA, warp 1 issues the MMAs, four softmax warps own a query row per thread; the next
+// query tile's loads and first scores overlap the end of the one before.  As in
 // attention_tcgen05.cu the softmax is online per 64 keys and O is rescaled only when the maximum has moved by more than 2^8; every
 // exponential goes to the MUFU unit (a quarter of them as polynomials changes no time: 8192 tokens, head_dim 64, 375 us either way).
 //
@@ -51,9 +52,10 @@ struct ApCfg {
   static constexpr int Q_SUB = AP_BM * 128, KV_SUB = BN * 128;  // rows x 64 values in the 128-byte swizzle
   static constexpr int Q_BYTES = SUBS * Q_SUB, KV_BYTES = SUBS * KV_SUB;
   static constexpr int STAGES = 2;
+  static constexpr int Q_BUFS = D == 64 ? 2 : 1;  // what two CTAs' shared memory leaves room for
   static constexpr int P_BUFS = D == 64 ? 1 : 2, P_COLS = BN / 2;
   static constexpr int P_COL = BN, O_COL = P_COL + P_BUFS * P_COLS;
-  static constexpr int SMEM_BYTES = Q_BYTES + 2 * STAGES * KV_BYTES + 256 + 1024;
+  static constexpr int SMEM_BYTES = Q_BUFS * Q_BYTES + 2 * STAGES * KV_BYTES + 256 + 1024;
   static_assert(O_COL + D <= AP_TMEM_COLS, "fits the columns of one CTA");
 };
 
@@ -162,34 +164,48 @@ __device__ __noinline__ void rescale_row(uint32_t o_tmem, float alpha) {
   tmem_wait_st();
 }
 
+// Which of the grid's tiles a CTA takes in its round `i`: rounds go through the tiles, long ones first, in alternating
+// directions, so that a CTA that gets the longest of one round gets the shortest of the next.
+__device__ __forceinline__ long tile_of_round(int i) {
+  const long g = gridDim.x;
+  return i * g + ((i & 1) ? g - 1 - blockIdx.x : blockIdx.x);
+}
+
 template <int D>
 __global__ void __launch_bounds__(AP_THREADS, 2)
 attention_packed_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                         const __grid_constant__ CUtensorMap tmV, const __grid_constant__ PackedArgs a) {
   using Cfg = ApCfg<D>;
   constexpr int BN = Cfg::BN, STAGES = Cfg::STAGES, SUBS = Cfg::SUBS, TILE = Cfg::KV_BYTES, P_BUFS = Cfg::P_BUFS;
+  constexpr int Q_BUFS = Cfg::Q_BUFS;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   uint8_t* q_smem = smem;
-  uint8_t* k_smem = smem + Cfg::Q_BYTES;
+  uint8_t* k_smem = smem + Q_BUFS * Cfg::Q_BYTES;
   uint8_t* v_smem = k_smem + STAGES * TILE;
-  uint64_t* q_full = reinterpret_cast<uint64_t*>(v_smem + STAGES * TILE);
-  uint64_t* k_full = q_full + 1;          // STAGES
-  uint64_t* v_full = k_full + STAGES;     // STAGES
-  uint64_t* s_full = v_full + STAGES;     // STAGES: scores of the tile in this stage complete (its K is free)
-  uint64_t* pv_done = s_full + STAGES;    // STAGES: products of the tile in this stage complete (V and P free, O quiescent)
-  uint64_t* s_free = pv_done + STAGES;    // 1: scores pulled into registers (4 arrivals)
-  uint64_t* p_ready = s_free + 1;         // 1: P of the tile stored (4 arrivals)
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(p_ready + 1);
+  uint64_t* q_full = reinterpret_cast<uint64_t*>(v_smem + STAGES * TILE);  // Q_BUFS
+  uint64_t* q_free = q_full + Q_BUFS;        // Q_BUFS: the last scores of this query tile are complete
+  uint64_t* k_full = q_free + Q_BUFS;        // STAGES
+  uint64_t* v_full = k_full + STAGES;        // STAGES
+  uint64_t* s_full = v_full + STAGES;        // STAGES: scores of the tile in this stage complete (its K is free)
+  uint64_t* pv_done = s_full + STAGES;       // STAGES: products of the tile in this stage complete (V and P free, O quiescent)
+  uint64_t* s_free = pv_done + STAGES;       // 1: scores pulled into registers (4 arrivals)
+  uint64_t* p_ready = s_free + 1;            // 1: P of the tile stored (4 arrivals)
+  uint64_t* o_free = p_ready + 1;            // 1: O of a query tile pulled into registers (4 arrivals)
+  uint64_t* unit_full = o_free + 1;          // 2: the next query tile is known
+  uint64_t* unit_free = unit_full + 2;       // 2: all who need it have read it (MMA and softmax warps: 5 arrivals)
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(unit_free + 2);
   int* s_abort = reinterpret_cast<int*>(tmem_slot + 1);
-  int* s_unit = s_abort + 1;  // 3
+  int* s_unit = s_abort + 1;  // two times 4: first row, length, first query (below 0: no more), head
 
   const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0);  // known uniform
   const int lane = threadIdx.x & 31;
-  const int h = static_cast<int>(blockIdx.x) % a.heads;
 
   if (threadIdx.x == 32) {
-    mbar_init(q_full, 1);
+    for (int s = 0; s < Q_BUFS; ++s) {
+      mbar_init(&q_full[s], 1);
+      mbar_init(&q_free[s], 1);
+    }
     for (int s = 0; s < STAGES; ++s) {
       mbar_init(&k_full[s], 1);
       mbar_init(&v_full[s], 1);
@@ -198,6 +214,11 @@ attention_packed_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
     }
     mbar_init(s_free, 4);
     mbar_init(p_ready, 4);
+    mbar_init(o_free, 4);
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&unit_full[s], 1);
+      mbar_init(&unit_free[s], 5);
+    }
     *s_abort = 0;
     fence_barrier_init();
     prefetch_tmap(&tmQ);
@@ -211,88 +232,137 @@ attention_packed_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
   }
   grid_dep_wait();  // the offsets may be the work of the preceding kernel
   grid_dep_launch();
+  Unit u;  // warp 0: the query tile of the coming round, and its head
+  int h = 0;
+  auto find = [&](int i) {
+    const long w = tile_of_round(i);
+    const long rank = w / a.heads;
+    h = static_cast<int>(w - rank * a.heads);
+    u = find_unit(a, rank < (1L << 30) ? static_cast<int>(rank) : (1 << 30));
+  };
+  auto write_unit = [&](int i) {
+    int* to = s_unit + 4 * (i & 1);
+    to[0] = u.begin;
+    to[1] = u.len;
+    to[2] = u.q0;
+    to[3] = h;
+  };
   if (warp == 0) {
-    const Unit u = find_unit(a, static_cast<int>(blockIdx.x) / a.heads);
-    if (lane == 0) {
-      s_unit[0] = u.begin;
-      s_unit[1] = u.len;
-      s_unit[2] = u.q0;
-    }
+    find(0);
+    if (lane == 0) write_unit(0);
   }
   tc_fence_before_sync();
   __syncthreads();
   tc_fence_after_sync();
   const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_slot, 0);
   const WaitCtx wc{s_abort, a.status};
-  const int begin = __shfl_sync(0xffffffffu, s_unit[0], 0), len = __shfl_sync(0xffffffffu, s_unit[1], 0);
-  const int q0 = __shfl_sync(0xffffffffu, s_unit[2], 0);
-  const int keys = a.causal ? min(len, q0 + AP_BM) : len;  // that this tile's queries see
-  const int nkv = q0 < 0 ? 0 : (keys + BN - 1) / BN;  // at least one for a tile that exists
+  auto key_tiles = [&](int len, int q0) { return ((a.causal ? min(len, q0 + AP_BM) : len) + BN - 1) / BN; };  // that its queries see
 
-  if (nkv == 0) {
-    // no such tile: the rows hold fewer than the grid has room for
-  } else if (warp == 0) {
+  // K, V, score and P buffers go round over all key tiles of all query tiles: tile number t uses stage t % STAGES.
+  if (warp == 0) {
     // ------------------------------ TMA producer (a converged warp, one lane issues) ------
     const bool issuer = elect_one();
-    const int g = h / a.group;
     auto load = [&](const CUtensorMap* tm, uint8_t* to, int sub_bytes, uint64_t* bar, int head, int row) {
       mbar_expect_tx(bar, SUBS * sub_bytes);
 #pragma unroll
       for (int s = 0; s < SUBS; ++s) tma_load_3d(to + s * sub_bytes, tm, bar, 64 * s, head, row);
     };
-    if (issuer) load(&tmQ, q_smem, Cfg::Q_SUB, q_full, h, begin + q0);
-    for (int j = 0; j < nkv; ++j) {
-      const int st = j % STAGES;
-      const uint32_t prev = ((j / STAGES) + 1) & 1;  // parity of this stage's previous use
-      if (j >= STAGES && !mbar_wait_vote(&s_full[st], prev, wc, DEV_TIMEOUT_ATTN_KV)) break;
-      if (issuer) load(&tmK, k_smem + st * TILE, Cfg::KV_SUB, &k_full[st], g, begin + j * BN);
-      if (j >= STAGES && !mbar_wait_vote(&pv_done[st], prev, wc, DEV_TIMEOUT_ATTN_KV)) break;
-      if (issuer) load(&tmV, v_smem + st * TILE, Cfg::KV_SUB, &v_full[st], g, begin + j * BN);
+    if (lane == 0) mbar_arrive(&unit_full[0]);  // nobody waits for the first one: it is known since the barrier above
+    bool ok = true;
+    for (int i = 0, t = 0; ok && u.q0 >= 0; ++i) {
+      const Unit now = u;
+      const int g = h / a.group, nkv = key_tiles(now.len, now.q0);
+      if (i >= Q_BUFS && !mbar_wait_vote(&q_free[i % Q_BUFS], ((i / Q_BUFS) + 1) & 1, wc, DEV_TIMEOUT_ATTN_Q)) break;
+      if (issuer)
+        load(&tmQ, q_smem + (i % Q_BUFS) * Cfg::Q_BYTES, Cfg::Q_SUB, &q_full[i % Q_BUFS], h, now.begin + now.q0);
+      for (int j = 0; j < nkv && ok; ++j, ++t) {
+        const int st = t % STAGES;
+        const uint32_t prev = ((t / STAGES) + 1) & 1;  // parity of this stage's previous use
+        if (t >= STAGES) ok = mbar_wait_vote(&s_full[st], prev, wc, DEV_TIMEOUT_ATTN_KV);
+        if (ok && issuer) load(&tmK, k_smem + st * TILE, Cfg::KV_SUB, &k_full[st], g, now.begin + j * BN);
+        if (ok && t >= STAGES) ok = mbar_wait_vote(&pv_done[st], prev, wc, DEV_TIMEOUT_ATTN_KV);
+        if (ok && issuer) load(&tmV, v_smem + st * TILE, Cfg::KV_SUB, &v_full[st], g, now.begin + j * BN);
+        if (ok && j == 0) {  // while the first tiles are under way: the next query tile, for the others too
+          find(i + 1);
+          if (i >= 1) ok = mbar_wait_vote(&unit_free[(i + 1) & 1], (((i + 1) >> 1) + 1) & 1, wc, DEV_TIMEOUT_ATTN_Q);
+          if (ok && lane == 0) {
+            write_unit(i + 1);
+            mbar_arrive(&unit_full[(i + 1) & 1]);
+          }
+          __syncwarp();
+        }
+      }
     }
   } else if (warp == 1) {
     // ------------------------------ MMA issuer (a converged warp, one lane issues) ------
     constexpr uint32_t IDESC_S = make_idesc(1, 1, AP_BM, BN, 0, 0);  // Q K^T, both K-major
     constexpr uint32_t IDESC_O = make_idesc(1, 1, AP_BM, D, 0, 1);      // P V, V is MN-major
-    const uint64_t q_desc = make_smem_desc_sw128(smem_u32(q_smem), 16, 1024);
+    const uint64_t q_desc0 = make_smem_desc_sw128(smem_u32(q_smem), 16, 1024);
     const uint64_t k_desc0 = make_smem_desc_sw128(smem_u32(k_smem), 16, 1024);
     const uint64_t v_desc0 = make_smem_desc_sw128(smem_u32(v_smem), Cfg::KV_SUB, 1024);
     const bool issuer = elect_one();
-    auto issue_s = [&](int j) {
-      const int st = j % STAGES;
-      if (!mbar_wait_vote(&k_full[st], (j / STAGES) & 1, wc, DEV_TIMEOUT_ATTN_KV)) return false;
-      tc_fence_after_sync();
-      if (issuer) {
+    bool ok = true;
+    int nkv = 0;  // of the current query tile
+    auto next = [&](int i) {
+      if (i > 0) ok = mbar_wait_vote(&unit_full[i & 1], (i >> 1) & 1, wc, DEV_TIMEOUT_ATTN_Q);
+      if (!ok) return false;
+      const int len = __shfl_sync(0xffffffffu, s_unit[4 * (i & 1) + 1], 0), q0 = __shfl_sync(0xffffffffu, s_unit[4 * (i & 1) + 2], 0);
+      if (lane == 0) mbar_arrive(&unit_free[i & 1]);
+      nkv = key_tiles(len, q0);
+      return q0 >= 0;
+    };
+    // step t: scores of tile t, products of tile t - 1, across query tiles
+    int i = 0, j = 0;       // query tile, key tile in it
+    int pi = 0, pj = -1;    // those of tile t - 1; pj < 0: none
+    bool more = next(0);
+    for (int t = 0; ok && (more || pj >= 0); ++t) {
+      if (more) {
+        const int st = t % STAGES;
+        if (j == 0) ok = mbar_wait_vote(&q_full[i % Q_BUFS], (i / Q_BUFS) & 1, wc, DEV_TIMEOUT_ATTN_Q);
+        // the softmax warps have pulled the scores of tile t - 1 into registers
+        if (ok && t >= 1) ok = mbar_wait_vote(s_free, (t - 1) & 1, wc, DEV_TIMEOUT_ATTN_S);
+        if (ok) ok = mbar_wait_vote(&k_full[st], (t / STAGES) & 1, wc, DEV_TIMEOUT_ATTN_KV);
+        if (!ok) break;
+        tc_fence_after_sync();
+        if (issuer) {
+          const uint64_t q_desc = q_desc0 + static_cast<uint32_t>((i % Q_BUFS) * (Cfg::Q_BYTES >> 4));
+          const uint64_t k_desc = k_desc0 + static_cast<uint32_t>(st * (TILE >> 4));
 #pragma unroll
-        for (int k = 0; k < D / 16; ++k) {  // 16 of head_dim: 32 bytes of a 128-byte row, four to a 64-wide subtile
-          const uint64_t q_adv = static_cast<uint64_t>(((k / 4) * Cfg::Q_SUB + (k % 4) * 32) >> 4);
-          const uint64_t k_adv = static_cast<uint64_t>(((k / 4) * Cfg::KV_SUB + (k % 4) * 32) >> 4);
-          mma_f16_ss(tmem_base, q_desc + q_adv, k_desc0 + static_cast<uint32_t>(st * (TILE >> 4)) + k_adv, IDESC_S, k != 0);
+          for (int k = 0; k < D / 16; ++k) {  // 16 of head_dim: 32 bytes of a 128-byte row, four to a 64-wide subtile
+            const uint64_t q_adv = static_cast<uint64_t>(((k / 4) * Cfg::Q_SUB + (k % 4) * 32) >> 4);
+            const uint64_t k_adv = static_cast<uint64_t>(((k / 4) * Cfg::KV_SUB + (k % 4) * 32) >> 4);
+            mma_f16_ss(tmem_base, q_desc + q_adv, k_desc + k_adv, IDESC_S, k != 0);
+          }
+          mma_commit(&s_full[st]);
+          if (j == nkv - 1) mma_commit(&q_free[i % Q_BUFS]);
         }
-        mma_commit(&s_full[st]);
       }
-      return true;
-    };
-    auto issue_pv = [&](int j) {
-      const int st = j % STAGES;
-      if (!mbar_wait_vote(&v_full[st], (j / STAGES) & 1, wc, DEV_TIMEOUT_ATTN_KV)) return false;
-      if (!mbar_wait_vote(p_ready, j & 1, wc, DEV_TIMEOUT_ATTN_P)) return false;
-      tc_fence_after_sync();
-      if (issuer) {
+      if (pj >= 0) {
+        const int st = (t - 1) % STAGES;
+        ok = mbar_wait_vote(&v_full[st], ((t - 1) / STAGES) & 1, wc, DEV_TIMEOUT_ATTN_KV);
+        if (ok) ok = mbar_wait_vote(p_ready, (t - 1) & 1, wc, DEV_TIMEOUT_ATTN_P);
+        // the first products of a query tile take O over from the one before
+        if (ok && pj == 0 && pi > 0) ok = mbar_wait_vote(o_free, (pi - 1) & 1, wc, DEV_TIMEOUT_ATTN_O);
+        if (!ok) break;
+        tc_fence_after_sync();
+        if (issuer) {
+          const uint64_t v_desc = v_desc0 + static_cast<uint32_t>(st * (TILE >> 4));
 #pragma unroll
-        for (int k = 0; k < BN / 16; ++k)  // 16 keys: 8 columns of bf16 pairs, 16 rows of V (128 bytes each)
-          mma_f16_ts(tmem_base + Cfg::O_COL, tmem_base + Cfg::P_COL + (j % P_BUFS) * Cfg::P_COLS + 8 * k,
-                     v_desc0 + static_cast<uint32_t>(st * (TILE >> 4)) + static_cast<uint64_t>((k * 16 * 128) >> 4), IDESC_O,
-                     (j != 0 || k != 0));
-        mma_commit(&pv_done[st]);
+          for (int k = 0; k < BN / 16; ++k)  // 16 keys: 8 columns of bf16 pairs, 16 rows of V (128 bytes each)
+            mma_f16_ts(tmem_base + Cfg::O_COL, tmem_base + Cfg::P_COL + ((t - 1) % P_BUFS) * Cfg::P_COLS + 8 * k,
+                       v_desc + static_cast<uint64_t>((k * 16 * 128) >> 4), IDESC_O, (pj != 0 || k != 0));
+          mma_commit(&pv_done[st]);
+        }
       }
-      return true;
-    };
-    bool ok = mbar_wait_vote(q_full, 0, wc, DEV_TIMEOUT_ATTN_Q);
-    for (int j = 0; j <= nkv && ok; ++j) {
-      // the softmax warps have pulled the scores of tile j - 1 into registers
-      if (j >= 1 && j < nkv) ok = mbar_wait_vote(s_free, (j - 1) & 1, wc, DEV_TIMEOUT_ATTN_S);
-      if (ok && j < nkv) ok = issue_s(j);
-      if (ok && j >= 1) ok = issue_pv(j - 1);
+      pj = -1;
+      if (more) {
+        pi = i;
+        pj = j;
+        if (++j == nkv) {
+          j = 0;
+          more = next(++i);
+        }
+      }
     }
   } else {
     // ------------------------------ softmax + epilogue ------------------------
@@ -301,120 +371,140 @@ attention_packed_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
     const uint32_t lane_base = tmem_base + (static_cast<uint32_t>(quad * 32) << 16);
     const uint32_t s_tmem = lane_base, o_tmem = lane_base + Cfg::O_COL;
     const float c = a.scale_log2e;
-    const int seen = a.causal ? min(len, q0 + row + 1) : len;  // keys that this row sees, at least one
-    float m_used = -INFINITY;  // running maximum (raw score units) that the exponentials refer to
-    float2 l2 = make_float2(0.f, 0.f);
-    bool ok = true;
-    uint32_t pre_s = 0;  // early test of s_full for the coming tile
     uint32_t ra[32], rb[32], rc[32], rd[32];  // scores of a tile, then packed P (the last two: of 128 keys)
-    for (int j = 0; j < nkv; ++j) {
-      const int st = j % STAGES;
-      const int kv0 = j * BN;
-      const bool masked = kv0 + BN > len || (a.causal && kv0 + BN > q0 + 1);  // some row does not see all of its keys
-      const uint32_t p_tmem = lane_base + Cfg::P_COL + (j % P_BUFS) * Cfg::P_COLS;
-      const int stp = (j + STAGES - 1) % STAGES;                      // stage and parity of the
-      const uint32_t parp = j >= 1 ? ((j - 1) / STAGES) & 1 : 0;      // previous tile's products
-      if (!mbar_wait_pre(pre_s, &s_full[st], (j / STAGES) & 1, wc, DEV_TIMEOUT_ATTN_S)) { ok = false; break; }
-      tc_fence_after_sync();
-      auto half_step = [&](uint32_t (&r0)[32], uint32_t (&r1)[32], bool second) {
-        const float mx = max_of2(r0, r1);
-        const bool need = (mx - m_used) * c > 8.0f;  // always true in the very first half (m_used = -inf)
-        if (__any_sync(0xffffffffu, need)) {
-          float alpha = 1.0f;
-          if (need) {
-            alpha = ex2_approx((m_used - mx) * c);
-            m_used = mx;
-            l2.x *= alpha;
-            l2.y *= alpha;
+    bool ok = true;
+    for (int i = 0, t = 0; ok; ++i) {
+      if (i > 0 && !mbar_wait_warp(&unit_full[i & 1], (i >> 1) & 1, wc, DEV_TIMEOUT_ATTN_Q)) break;
+      const int* unit = s_unit + 4 * (i & 1);
+      const int begin = __shfl_sync(0xffffffffu, unit[0], 0), len = __shfl_sync(0xffffffffu, unit[1], 0);
+      const int q0 = __shfl_sync(0xffffffffu, unit[2], 0), h = __shfl_sync(0xffffffffu, unit[3], 0);
+      mbar_arrive_lane0(&unit_free[i & 1], lane);
+      if (q0 < 0) break;
+      const int nkv = key_tiles(len, q0);
+      const int seen = a.causal ? min(len, q0 + row + 1) : len;  // keys that this row sees, at least one
+      float m_used = -INFINITY;  // running maximum (raw score units) that the exponentials refer to
+      float2 l2 = make_float2(0.f, 0.f);
+      uint32_t pre_s = 0;  // early test of s_full for the coming tile
+      for (int j = 0; j < nkv; ++j, ++t) {
+        const int st = t % STAGES;
+        const int kv0 = j * BN;
+        const bool masked = kv0 + BN > len || (a.causal && kv0 + BN > q0 + 1);  // some row does not see all of its keys
+        const uint32_t p_tmem = lane_base + Cfg::P_COL + (t % P_BUFS) * Cfg::P_COLS;
+        const int stp = (t + STAGES - 1) % STAGES;                  // stage and parity of the
+        const uint32_t parp = t >= 1 ? ((t - 1) / STAGES) & 1 : 0;  // previous tile's products
+        if (!mbar_wait_pre(pre_s, &s_full[st], (t / STAGES) & 1, wc, DEV_TIMEOUT_ATTN_S)) { ok = false; break; }
+        tc_fence_after_sync();
+        auto half_step = [&](uint32_t (&r0)[32], uint32_t (&r1)[32], bool second) {
+          const float mx = max_of2(r0, r1);
+          const bool need = (mx - m_used) * c > 8.0f;  // always true in the very first half (m_used = -inf)
+          if (__any_sync(0xffffffffu, need)) {
+            float alpha = 1.0f;
+            if (need) {
+              alpha = ex2_approx((m_used - mx) * c);
+              m_used = mx;
+              l2.x *= alpha;
+              l2.y *= alpha;
+            }
+            if (j >= 1 && ok) {
+              ok = mbar_wait_warp(&pv_done[stp], parp, wc, DEV_TIMEOUT_ATTN_O);
+              if (ok) rescale_row<D>(o_tmem, alpha);
+            }
+            if (second) {  // the first half of P was formed against the older maximum
+              scale_packed(ra, alpha);
+              scale_packed(rb, alpha);
+            }
           }
-          if (j >= 1 && ok) {
-            ok = mbar_wait_warp(&pv_done[stp], parp, wc, DEV_TIMEOUT_ATTN_O);
-            if (ok) rescale_row<D>(o_tmem, alpha);
-          }
-          if (second) {  // the first half of P was formed against the older maximum
-            scale_packed(ra, alpha);
-            scale_packed(rb, alpha);
-          }
-        }
-        const float nmc = -m_used * c;
-        exp_pack<false>(r0, c, nmc, l2);
-        exp_pack<false>(r1, c, nmc, l2);
-      };
-      tmem_ld_32x32b_x32(s_tmem, ra);
-      tmem_ld_32x32b_x32(s_tmem + 32, rb);
-      tmem_wait_ld();
-      if constexpr (BN == 64) {
-        tc_fence_before_sync();
-        __syncwarp();
-        mbar_arrive_lane0(s_free, lane);  // the score buffer can take the next tile
-      }
-      if (masked) { mask_cols(ra, kv0, seen); mask_cols(rb, kv0 + 32, seen); }
-      half_step(ra, rb, false);
-      if constexpr (BN == 128) {
-        // the second half is only loaded now: with all 128 scores live the kernel spills
-        tmem_ld_32x32b_x32(s_tmem + 64, rc);
-        tmem_ld_32x32b_x32(s_tmem + 96, rd);
+          const float nmc = -m_used * c;
+          exp_pack<false>(r0, c, nmc, l2);
+          exp_pack<false>(r1, c, nmc, l2);
+        };
+        tmem_ld_32x32b_x32(s_tmem, ra);
+        tmem_ld_32x32b_x32(s_tmem + 32, rb);
         tmem_wait_ld();
+        if constexpr (BN == 64) {
+          tc_fence_before_sync();
+          __syncwarp();
+          mbar_arrive_lane0(s_free, lane);  // the score buffer can take the next tile
+        }
+        if (masked) { mask_cols(ra, kv0, seen); mask_cols(rb, kv0 + 32, seen); }
+        half_step(ra, rb, false);
+        // Products of an earlier query tile are complete: its epilogue has waited for the last ones.
+        if constexpr (BN == 128) {
+          // the second half is only loaded now: with all 128 scores live the kernel spills
+          tmem_ld_32x32b_x32(s_tmem + 64, rc);
+          tmem_ld_32x32b_x32(s_tmem + 96, rd);
+          tmem_wait_ld();
+          tc_fence_before_sync();
+          __syncwarp();
+          mbar_arrive_lane0(s_free, lane);  // the score buffer can take the next tile
+          if (masked) { mask_cols(rc, kv0 + 64, seen); mask_cols(rd, kv0 + 96, seen); }
+          uint32_t pre_pv = 1;
+          if (j >= 1) pre_pv = mbar_test_wait(&pv_done[stp], parp);
+          half_step(rc, rd, true);
+          // P is free once the products of the previous tile are complete (tested half a tile ago)
+          if (j >= 1 && ok) ok = mbar_wait_pre(pre_pv, &pv_done[stp], parp, wc, DEV_TIMEOUT_ATTN_O);
+        } else {
+          // this buffer of P is free once the products of the tile before the last are complete
+          if (j >= 2 && ok) ok = mbar_wait_warp(&pv_done[st], ((t - 2) / STAGES) & 1, wc, DEV_TIMEOUT_ATTN_O);
+        }
+        if (!ok) break;
+        tmem_st_32x32b_x16(p_tmem, reinterpret_cast<uint32_t(&)[16]>(ra));
+        tmem_st_32x32b_x16(p_tmem + 16, reinterpret_cast<uint32_t(&)[16]>(rb));
+        if constexpr (BN == 128) {
+          tmem_st_32x32b_x16(p_tmem + 32, reinterpret_cast<uint32_t(&)[16]>(rc));
+          tmem_st_32x32b_x16(p_tmem + 48, reinterpret_cast<uint32_t(&)[16]>(rd));
+        }
+        if (kv0 + BN > len) {
+          // rows of V behind the sequence's end become zeros, whatever they are
+          ok = mbar_wait_warp(&v_full[st], (t / STAGES) & 1, wc, DEV_TIMEOUT_ATTN_KV);
+          if (ok && row < BN && kv0 + row >= len) {
+#pragma unroll
+            for (int s = 0; s < SUBS; ++s)
+#pragma unroll
+              for (int k = 0; k < 8; ++k)
+                *reinterpret_cast<uint4*>(v_smem + st * TILE + s * Cfg::KV_SUB + row * 128 + k * 16) = make_uint4(0, 0, 0, 0);
+          }
+          fence_proxy_async_smem();
+        }
+        pre_s = 0;
+        if (j + 1 < nkv) pre_s = mbar_test_wait(&s_full[(t + 1) % STAGES], ((t + 1) / STAGES) & 1);
+        tmem_wait_st();
         tc_fence_before_sync();
         __syncwarp();
-        mbar_arrive_lane0(s_free, lane);  // the score buffer can take the next tile
-        if (masked) { mask_cols(rc, kv0 + 64, seen); mask_cols(rd, kv0 + 96, seen); }
-        uint32_t pre_pv = 1;
-        if (j >= 1) pre_pv = mbar_test_wait(&pv_done[stp], parp);
-        half_step(rc, rd, true);
-        // P is free once the products of the previous tile are complete (tested half a tile ago)
-        if (j >= 1 && ok) ok = mbar_wait_pre(pre_pv, &pv_done[stp], parp, wc, DEV_TIMEOUT_ATTN_O);
-      } else {
-        // this buffer of P is free once the products of the tile before the last are complete
-        if (j >= 2 && ok) ok = mbar_wait_warp(&pv_done[st], ((j - 2) / STAGES) & 1, wc, DEV_TIMEOUT_ATTN_O);
+        mbar_arrive_lane0(p_ready, lane);
       }
-      if (!ok) break;
-      tmem_st_32x32b_x16(p_tmem, reinterpret_cast<uint32_t(&)[16]>(ra));
-      tmem_st_32x32b_x16(p_tmem + 16, reinterpret_cast<uint32_t(&)[16]>(rb));
-      if constexpr (BN == 128) {
-        tmem_st_32x32b_x16(p_tmem + 32, reinterpret_cast<uint32_t(&)[16]>(rc));
-        tmem_st_32x32b_x16(p_tmem + 48, reinterpret_cast<uint32_t(&)[16]>(rd));
-      }
-      if (kv0 + BN > len) {
-        // rows of V behind the sequence's end become zeros, whatever they are
-        ok = mbar_wait_warp(&v_full[st], (j / STAGES) & 1, wc, DEV_TIMEOUT_ATTN_KV);
-        if (ok && row < BN && kv0 + row >= len) {
-#pragma unroll
-          for (int s = 0; s < SUBS; ++s)
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-              *reinterpret_cast<uint4*>(v_smem + st * TILE + s * Cfg::KV_SUB + row * 128 + i * 16) = make_uint4(0, 0, 0, 0);
-        }
-        fence_proxy_async_smem();
-      }
-      pre_s = 0;
-      if (j + 1 < nkv) pre_s = mbar_test_wait(&s_full[(j + 1) % STAGES], ((j + 1) / STAGES) & 1);
-      tmem_wait_st();
-      tc_fence_before_sync();
-      __syncwarp();
-      mbar_arrive_lane0(p_ready, lane);
-    }
-    const float l = l2.x + l2.y;
-    if (ok && mbar_wait_warp(&pv_done[(nkv - 1) % STAGES], ((nkv - 1) / STAGES) & 1, wc, DEV_TIMEOUT_ATTN_O)) {
+      if (!ok || !mbar_wait_warp(&pv_done[(t - 1) % STAGES], ((t - 1) / STAGES) & 1, wc, DEV_TIMEOUT_ATTN_O)) break;
       tc_fence_after_sync();
-      const float inv = 1.0f / l;
+      const float inv = 1.0f / (l2.x + l2.y);
       uint4* to = reinterpret_cast<uint4*>(a.out + static_cast<long>(begin + q0 + row) * a.ldo + h * D);
-#pragma unroll 1
-      for (int part = 0; part < D / 32; ++part) {
-        uint32_t o[32];
-        tmem_ld_32x32b_x32(o_tmem + 32 * part, o);
-        tmem_wait_ld();
+      auto store = [&](uint32_t (&o)[32], int part) {
         if (q0 + row < len) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
+          for (int k = 0; k < 4; ++k) {
             uint4 u;
-            u.x = pack_bf16x2(__uint_as_float(o[8 * i]) * inv, __uint_as_float(o[8 * i + 1]) * inv);
-            u.y = pack_bf16x2(__uint_as_float(o[8 * i + 2]) * inv, __uint_as_float(o[8 * i + 3]) * inv);
-            u.z = pack_bf16x2(__uint_as_float(o[8 * i + 4]) * inv, __uint_as_float(o[8 * i + 5]) * inv);
-            u.w = pack_bf16x2(__uint_as_float(o[8 * i + 6]) * inv, __uint_as_float(o[8 * i + 7]) * inv);
-            to[4 * part + i] = u;
+            u.x = pack_bf16x2(__uint_as_float(o[8 * k]) * inv, __uint_as_float(o[8 * k + 1]) * inv);
+            u.y = pack_bf16x2(__uint_as_float(o[8 * k + 2]) * inv, __uint_as_float(o[8 * k + 3]) * inv);
+            u.z = pack_bf16x2(__uint_as_float(o[8 * k + 4]) * inv, __uint_as_float(o[8 * k + 5]) * inv);
+            u.w = pack_bf16x2(__uint_as_float(o[8 * k + 6]) * inv, __uint_as_float(o[8 * k + 7]) * inv);
+            to[4 * part + k] = u;
           }
         }
+      };
+      tmem_ld_32x32b_x32(o_tmem, ra);
+      tmem_ld_32x32b_x32(o_tmem + 32, rb);
+      if constexpr (D == 128) {
+        tmem_ld_32x32b_x32(o_tmem + 64, rc);
+        tmem_ld_32x32b_x32(o_tmem + 96, rd);
+      }
+      tmem_wait_ld();
+      tc_fence_before_sync();
+      __syncwarp();
+      mbar_arrive_lane0(o_free, lane);  // the next query tile's products may begin
+      store(ra, 0);
+      store(rb, 1);
+      if constexpr (D == 128) {
+        store(rc, 2);
+        store(rd, 3);
       }
     }
   }
@@ -763,7 +853,10 @@ int launch_inst(const CUtensorMap* tm, const PackedArgs& a, long units, cudaStre
   static bool done[64] = {false};
   int rc = prepare_kernel(kern, ApCfg<D>::SMEM_BYTES, 0, done);
   if (rc) return rc;
-  launch_dependent(kern, static_cast<unsigned>(units * a.heads), AP_THREADS, ApCfg<D>::SMEM_BYTES, stream, tm[0], tm[1], tm[2], a);
+  const long tiles = units * a.heads, slots = 2L * device_sm_count();
+  const bool rounds = tiles > slots && packed_rounds(a.rows, a.count);
+  launch_dependent(kern, static_cast<unsigned>(rounds ? slots : tiles), AP_THREADS, ApCfg<D>::SMEM_BYTES, stream, tm[0],
+                   tm[1], tm[2], a);
   return after_launch("attention_packed_kernel");
 }
 

@@ -107,4 +107,8 @@ inline bool packed_two_heads(int head_dim, int group, int rows, int count) {
   return head_dim == 128 && group % 2 == 0 && rows >= 256L * count;
 }
 
+// Packed attention, one head a CTA: whether the CTAs that fit the SMs go through the tiles in rounds, or each tile has a CTA of
+// its own (where tiles are long, the order in which SMs become free shares them out better).
+inline bool packed_rounds(int rows, int count) { return rows < 1024L * count; }
+
 }  // namespace sd3
