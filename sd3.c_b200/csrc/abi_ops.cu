@@ -428,7 +428,7 @@ int sd3_layer_norm_backward(const void* dy, long lddy, const void* x, long ldx, 
     return SD3_ERR_INVALID_ARG;
   }
   return launch_layer_norm_backward(dy, lddy, x, ldx, dtype == SD3_DTYPE_F32, w, mean, rstd, dx, dw, db, rows, C,
-                                    static_cast<float*>(scratch), S(stream));
+                                    static_cast<float*>(scratch), status_word_for(S(stream)), S(stream));
 }
 
 int sd3_skinny_linear(const float* in, long ld_in, const void* w, int w_dtype, const float* bias,

@@ -267,7 +267,7 @@ int launch_layer_norm(const void* x, long ldx, int f32, const float* w, const fl
 size_t layer_norm_backward_scratch_bytes(long rows, int C);
 int launch_layer_norm_backward(const void* dy, long lddy, const void* x, long ldx, int f32, const float* w,
                                const float* mean, const float* rstd, void* dx, float* dw, float* db, long rows, int C,
-                               float* scratch, cudaStream_t stream);
+                               float* scratch, int* dev_status, cudaStream_t stream);
 
 // Skinny linear for M = B <= 64 rows:  out[b, n] = act_out(sum_k in[b,k] W[n,k] + bias[n] + add[b,n])
 // W is (N, K) row-major, bf16 or fp32 (w_f32).  act: 0 none, 1 SiLU.  w_static: no kernel that may

@@ -25,6 +25,7 @@ constexpr int LNB_THREADS = 512;   // at most, of a CTA
 constexpr int LNB_PER_THREAD = 16; // values of a row that a thread holds, at most
 constexpr int LNB_MAX_C = LNB_THREADS * LNB_PER_THREAD;  // wider rows: the kernels at the end of this file
 constexpr int LNB_MAX_WARPS = LNB_THREADS / 32;
+constexpr int LNB_MAX_TEAMS = 15;  // of several warps: named barriers 1 to 15
 
 // VEC values of type T as they lie in memory: 16 bytes, or one value where rows are not 16-byte aligned
 template <typename T, int VEC>
@@ -93,6 +94,7 @@ struct LnFwdArgs {
   float eps;
 };
 
+// One or two rows a team: weight and bias on their way with the row.
 template <typename T, int VEC, int NV, int LANES>
 __global__ void __launch_bounds__(LNB_THREADS, 1) layer_norm_kernel(const __grid_constant__ LnFwdArgs a) {
   __shared__ float2 part[2][LNB_MAX_WARPS];  // mean and squared deviations of each warp, two rows' worth
@@ -159,9 +161,11 @@ __global__ void __launch_bounds__(LNB_THREADS, 1) layer_norm_kernel(const __grid
       if ((threadIdx.x & 31) == 0) part[buf][warp] = make_float2(mean, m2);
       team_barrier(1 + team, ts);
       float s = 0.f;
+#pragma unroll 4
       for (int k = 0; k < a.warps; ++k) s = fmaf(part[buf][warp0 + k].x, n_of[warp0 + k], s);
       mean = s * inv_c;
       m2 = 0.f;
+#pragma unroll 4
       for (int k = 0; k < a.warps; ++k) {
         const float2 p = part[buf][warp0 + k];
         m2 += fmaf((p.x - mean) * (p.x - mean), n_of[warp0 + k], p.y);
@@ -178,6 +182,152 @@ __global__ void __launch_bounds__(LNB_THREADS, 1) layer_norm_kernel(const __grid
           float o[VEC];
 #pragma unroll
           for (int j = 0; j < VEC; ++j) o[j] = fmaf((v[i][j] - mean) * rstd, w[i][j], b[i][j]);
+          Raw<T, VEC>::store(out + c * VEC, o);
+        }
+      }
+      if (t == 0) {
+        if (a.mean) a.mean[row] = mean;
+        if (a.rstd) a.rstd[row] = rstd;
+      }
+    }
+  }
+}
+
+// Several rows a team: weight and bias in shared memory, so that two CTAs of 512 threads fit an SM (in registers, 32 more a thread,
+// one does: 32768 x 1536, bf16, 52 us against 46; fp32 105 against 79).  VEC 8: the lower halves of all pieces, then the upper ones, so that the 16 bytes that
+// neighbouring threads read are neighbours.
+template <int VEC>
+__device__ __forceinline__ int vector_at(int c, int nvec) {  // of column c
+  if constexpr (VEC == 8) return ((c >> 2) & 1) * 4 * nvec + (c >> 3) * 4 + (c & 3);
+  return c;
+}
+template <int VEC>
+__device__ __forceinline__ void stage_vector(float* to, const float* from, float otherwise, int C) {
+  for (int c = threadIdx.x; c < C; c += blockDim.x) to[vector_at<VEC>(c, C / VEC)] = from ? from[c] : otherwise;
+}
+// piece c of a vector
+template <int VEC>
+__device__ __forceinline__ void staged(const float* v, int c, int nvec, float (&f)[VEC]) {
+  if constexpr (VEC == 1) {
+    f[0] = v[c];
+  } else {
+#pragma unroll
+    for (int h = 0; h < VEC / 4; ++h) {
+      const float4 t = reinterpret_cast<const float4*>(v)[h * nvec + c];
+      f[4 * h] = t.x; f[4 * h + 1] = t.y; f[4 * h + 2] = t.z; f[4 * h + 3] = t.w;
+    }
+  }
+}
+
+// sums over one piece, two values an instruction
+template <int VEC>
+__device__ __forceinline__ float sum_of(const float (&v)[VEC]) {
+  if constexpr (VEC == 1) return v[0];
+  float2 s = make_float2(v[0], v[1]);
+#pragma unroll
+  for (int j = 2; j < VEC; j += 2) s = __fadd2_rn(s, make_float2(v[j], v[j + 1]));
+  return s.x + s.y;
+}
+template <int VEC>
+__device__ __forceinline__ float squares_of(const float (&v)[VEC], float mean) {
+  if constexpr (VEC == 1) return (v[0] - mean) * (v[0] - mean);
+  float2 s = make_float2(0.f, 0.f);
+#pragma unroll
+  for (int j = 0; j < VEC; j += 2) {
+    const float2 d = __fadd2_rn(make_float2(v[j], v[j + 1]), make_float2(-mean, -mean));
+    s = __ffma2_rn(d, d, s);
+  }
+  return s.x + s.y;
+}
+
+template <typename T, int VEC, int NV, int LANES>
+__global__ void __launch_bounds__(LNB_THREADS, 2) layer_norm_many_kernel(const __grid_constant__ LnFwdArgs a) {
+  extern __shared__ __align__(16) float vectors[];  // w, b
+  __shared__ float2 part[2][LNB_MAX_WARPS];  // mean and squared deviations of each warp, two rows' worth
+  __shared__ float n_of[LNB_MAX_WARPS];      // values that each warp holds of a row
+  grid_dep_wait();
+  grid_dep_launch();
+  const int ts = a.warps > 1 ? 32 * a.warps : LANES;  // threads of a team
+  const int team = threadIdx.x / ts, t = threadIdx.x % ts;
+  const int warp0 = team * a.warps;  // the team's first warp (several warps a team)
+  const int nvec = a.C / VEC;
+  const float inv_c = 1.0f / static_cast<float>(a.C);
+  const long step = static_cast<long>(gridDim.x) * a.teams;
+  const long first = static_cast<long>(blockIdx.x) * a.teams;
+  Raw<T, VEC> next[NV];
+  auto request = [&](long row) {
+    const T* p = static_cast<const T*>(a.x) + row * a.ldx;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = t + i * ts;
+      if (row < a.rows && c < nvec) next[i].load(p + c * VEC);
+      else next[i].zero();
+    }
+  };
+  request(first + team);
+  stage_vector<VEC>(vectors, a.w, 1.f, a.C);
+  stage_vector<VEC>(vectors + a.C, a.b, 0.f, a.C);
+  int count = 0;  // values of this thread
+#pragma unroll
+  for (int i = 0; i < NV; ++i) count += t + i * ts < nvec ? VEC : 0;
+  const float n_warp = lanes_sum<LANES>(static_cast<float>(count));
+  const float inv_n = n_warp > 0.f ? 1.0f / n_warp : 0.f;
+  if ((threadIdx.x & 31) == 0) n_of[threadIdx.x >> 5] = n_warp;
+  __syncthreads();
+  int buf = 0;
+  // `base` is the same for the whole CTA: lanes of one warp may belong to teams with and without a row
+  for (long base = first; base < a.rows; base += step) {
+    const long row = base + team;
+    float v[NV][VEC];
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      next[i].get(v[i]);
+      sum += sum_of<VEC>(v[i]);
+    }
+    request(row + step);
+    float mean = lanes_sum<LANES>(sum) * inv_n;
+    float m2 = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      if (t + i * ts < nvec) m2 += squares_of<VEC>(v[i], mean);
+    m2 = lanes_sum<LANES>(m2);
+    if (a.warps > 1) {
+      if ((threadIdx.x & 31) == 0) part[buf][threadIdx.x >> 5] = make_float2(mean, m2);
+      team_barrier(1 + team, ts);
+      float total = 0.f;
+#pragma unroll 4
+      for (int k = 0; k < a.warps; ++k) total = fmaf(part[buf][warp0 + k].x, n_of[warp0 + k], total);
+      mean = total * inv_c;
+      m2 = 0.f;
+#pragma unroll 4
+      for (int k = 0; k < a.warps; ++k) {
+        const float2 p = part[buf][warp0 + k];
+        m2 += fmaf((p.x - mean) * (p.x - mean), n_of[warp0 + k], p.y);
+      }
+      buf ^= 1;
+    }
+    const float rstd = 1.0f / sqrtf(m2 * inv_c + a.eps);
+    if (row < a.rows) {
+      T* out = static_cast<T*>(a.y) + row * a.C;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int c = t + i * ts;
+        if (c < nvec) {
+          float w[VEC], b[VEC], o[VEC];
+          staged<VEC>(vectors, c, nvec, w);
+          staged<VEC>(vectors + a.C, c, nvec, b);
+          if constexpr (VEC == 1) {
+            o[0] = fmaf((v[i][0] - mean) * rstd, w[0], b[0]);
+          } else {
+#pragma unroll
+            for (int j = 0; j < VEC; j += 2) {
+              const float2 u = __fmul2_rn(__fadd2_rn(make_float2(v[i][j], v[i][j + 1]), make_float2(-mean, -mean)), make_float2(rstd, rstd));
+              const float2 y = __ffma2_rn(u, make_float2(w[j], w[j + 1]), make_float2(b[j], b[j + 1]));
+              o[j] = y.x;
+              o[j + 1] = y.y;
+            }
+          }
           Raw<T, VEC>::store(out + c * VEC, o);
         }
       }
@@ -335,26 +485,214 @@ __global__ void __launch_bounds__(LNB_THREADS, 1) layer_norm_backward_kernel(con
   for (int c = threadIdx.x; c < 2 * a.C; c += blockDim.x) out[c] = sums[c];
 }
 
-// dw and db: the sums of `parts` partial rows of 2 C values.  A thread adds every eighth of its column's, then the
-// eight threads of a column are added up.
-__global__ void __launch_bounds__(256) layer_norm_columns_kernel(const float* partial, int parts, int C, float* dw,
-                                                                 float* db) {
-  __shared__ float s[8][32];
+// dw and db: the sums of `parts` partial rows of 2 C values.  Thread k of the 32 of a column adds parts k, k + 32, ...; then the
+// 32 are added up in order.
+__global__ void __launch_bounds__(1024) layer_norm_columns_kernel(const float* partial, int parts, int C, float* dw, float* db) {
+  __shared__ float s[32][33];
   grid_dep_wait();
   grid_dep_launch();
-  const int col = blockIdx.x * 32 + (threadIdx.x & 31), k0 = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31, k0 = threadIdx.x >> 5;
+  const int col = blockIdx.x * 32 + lane;
   float v = 0.f;
-  if (col < 2 * C)
-    for (int k = k0; k < parts; k += 8) v += partial[static_cast<long>(k) * 2 * C + col];
-  s[k0][threadIdx.x & 31] = v;
+  if (col < 2 * C) {
+#pragma unroll 8
+    for (int k = k0; k < parts; k += 32) v += partial[static_cast<long>(k) * 2 * C + col];
+  }
+  s[k0][lane] = v;
   __syncthreads();
   if (k0 == 0 && col < 2 * C) {
     float r = 0.f;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) r += s[k][threadIdx.x & 31];
+    for (int k = 0; k < 32; ++k) r += s[k][lane];
     float* out = col < C ? dw : db;
     if (out) out[col < C ? col : col - C] = r;
   }
+}
+
+// ----------------------------------------------------------------------------
+// Backward of aligned rows of 512 bytes and more: the same teams, with rows that come through shared memory.  Each team has a ring
+// of its own, `depth` rows of x and dy that its first thread requests ahead by bulk copies; behind the team's barrier of a row
+// everyone has finished the row before, whose place is then requested anew.  With neither the coming row nor the weight in
+// registers, 1024 threads fit an SM.
+// ----------------------------------------------------------------------------
+constexpr int LNR_THREADS = 1024;
+constexpr int LNR_MAX_WARPS = LNR_THREADS / 32;
+constexpr int LNR_SMEM = 200 * 1024;
+
+struct LnRing {
+  int depth, row_bytes;
+  int* status;
+};
+
+template <typename T>
+struct Vec16;
+template <>
+struct Vec16<bf16> {
+  static constexpr int N = 8;
+  __device__ __forceinline__ static void load(const uint8_t* p, float (&f)[8]) {
+    const uint4 v = *reinterpret_cast<const uint4*>(p);
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      f[2 * i] = __uint_as_float(w[i] << 16);
+      f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+  }
+};
+template <>
+struct Vec16<float> {
+  static constexpr int N = 4;
+  __device__ __forceinline__ static void load(const uint8_t* p, float (&f)[4]) {
+    const float4 v = *reinterpret_cast<const float4*>(p);
+    f[0] = v.x; f[1] = v.y; f[2] = v.z; f[3] = v.w;
+  }
+};
+
+template <typename T, int NV>
+__global__ void __launch_bounds__(LNR_THREADS, 1) layer_norm_backward_ring_kernel(const __grid_constant__ LnBwdArgs a,
+                                                                                  const __grid_constant__ LnRing ring) {
+  constexpr int VEC = Vec16<T>::N;
+  extern __shared__ __align__(16) uint8_t ring_smem[];  // w, then the rings (x, dy of a row next to each other); at the end 2 C sums
+  float* w_smem = reinterpret_cast<float*>(ring_smem);
+  uint8_t* rows_smem = ring_smem + 4 * a.C;
+  __shared__ float2 part[2][LNR_MAX_WARPS];
+  __shared__ uint64_t full[LNR_MAX_WARPS * 8];
+  __shared__ int s_abort;
+  const int ts = 32 * a.warps, team = threadIdx.x / ts, t = threadIdx.x % ts, warp0 = team * a.warps;
+  const int nvec = a.C / VEC;
+  uint64_t* bar = full + team * 8;
+  uint8_t* mine = rows_smem + static_cast<long>(team) * ring.depth * 2 * ring.row_bytes;
+  if (t == 0) {
+    for (int s = 0; s < ring.depth; ++s) mbar_init(&bar[s], 1);
+    if (threadIdx.x == 0) s_abort = 0;
+    fence_barrier_init();
+  }
+  __syncthreads();
+  grid_dep_wait();
+  grid_dep_launch();
+  const WaitCtx wc{&s_abort, ring.status};
+  const long step = static_cast<long>(gridDim.x) * a.teams;
+  const long first = static_cast<long>(blockIdx.x) * a.teams + team;
+  auto request = [&](long row, int s) {
+    if (row < a.rows) {
+      uint8_t* to = mine + s * 2 * ring.row_bytes;
+      mbar_expect_tx(&bar[s], 2 * ring.row_bytes);
+      bulk_load(to, static_cast<const T*>(a.x) + row * a.ldx, ring.row_bytes, &bar[s]);
+      bulk_load(to + ring.row_bytes, static_cast<const T*>(a.dy) + row * a.lddy, ring.row_bytes, &bar[s]);
+    }
+  };
+  if (t == 0)
+    for (int s = 0; s < ring.depth; ++s) request(first + s * step, s);
+  stage_vector<VEC>(w_smem, a.w, 1.f, a.C);
+  __syncthreads();
+  float2 dw[NV][VEC / 2], db[NV][VEC / 2];
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+#pragma unroll
+    for (int j = 0; j < VEC / 2; ++j) dw[i][j] = db[i][j] = make_float2(0.f, 0.f);
+  const float inv_c = 1.0f / static_cast<float>(a.C);
+  float next_mean = first < a.rows ? a.mean[first] : 0.f, next_rstd = first < a.rows ? a.rstd[first] : 0.f;
+  int buf = 0, s = 0, s_before = 0;
+  uint32_t parity = 0;
+  for (long row = first; row < a.rows; row += step) {
+    const float mean = next_mean, rstd = next_rstd;
+    if (row + step < a.rows) {
+      next_mean = a.mean[row + step];
+      next_rstd = a.rstd[row + step];
+    }
+    if (!mbar_wait(&bar[s], parity, wc, DEV_TIMEOUT_LN_ROW)) break;
+    const uint8_t* px = mine + s * 2 * ring.row_bytes;
+    float2 sg2 = make_float2(0.f, 0.f), sgu2 = sg2;
+    const float2 m2 = make_float2(-mean, -mean), r2 = make_float2(rstd, rstd);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = t + i * ts;
+      if (c < nvec) {
+        float x[VEC], dy[VEC], w[VEC];
+        Vec16<T>::load(px + c * 16, x);
+        Vec16<T>::load(px + ring.row_bytes + c * 16, dy);
+        staged<VEC>(w_smem, c, nvec, w);
+#pragma unroll
+        for (int j = 0; j < VEC; j += 2) {
+          const float2 d = make_float2(dy[j], dy[j + 1]);
+          const float2 u = __fmul2_rn(__fadd2_rn(make_float2(x[j], x[j + 1]), m2), r2), g = __fmul2_rn(d, make_float2(w[j], w[j + 1]));
+          sg2 = __fadd2_rn(sg2, g);
+          sgu2 = __ffma2_rn(g, u, sgu2);
+          dw[i][j / 2] = __ffma2_rn(d, u, dw[i][j / 2]);
+          db[i][j / 2] = __fadd2_rn(db[i][j / 2], d);
+        }
+      }
+    }
+    float sg = lanes_sum<32>(sg2.x + sg2.y), sgu = lanes_sum<32>(sgu2.x + sgu2.y);
+    if (a.warps > 1) {
+      if ((threadIdx.x & 31) == 0) part[buf][threadIdx.x >> 5] = make_float2(sg, sgu);
+      team_barrier(1 + team, ts);
+      sg = 0.f;
+      sgu = 0.f;
+#pragma unroll 4
+      for (int k = 0; k < a.warps; ++k) {
+        sg += part[buf][warp0 + k].x;
+        sgu += part[buf][warp0 + k].y;
+      }
+      buf ^= 1;
+    } else {
+      __syncwarp();
+    }
+    // everyone has finished the row before, which is read twice
+    if (t == 0 && row != first) request(row + (ring.depth - 1) * step, s_before);
+    s_before = s;
+    if (++s == ring.depth) { s = 0; parity ^= 1; }
+    const float mg = sg * inv_c, mgu = sgu * inv_c;
+    T* out = static_cast<T*>(a.dx) + row * a.C;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = t + i * ts;
+      if (c < nvec) {
+        float x[VEC], dy[VEC], w[VEC], o[VEC];
+        Vec16<T>::load(px + c * 16, x);
+        Vec16<T>::load(px + ring.row_bytes + c * 16, dy);
+        staged<VEC>(w_smem, c, nvec, w);
+#pragma unroll
+        for (int j = 0; j < VEC; j += 2) {
+          const float2 u = __fmul2_rn(__fadd2_rn(make_float2(x[j], x[j + 1]), m2), r2);
+          const float2 g = __ffma2_rn(make_float2(dy[j], dy[j + 1]), make_float2(w[j], w[j + 1]), make_float2(-mg, -mg));
+          const float2 d = __fmul2_rn(__ffma2_rn(u, make_float2(-mgu, -mgu), g), r2);
+          o[j] = d.x;
+          o[j + 1] = d.y;
+        }
+        Raw<T, VEC>::store(out + c * VEC, o);
+      }
+    }
+  }
+  __syncthreads();  // every row has landed and been read: the rings hold the sums from here on
+  if (s_abort) drain_after_abort();
+  float4* sums = reinterpret_cast<float4*>(rows_smem);
+  for (int k = 0; k < a.teams; ++k) {
+    if (team == k) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int c = t + i * ts;
+        if (c < nvec) {
+#pragma unroll
+          for (int j = 0; j < VEC; j += 4) {
+            float4 p = make_float4(dw[i][j / 2].x, dw[i][j / 2].y, dw[i][j / 2 + 1].x, dw[i][j / 2 + 1].y);
+            float4 q = make_float4(db[i][j / 2].x, db[i][j / 2].y, db[i][j / 2 + 1].x, db[i][j / 2 + 1].y);
+            float4 *sp = sums + (c * VEC + j) / 4, *sq = sums + (a.C + c * VEC + j) / 4;
+            if (k > 0) {
+              const float4 op = *sp, oq = *sq;
+              p.x += op.x; p.y += op.y; p.z += op.z; p.w += op.w;
+              q.x += oq.x; q.y += oq.y; q.z += oq.z; q.w += oq.w;
+            }
+            *sp = p;
+            *sq = q;
+          }
+        }
+      }
+    }
+    __syncthreads();
+  }
+  float4* out = reinterpret_cast<float4*>(a.partial + static_cast<long>(blockIdx.x) * 2 * a.C);
+  for (int c = threadIdx.x; c < a.C / 2; c += blockDim.x) out[c] = sums[c];
 }
 
 // ----------------------------------------------------------------------------
@@ -512,14 +850,30 @@ int with_shape(const LnShape& s, bool f32, const F& f) {
   return s.vec == 8 ? with_pieces<bf16, 8>(s, f) : with_pieces<bf16, 1>(s, f);
 }
 
+template <typename K>
+int allow_smem(K kern, size_t smem, size_t most) {
+  if (smem <= 40 * 1024) return ST_OK;
+  return check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(most)),
+                    "cudaFuncSetAttribute(layer_norm)");
+}
+
 struct LaunchForward {
   const LnFwdArgs& a;
+  bool many;
   int grid, threads;
   cudaStream_t stream;
   template <typename T, int VEC, int NV, int LANES>
   int run() const {
-    launch_dependent(layer_norm_kernel<T, VEC, NV, LANES>, grid, threads, 0, stream, a);
-    return after_launch("layer_norm_kernel");
+    if (!many) {
+      launch_dependent(layer_norm_kernel<T, VEC, NV, LANES>, grid, threads, 0, stream, a);
+      return after_launch("layer_norm_kernel");
+    }
+    auto kern = layer_norm_many_kernel<T, VEC, NV, LANES>;
+    const size_t smem = 2 * sizeof(float) * a.C;
+    int rc = allow_smem(kern, smem, 2 * sizeof(float) * LNB_MAX_C);
+    if (rc) return rc;
+    launch_dependent(kern, grid, threads, smem, stream, a);
+    return after_launch("layer_norm_many_kernel");
   }
 };
 
@@ -542,6 +896,42 @@ struct LaunchBackward {
   }
 };
 
+// The ring kernels: f.template run<T, NV>() of the shape
+template <typename F>
+int with_ring(const LnShape& s, bool f32, const F& f) {
+  if (f32) return s.nv == 1 ? f.template run<float, 1>() : s.nv == 2 ? f.template run<float, 2>() : f.template run<float, 4>();
+  return s.nv == 1 ? f.template run<bf16, 1>() : f.template run<bf16, 2>();
+}
+
+struct LaunchBackwardRing {
+  const LnBwdArgs& a;
+  const LnRing& ring;
+  int grid, threads;
+  size_t smem;
+  cudaStream_t stream;
+  template <typename T, int NV>
+  int run() const {
+    int rc = allow_smem(layer_norm_backward_ring_kernel<T, NV>, smem, LNR_SMEM);
+    if (rc) return rc;
+    launch_dependent(layer_norm_backward_ring_kernel<T, NV>, grid, threads, smem, stream, a, ring);
+    return after_launch("layer_norm_backward_ring_kernel");
+  }
+};
+
+// The ring of a team: at least two rows, eight at most, no more than the team goes through and shared memory holds.
+LnRing ring_for(const LnShape& s, int C, int row_bytes, long rows, int grid, int* status) {
+  LnRing r;
+  const long per_team = (rows + static_cast<long>(grid) * s.teams - 1) / (static_cast<long>(grid) * s.teams);
+  long depth = (LNR_SMEM - 4L * C) / (2L * s.teams * row_bytes);
+  if (depth > 8) depth = 8;
+  if (depth > per_team) depth = per_team;
+  if (depth < 2) depth = 2;
+  r.depth = static_cast<int>(depth);
+  r.row_bytes = row_bytes;
+  r.status = status;
+  return r;
+}
+
 // widest row that a CTA's registers hold
 bool row_fits(int C, const LnShape& s) {
   return C <= s.vec * 32 * s.nv * s.warps;
@@ -561,10 +951,11 @@ int launch_layer_norm(const void* x, long ldx, int f32, const float* w, const fl
     launch_dependent(f32 ? layer_norm_wide_kernel<float> : layer_norm_wide_kernel<bf16>, grid, LNB_THREADS, 0, stream, a);
     return after_launch("layer_norm_wide_kernel");
   }
-  const int grid = fit_teams(&s, rows, sms);
+  const bool many = rows > 2L * sms * s.teams;
+  const int grid = fit_teams(&s, rows, many ? 2 * sms : sms);
   a.warps = s.warps;
   a.teams = s.teams;
-  return with_shape(s, f32 != 0, LaunchForward{a, grid, cta_threads(s), stream});
+  return with_shape(s, f32 != 0, LaunchForward{a, many, grid, cta_threads(s), stream});
 }
 
 // room for the partial rows of dw and db: one per CTA
@@ -577,7 +968,7 @@ size_t layer_norm_backward_scratch_bytes(long rows, int C) {
 
 int launch_layer_norm_backward(const void* dy, long lddy, const void* x, long ldx, int f32, const float* w,
                                const float* mean, const float* rstd, void* dx, float* dw, float* db, long rows, int C,
-                               float* scratch, cudaStream_t stream) {
+                               float* scratch, int* dev_status, cudaStream_t stream) {
   LnBwdArgs a = {dy, lddy, x, ldx, w, mean, rstd, dx, scratch, rows, C, 1, 1};
   const int sms = device_sm_count();
   int parts = 0;
@@ -597,14 +988,30 @@ int launch_layer_norm_backward(const void* dy, long lddy, const void* x, long ld
       rc = after_launch("layer_norm_backward_wide_kernel");
       if (rc) return rc;
     } else {
+      const int row_bytes = C * (f32 ? 4 : 2);
+      const bool ring = f32 && s.vec > 1 && row_bytes >= 512;
+      if (ring) {  // as many teams as threads and shared memory (two rows each) leave room for
+        s.teams = LNR_MAX_WARPS / s.warps;
+        if (s.warps > 1 && s.teams > LNB_MAX_TEAMS) s.teams = LNB_MAX_TEAMS;
+        const long most = (LNR_SMEM - 4L * C) / (4L * row_bytes);
+        if (s.teams > most) s.teams = static_cast<int>(most);
+      }
       parts = fit_teams(&s, rows, sms);
       a.warps = s.warps;
       a.teams = s.teams;
-      int rc = with_shape(s, f32 != 0, LaunchBackward{a, parts, cta_threads(s), stream});
+      int rc;
+      if (ring) {
+        const LnRing r = ring_for(s, C, row_bytes, rows, parts, dev_status);
+        size_t smem = static_cast<size_t>(s.teams) * r.depth * 2 * row_bytes;
+        if (smem < 2 * sizeof(float) * C) smem = 2 * sizeof(float) * C;
+        rc = with_ring(s, f32 != 0, LaunchBackwardRing{a, r, parts, cta_threads(s), smem + sizeof(float) * C, stream});
+      } else {
+        rc = with_shape(s, f32 != 0, LaunchBackward{a, parts, cta_threads(s), stream});
+      }
       if (rc) return rc;
     }
   }
-  launch_dependent(layer_norm_columns_kernel, (2 * C + 31) / 32, 256, 0, stream, scratch, parts, C, dw, db);
+  launch_dependent(layer_norm_columns_kernel, (2 * C + 31) / 32, 1024, 0, stream, scratch, parts, C, dw, db);
   return after_launch("layer_norm_columns_kernel");
 }
 

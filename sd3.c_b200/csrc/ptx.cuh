@@ -28,6 +28,7 @@ enum : int {
   DEV_TIMEOUT_ATTN_O = 113,
   DEV_TIMEOUT_ATTN_KV = 114,
   DEV_TIMEOUT_ATTN_Q = 115,
+  DEV_TIMEOUT_LN_ROW = 121,
   DEV_TIMEOUT_SELFTEST = 199,  // the self-test kernel's wait on a barrier nobody arrives on
 };
 
@@ -239,6 +240,14 @@ __device__ __forceinline__ void tma_load_2d(void* smem_dst, const void* tmap, ui
       "[%0], [%1, {%3, %4}], [%2];"
       ::"r"(smem_u32(smem_dst)),
       "l"(reinterpret_cast<uint64_t>(tmap)), "r"(smem_u32(bar)), "r"(x), "r"(y)
+      : "memory");
+}
+
+// bytes (a multiple of 16) from 16-byte aligned global to shared memory, credited to bar
+__device__ __forceinline__ void bulk_load(void* smem_dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+      ::"r"(smem_u32(smem_dst)), "l"(reinterpret_cast<uint64_t>(src)), "r"(bytes), "r"(smem_u32(bar))
       : "memory");
 }
 
