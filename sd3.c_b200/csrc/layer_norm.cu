@@ -22,7 +22,7 @@ int device_sm_count();
 namespace {
 
 constexpr int LNB_THREADS = 512;   // at most, of a CTA
-constexpr int LNB_PER_THREAD = 16; // values of a row that a thread holds, at most
+constexpr int LNB_PER_THREAD = 24; // values of a row that a thread holds, at most
 constexpr int LNB_MAX_C = LNB_THREADS * LNB_PER_THREAD;  // wider rows: the kernels at the end of this file
 constexpr int LNB_MAX_WARPS = LNB_THREADS / 32;
 constexpr int LNB_MAX_TEAMS = 15;  // of several warps: named barriers 1 to 15
@@ -172,7 +172,7 @@ __global__ void __launch_bounds__(LNB_THREADS, 1) layer_norm_kernel(const __grid
       }
       buf ^= 1;
     }
-    const float rstd = 1.0f / sqrtf(m2 * inv_c + a.eps);
+    const float rstd = rsqrtf(m2 * inv_c + a.eps);
     if (row < a.rows) {
       T* out = static_cast<T*>(a.y) + row * a.C;
 #pragma unroll
@@ -203,7 +203,19 @@ __device__ __forceinline__ int vector_at(int c, int nvec) {  // of column c
 }
 template <int VEC>
 __device__ __forceinline__ void stage_vector(float* to, const float* from, float otherwise, int C) {
-  for (int c = threadIdx.x; c < C; c += blockDim.x) to[vector_at<VEC>(c, C / VEC)] = from ? from[c] : otherwise;
+  for (int c0 = threadIdx.x; c0 < C; c0 += 8 * blockDim.x) {  // eight loads in flight
+    float r[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int c = c0 + k * blockDim.x;
+      r[k] = from && c < C ? from[c] : otherwise;
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int c = c0 + k * blockDim.x;
+      if (c < C) to[vector_at<VEC>(c, C / VEC)] = r[k];
+    }
+  }
 }
 // piece c of a vector
 template <int VEC>
@@ -307,7 +319,7 @@ __global__ void __launch_bounds__(LNB_THREADS, 2) layer_norm_many_kernel(const _
       }
       buf ^= 1;
     }
-    const float rstd = 1.0f / sqrtf(m2 * inv_c + a.eps);
+    const float rstd = rsqrtf(m2 * inv_c + a.eps);
     if (row < a.rows) {
       T* out = static_cast<T*>(a.y) + row * a.C;
 #pragma unroll
@@ -353,7 +365,7 @@ struct LnBwdArgs {
 
 template <typename T, int VEC, int NV, int LANES>
 __global__ void __launch_bounds__(LNB_THREADS, 1) layer_norm_backward_kernel(const __grid_constant__ LnBwdArgs a) {
-  extern __shared__ float sums[];  // 2 C: dw and db of this CTA, at the end
+  extern __shared__ __align__(16) float sums[];  // w; at the end 2 C: dw and db of this CTA
   __shared__ float2 part[2][LNB_MAX_WARPS];
   grid_dep_wait();
   grid_dep_launch();
@@ -362,17 +374,11 @@ __global__ void __launch_bounds__(LNB_THREADS, 1) layer_norm_backward_kernel(con
   const int warp0 = team * a.warps;
   const int nvec = a.C / VEC;
   const float inv_c = 1.0f / static_cast<float>(a.C);
-  float w[NV][VEC], dw[NV][VEC], db[NV][VEC];
+  float dw[NV][VEC], db[NV][VEC];
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int c = t + i * ts;
+  for (int i = 0; i < NV; ++i)
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) {
-      w[i][j] = c < nvec && a.w ? a.w[c * VEC + j] : 1.f;
-      dw[i][j] = 0.f;
-      db[i][j] = 0.f;
-    }
-  }
+    for (int j = 0; j < VEC; ++j) dw[i][j] = db[i][j] = 0.f;
   const long step = static_cast<long>(gridDim.x) * a.teams;
   const long first = static_cast<long>(blockIdx.x) * a.teams;
   Raw<T, VEC> nx[NV], ny[NV];
@@ -395,6 +401,8 @@ __global__ void __launch_bounds__(LNB_THREADS, 1) layer_norm_backward_kernel(con
     nrstd = row < a.rows ? a.rstd[row] : 0.f;
   };
   request(first + team);
+  stage_vector<VEC>(sums, a.w, 1.f, a.C);
+  __syncthreads();
   int buf = 0;
   for (long base = first; base < a.rows; base += step) {
     const long row = base + team;
@@ -407,16 +415,33 @@ __global__ void __launch_bounds__(LNB_THREADS, 1) layer_norm_backward_kernel(con
     float sg = 0.f, sgu = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      float x[VEC], dy[VEC];
+      if (t + i * ts >= nvec) continue;
+      float x[VEC], dy[VEC], w[VEC];
       rx[i].get(x);
       ry[i].get(dy);
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        const float u = (x[j] - mean) * rstd, g = dy[j] * w[i][j];
+      staged<VEC>(sums, t + i * ts, nvec, w);
+      if constexpr (VEC == 1) {
+        const float u = (x[0] - mean) * rstd, g = dy[0] * w[0];
         sg += g;
         sgu = fmaf(g, u, sgu);
-        dw[i][j] = fmaf(dy[j], u, dw[i][j]);
-        db[i][j] += dy[j];
+        dw[i][0] = fmaf(dy[0], u, dw[i][0]);
+        db[i][0] += dy[0];
+      } else {
+        float2 g2 = make_float2(0.f, 0.f), gu2 = g2;
+#pragma unroll
+        for (int j = 0; j < VEC; j += 2) {
+          const float2 d = make_float2(dy[j], dy[j + 1]);
+          const float2 u = __fmul2_rn(__fadd2_rn(make_float2(x[j], x[j + 1]), make_float2(-mean, -mean)), make_float2(rstd, rstd));
+          const float2 g = __fmul2_rn(d, make_float2(w[j], w[j + 1]));
+          g2 = __fadd2_rn(g2, g);
+          gu2 = __ffma2_rn(g, u, gu2);
+          const float2 p = __ffma2_rn(d, u, make_float2(dw[i][j], dw[i][j + 1]));
+          const float2 q = __fadd2_rn(make_float2(db[i][j], db[i][j + 1]), d);
+          dw[i][j] = p.x; dw[i][j + 1] = p.y;
+          db[i][j] = q.x; db[i][j + 1] = q.y;
+        }
+        sg += g2.x + g2.y;
+        sgu += gu2.x + gu2.y;
       }
     }
     sg = lanes_sum<LANES>(sg);
@@ -426,6 +451,7 @@ __global__ void __launch_bounds__(LNB_THREADS, 1) layer_norm_backward_kernel(con
       team_barrier(1 + team, ts);
       sg = 0.f;
       sgu = 0.f;
+#pragma unroll 4
       for (int k = 0; k < a.warps; ++k) {
         sg += part[buf][warp0 + k].x;
         sgu += part[buf][warp0 + k].y;
@@ -439,19 +465,28 @@ __global__ void __launch_bounds__(LNB_THREADS, 1) layer_norm_backward_kernel(con
       for (int i = 0; i < NV; ++i) {
         const int c = t + i * ts;
         if (c < nvec) {
-          float x[VEC], dy[VEC], o[VEC];
+          float x[VEC], dy[VEC], w[VEC], o[VEC];
           rx[i].get(x);
           ry[i].get(dy);
+          staged<VEC>(sums, c, nvec, w);
+          if constexpr (VEC == 1) {
+            o[0] = rstd * (fmaf(dy[0], w[0], -mg) - (x[0] - mean) * rstd * mgu);
+          } else {
 #pragma unroll
-          for (int j = 0; j < VEC; ++j) {
-            const float u = (x[j] - mean) * rstd;
-            o[j] = rstd * (fmaf(dy[j], w[i][j], -mg) - u * mgu);
+            for (int j = 0; j < VEC; j += 2) {
+              const float2 u = __fmul2_rn(__fadd2_rn(make_float2(x[j], x[j + 1]), make_float2(-mean, -mean)), make_float2(rstd, rstd));
+              const float2 g = __ffma2_rn(make_float2(dy[j], dy[j + 1]), make_float2(w[j], w[j + 1]), make_float2(-mg, -mg));
+              const float2 d = __fmul2_rn(__ffma2_rn(u, make_float2(-mgu, -mgu), g), make_float2(rstd, rstd));
+              o[j] = d.x;
+              o[j + 1] = d.y;
+            }
           }
           Raw<T, VEC>::store(out + c * VEC, o);
         }
       }
     }
   }
+  __syncthreads();  // w is not needed any more
   // the teams' sums: those of one warp by shuffles, then one group of threads after the other in shared memory
 #pragma unroll
   for (int o = LANES; o < 32; o <<= 1)
@@ -471,10 +506,23 @@ __global__ void __launch_bounds__(LNB_THREADS, 1) layer_norm_backward_kernel(con
       for (int i = 0; i < NV; ++i) {
         const int c = t + i * ts;
         if (c < nvec) {
+          if constexpr (VEC == 1) {
+            sums[c] = dw[i][0] + (s > 0 ? sums[c] : 0.f);
+            sums[a.C + c] = db[i][0] + (s > 0 ? sums[a.C + c] : 0.f);
+          } else {
 #pragma unroll
-          for (int j = 0; j < VEC; ++j) {
-            sums[c * VEC + j] = dw[i][j] + (s > 0 ? sums[c * VEC + j] : 0.f);
-            sums[a.C + c * VEC + j] = db[i][j] + (s > 0 ? sums[a.C + c * VEC + j] : 0.f);
+            for (int j = 0; j < VEC; j += 4) {
+              float4 p = make_float4(dw[i][j], dw[i][j + 1], dw[i][j + 2], dw[i][j + 3]);
+              float4 q = make_float4(db[i][j], db[i][j + 1], db[i][j + 2], db[i][j + 3]);
+              float4 *sp = reinterpret_cast<float4*>(sums) + (c * VEC + j) / 4, *sq = sp + a.C / 4;
+              if (s > 0) {
+                const float4 op = *sp, oq = *sq;
+                p.x += op.x; p.y += op.y; p.z += op.z; p.w += op.w;
+                q.x += oq.x; q.y += oq.y; q.z += oq.z; q.w += oq.w;
+              }
+              *sp = p;
+              *sq = q;
+            }
           }
         }
       }
@@ -510,7 +558,7 @@ __global__ void __launch_bounds__(1024) layer_norm_columns_kernel(const float* p
 }
 
 // ----------------------------------------------------------------------------
-// Backward of aligned rows of 512 bytes and more: the same teams, with rows that come through shared memory.  Each team has a ring
+// Backward of aligned fp32 rows of 512 bytes and more: the same teams, with rows that come through shared memory.  Each team has a ring
 // of its own, `depth` rows of x and dy that its first thread requests ahead by bulk copies; behind the team's barrier of a row
 // everyone has finished the row before, whose place is then requested anew.  With neither the coming row nor the weight in
 // registers, 1024 threads fit an SM.
@@ -524,34 +572,16 @@ struct LnRing {
   int* status;
 };
 
-template <typename T>
-struct Vec16;
-template <>
-struct Vec16<bf16> {
-  static constexpr int N = 8;
-  __device__ __forceinline__ static void load(const uint8_t* p, float (&f)[8]) {
-    const uint4 v = *reinterpret_cast<const uint4*>(p);
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      f[2 * i] = __uint_as_float(w[i] << 16);
-      f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-    }
-  }
-};
-template <>
-struct Vec16<float> {
-  static constexpr int N = 4;
-  __device__ __forceinline__ static void load(const uint8_t* p, float (&f)[4]) {
-    const float4 v = *reinterpret_cast<const float4*>(p);
-    f[0] = v.x; f[1] = v.y; f[2] = v.z; f[3] = v.w;
-  }
-};
+__device__ __forceinline__ void load16(const uint8_t* p, float (&f)[4]) {
+  const float4 v = *reinterpret_cast<const float4*>(p);
+  f[0] = v.x; f[1] = v.y; f[2] = v.z; f[3] = v.w;
+}
 
-template <typename T, int NV>
+template <int NV>
 __global__ void __launch_bounds__(LNR_THREADS, 1) layer_norm_backward_ring_kernel(const __grid_constant__ LnBwdArgs a,
                                                                                   const __grid_constant__ LnRing ring) {
-  constexpr int VEC = Vec16<T>::N;
+  typedef float T;
+  constexpr int VEC = 4;
   extern __shared__ __align__(16) uint8_t ring_smem[];  // w, then the rings (x, dy of a row next to each other); at the end 2 C sums
   float* w_smem = reinterpret_cast<float*>(ring_smem);
   uint8_t* rows_smem = ring_smem + 4 * a.C;
@@ -609,8 +639,8 @@ __global__ void __launch_bounds__(LNR_THREADS, 1) layer_norm_backward_ring_kerne
       const int c = t + i * ts;
       if (c < nvec) {
         float x[VEC], dy[VEC], w[VEC];
-        Vec16<T>::load(px + c * 16, x);
-        Vec16<T>::load(px + ring.row_bytes + c * 16, dy);
+        load16(px + c * 16, x);
+        load16(px + ring.row_bytes + c * 16, dy);
         staged<VEC>(w_smem, c, nvec, w);
 #pragma unroll
         for (int j = 0; j < VEC; j += 2) {
@@ -649,8 +679,8 @@ __global__ void __launch_bounds__(LNR_THREADS, 1) layer_norm_backward_ring_kerne
       const int c = t + i * ts;
       if (c < nvec) {
         float x[VEC], dy[VEC], w[VEC], o[VEC];
-        Vec16<T>::load(px + c * 16, x);
-        Vec16<T>::load(px + ring.row_bytes + c * 16, dy);
+        load16(px + c * 16, x);
+        load16(px + ring.row_bytes + c * 16, dy);
         staged<VEC>(w_smem, c, nvec, w);
 #pragma unroll
         for (int j = 0; j < VEC; j += 2) {
@@ -784,11 +814,11 @@ struct LnShape {
   int vec, nv, lanes, warps, teams;
 };
 
-// As many pieces a thread as leave no more places idle than fewer would (a wide team spends more on its barrier), up to 16
-// values of bf16 and 8 of fp32, whose two rows in flight take as many registers; 16 where nothing else holds the row.
-LnShape ln_shape(int C, bool f32, bool aligned) {
+// The pieces a thread, up to `most` values, that leave the fewest places idle, the most of them where that is the same: what a row
+// costs a warp beside its values (two reductions, a barrier, the merge) is as much as sixteen of them.
+LnShape ln_shape(int C, bool aligned_f32, bool aligned_bf16, int most) {
   LnShape s;
-  s.vec = aligned ? (f32 ? 4 : 8) : 1;
+  s.vec = aligned_f32 ? 4 : aligned_bf16 ? 8 : 1;
   const int nvec = C / s.vec;
   s.nv = 1;
   s.lanes = 32;
@@ -797,8 +827,8 @@ LnShape ln_shape(int C, bool f32, bool aligned) {
     while (s.lanes > 4 && nvec <= s.lanes / 2) s.lanes /= 2;
   } else {
     long best = -1;
-    for (int most = s.vec == 8 ? 16 : 8; best < 0 && most <= LNB_PER_THREAD; most *= 2)
-      for (int nv = 1; nv * s.vec <= most; nv = s.vec == 1 && nv == 1 ? 4 : 2 * nv) {
+    for (; best < 0 && most <= LNB_PER_THREAD; most *= 2)
+      for (int nv = 1; nv * s.vec <= most; nv = s.vec > 1 ? nv + 1 : nv == 1 ? 4 : 2 * nv) {
         const int warps = (nvec + 32 * nv - 1) / (32 * nv);
         if (warps > LNB_MAX_WARPS) continue;
         const long places = static_cast<long>(warps) * nv;
@@ -833,8 +863,9 @@ int with_pieces(const LnShape& s, const F& f) {
   if (s.nv == 1) return f.template run<T, VEC, 1, 32>();
   if constexpr (VEC > 1) {
     if (s.nv == 2) return f.template run<T, VEC, 2, 32>();
+    if (s.nv == 3) return f.template run<T, VEC, 3, 32>();
   }
-  if constexpr (VEC == 1 || VEC == 4) {
+  if constexpr (VEC < 8) {
     if (s.nv == 4) return f.template run<T, VEC, 4, 32>();
   }
   if constexpr (VEC == 1) {
@@ -896,11 +927,10 @@ struct LaunchBackward {
   }
 };
 
-// The ring kernels: f.template run<T, NV>() of the shape
+// The ring kernel: f.template run<NV>() of the shape
 template <typename F>
-int with_ring(const LnShape& s, bool f32, const F& f) {
-  if (f32) return s.nv == 1 ? f.template run<float, 1>() : s.nv == 2 ? f.template run<float, 2>() : f.template run<float, 4>();
-  return s.nv == 1 ? f.template run<bf16, 1>() : f.template run<bf16, 2>();
+int with_ring(const LnShape& s, const F& f) {
+  return s.nv == 1 ? f.template run<1>() : s.nv == 2 ? f.template run<2>() : s.nv == 3 ? f.template run<3>() : f.template run<4>();
 }
 
 struct LaunchBackwardRing {
@@ -909,11 +939,11 @@ struct LaunchBackwardRing {
   int grid, threads;
   size_t smem;
   cudaStream_t stream;
-  template <typename T, int NV>
+  template <int NV>
   int run() const {
-    int rc = allow_smem(layer_norm_backward_ring_kernel<T, NV>, smem, LNR_SMEM);
+    int rc = allow_smem(layer_norm_backward_ring_kernel<NV>, smem, LNR_SMEM);
     if (rc) return rc;
-    launch_dependent(layer_norm_backward_ring_kernel<T, NV>, grid, threads, smem, stream, a, ring);
+    launch_dependent(layer_norm_backward_ring_kernel<NV>, grid, threads, smem, stream, a, ring);
     return after_launch("layer_norm_backward_ring_kernel");
   }
 };
@@ -945,13 +975,15 @@ int launch_layer_norm(const void* x, long ldx, int f32, const float* w, const fl
                       float* rstd, long rows, int C, cudaStream_t stream) {
   LnFwdArgs a = {x, ldx, w, b, y, mean, rstd, rows, C, 1, 1, eps};
   const int sms = device_sm_count();
-  LnShape s = ln_shape(C, f32 != 0, C % (f32 ? 4 : 8) == 0 && row_aligned(x, ldx, f32) && row_aligned(y, C, f32));
+  const bool aligned = C % (f32 ? 4 : 8) == 0 && row_aligned(x, ldx, f32) && row_aligned(y, C, f32);
+  LnShape s = ln_shape(C, f32 && aligned, !f32 && aligned, f32 ? 8 : 16);
+  const bool many = rows > 2L * sms * s.teams;
+  if (many) s = ln_shape(C, f32 && aligned, !f32 && aligned, f32 ? 16 : 24);
   if (!row_fits(C, s)) {
     const int grid = static_cast<int>(rows < 4L * sms ? rows : 4L * sms);
     launch_dependent(f32 ? layer_norm_wide_kernel<float> : layer_norm_wide_kernel<bf16>, grid, LNB_THREADS, 0, stream, a);
     return after_launch("layer_norm_wide_kernel");
   }
-  const bool many = rows > 2L * sms * s.teams;
   const int grid = fit_teams(&s, rows, many ? 2 * sms : sms);
   a.warps = s.warps;
   a.teams = s.teams;
@@ -973,8 +1005,8 @@ int launch_layer_norm_backward(const void* dy, long lddy, const void* x, long ld
   const int sms = device_sm_count();
   int parts = 0;
   if (rows > 0) {
-    LnShape s = ln_shape(C, f32 != 0, C % (f32 ? 4 : 8) == 0 && row_aligned(x, ldx, f32) && row_aligned(dy, lddy, f32) &&
-                                          row_aligned(dx, C, f32));
+    const bool aligned = C % (f32 ? 4 : 8) == 0 && row_aligned(x, ldx, f32) && row_aligned(dy, lddy, f32) && row_aligned(dx, C, f32);
+    LnShape s = ln_shape(C, f32 && aligned, !f32 && aligned, f32 ? 8 : 16);
     if (!row_fits(C, s)) {
       // the columns first: dx may lie where x or dy does
       parts = static_cast<int>(rows < LNB_WIDE_PARTS ? rows : LNB_WIDE_PARTS);
@@ -1004,7 +1036,7 @@ int launch_layer_norm_backward(const void* dy, long lddy, const void* x, long ld
         const LnRing r = ring_for(s, C, row_bytes, rows, parts, dev_status);
         size_t smem = static_cast<size_t>(s.teams) * r.depth * 2 * row_bytes;
         if (smem < 2 * sizeof(float) * C) smem = 2 * sizeof(float) * C;
-        rc = with_ring(s, f32 != 0, LaunchBackwardRing{a, r, parts, cta_threads(s), smem + sizeof(float) * C, stream});
+        rc = with_ring(s, LaunchBackwardRing{a, r, parts, cta_threads(s), smem + sizeof(float) * C, stream});
       } else {
         rc = with_shape(s, f32 != 0, LaunchBackward{a, parts, cta_threads(s), stream});
       }

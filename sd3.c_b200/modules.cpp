@@ -242,7 +242,7 @@ Rows rows_of(const Tensor& t, const char* name) {
 Tensor vector_f32(const Tensor& v, int64_t n, const Tensor& x, const char* name) {
   TORCH_CHECK(v.is_cuda() && v.device() == x.device() && v.numel() == n, name, ": ", std::to_string(n),
               " values on ", x.device().str(), " expected");
-  return v.to(torch::kFloat32).contiguous();
+  return v.scalar_type() == torch::kFloat32 && v.is_contiguous() ? v : v.to(torch::kFloat32).contiguous();
 }
 
 Tensor linear_impl(const Tensor& x_in, const Tensor& W, const Tensor& b, int act) {
@@ -348,12 +348,11 @@ std::vector<Tensor> LayerNorm_forward(Tensor& x_in, Tensor& w, Tensor& b, float 
     c10::cuda::CUDAGuard guard(x.t.device());
     Tensor wf = vector_f32(w, x.C, x.t, "w"), bf = vector_f32(b, x.C, x.t, "b");
     Tensor out = torch::empty(x_in.sizes(), x_in.options());
-    Tensor stats = torch::empty({2, x.rows}, wf.options());
-    float* mean = stats.data_ptr<float>();
+    Tensor mean = torch::empty({x.rows}, wf.options()), rstd = torch::empty({x.rows}, wf.options());
     ok(sd3_layer_norm(x.t.data_ptr(), x.ld, tag(x.t), wf.data_ptr<float>(), bf.data_ptr<float>(), eps, out.data_ptr(),
-                      mean, mean + x.rows, x.rows, (int)x.C, stream()),
+                      mean.data_ptr<float>(), rstd.data_ptr<float>(), x.rows, (int)x.C, stream()),
        "sd3_layer_norm");
-    return {out, stats[0], stats[1]};
+    return {out, mean, rstd};
   }
   Tensor x = dev(x_in, "x");
   c10::cuda::CUDAGuard guard(x.device());
