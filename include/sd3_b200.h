@@ -252,7 +252,7 @@ SD3_API int sd3_layer_norm(const void* x, long ldx, int dtype, const float* w, c
  * dw = sum over rows of dy * (x - mean) * rstd and db = sum over rows of dy, (C) f32 each, written (not added to);
  * dw or db may be NULL.  x, ldx, w, mean and rstd as given to and left by the forward.  dx may be dy or x where those
  * are contiguous.  The sums are formed in a fixed order: the same bits on every call.  scratch: device memory of at
- * least sd3_layer_norm_backward_scratch_bytes(rows, C) bytes on the current device, 4-byte aligned, used by this call
+ * least sd3_layer_norm_backward_scratch_bytes(rows, C) bytes on the current device, 16-byte aligned, used by this call
  * alone until it is complete.  rows may be 0: dw = db = 0.
  * Replaces LayerNorm_backward (modules.cpp:87-152). */
 SD3_API long sd3_layer_norm_backward_scratch_bytes(long rows, int C);

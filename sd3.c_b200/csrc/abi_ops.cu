@@ -421,9 +421,9 @@ int sd3_layer_norm_backward(const void* dy, long lddy, const void* x, long ldx, 
                    ldx, lddy);
     return SD3_ERR_INVALID_ARG;
   }
-  if (rows > 0 && (!scratch || (reinterpret_cast<uintptr_t>(scratch) & 3) ||
+  if (rows > 0 && (!scratch || (reinterpret_cast<uintptr_t>(scratch) & 15) ||
                    scratch_bytes < sd3_layer_norm_backward_scratch_bytes(rows, C))) {
-    set_last_error("sd3_layer_norm_backward: %ld bytes of scratch needed, got %ld",
+    set_last_error("sd3_layer_norm_backward: %ld bytes of 16-byte aligned scratch needed, got %ld",
                    sd3_layer_norm_backward_scratch_bytes(rows, C), scratch ? scratch_bytes : 0L);
     return SD3_ERR_INVALID_ARG;
   }

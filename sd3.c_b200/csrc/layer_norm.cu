@@ -21,13 +21,16 @@ int device_sm_count();
 
 namespace {
 
-constexpr int LNB_THREADS = 512;   // at most, of a CTA
-constexpr int LNB_PER_THREAD = 24; // values of a row that a thread holds, at most
-constexpr int LNB_MAX_C = LNB_THREADS * LNB_PER_THREAD;  // wider rows: the kernels at the end of this file
-constexpr int LNB_MAX_WARPS = LNB_THREADS / 32;
+// Threads of a CTA, and values of a row that a thread holds, at most: pieces of one or two values need so few registers that an SM
+// holds 1024 threads, and so many instructions that it should.
+__host__ __device__ constexpr int lnb_threads(int vec) { return vec <= 2 ? 1024 : 512; }
+__host__ __device__ constexpr int lnb_values(int vec) { return vec <= 2 ? 8 : 24; }
+constexpr int LNB_MAX_WARPS = 32;
+constexpr int LNB_MAX_C = 512 * 24;  // wider rows: the kernels at the end of this file
+constexpr int LNB_WIDE_THREADS = 512;
 constexpr int LNB_MAX_TEAMS = 15;  // of several warps: named barriers 1 to 15
 
-// VEC values of type T as they lie in memory: 16 bytes, or one value where rows are not 16-byte aligned
+// VEC values of type T as they lie in memory: 16 bytes, or two or one where rows are not aligned for more
 template <typename T, int VEC>
 struct Raw;
 template <>
@@ -57,6 +60,22 @@ struct Raw<float, 4> {
   __device__ __forceinline__ static void store(float* p, const float (&f)[4]) {
     *reinterpret_cast<float4*>(p) = make_float4(f[0], f[1], f[2], f[3]);
   }
+};
+template <>
+struct Raw<bf16, 2> {
+  uint32_t v;
+  __device__ __forceinline__ void load(const bf16* p) { v = *reinterpret_cast<const uint32_t*>(p); }
+  __device__ __forceinline__ void zero() { v = 0; }
+  __device__ __forceinline__ void get(float (&f)[2]) const { f[0] = __uint_as_float(v << 16); f[1] = __uint_as_float(v & 0xffff0000u); }
+  __device__ __forceinline__ static void store(bf16* p, const float (&f)[2]) { *reinterpret_cast<uint32_t*>(p) = pack_bf16x2(f[0], f[1]); }
+};
+template <>
+struct Raw<float, 2> {
+  float2 v;
+  __device__ __forceinline__ void load(const float* p) { v = *reinterpret_cast<const float2*>(p); }
+  __device__ __forceinline__ void zero() { v = make_float2(0.f, 0.f); }
+  __device__ __forceinline__ void get(float (&f)[2]) const { f[0] = v.x; f[1] = v.y; }
+  __device__ __forceinline__ static void store(float* p, const float (&f)[2]) { *reinterpret_cast<float2*>(p) = make_float2(f[0], f[1]); }
 };
 __device__ __forceinline__ float to_float(float v) { return v; }
 __device__ __forceinline__ float to_float(bf16 v) { return __bfloat162float(v); }
@@ -96,7 +115,7 @@ struct LnFwdArgs {
 
 // One or two rows a team: weight and bias on their way with the row.
 template <typename T, int VEC, int NV, int LANES>
-__global__ void __launch_bounds__(LNB_THREADS, 1) layer_norm_kernel(const __grid_constant__ LnFwdArgs a) {
+__global__ void __launch_bounds__(lnb_threads(VEC), 1) layer_norm_kernel(const __grid_constant__ LnFwdArgs a) {
   __shared__ float2 part[2][LNB_MAX_WARPS];  // mean and squared deviations of each warp, two rows' worth
   __shared__ float n_of[LNB_MAX_WARPS];      // values that each warp holds of a row
   grid_dep_wait();
@@ -222,6 +241,9 @@ template <int VEC>
 __device__ __forceinline__ void staged(const float* v, int c, int nvec, float (&f)[VEC]) {
   if constexpr (VEC == 1) {
     f[0] = v[c];
+  } else if constexpr (VEC == 2) {
+    const float2 t = reinterpret_cast<const float2*>(v)[c];
+    f[0] = t.x; f[1] = t.y;
   } else {
 #pragma unroll
     for (int h = 0; h < VEC / 4; ++h) {
@@ -253,7 +275,7 @@ __device__ __forceinline__ float squares_of(const float (&v)[VEC], float mean) {
 }
 
 template <typename T, int VEC, int NV, int LANES>
-__global__ void __launch_bounds__(LNB_THREADS, 2) layer_norm_many_kernel(const __grid_constant__ LnFwdArgs a) {
+__global__ void __launch_bounds__(lnb_threads(VEC), VEC <= 2 ? 1 : 2) layer_norm_many_kernel(const __grid_constant__ LnFwdArgs a) {
   extern __shared__ __align__(16) float vectors[];  // w, b
   __shared__ float2 part[2][LNB_MAX_WARPS];  // mean and squared deviations of each warp, two rows' worth
   __shared__ float n_of[LNB_MAX_WARPS];      // values that each warp holds of a row
@@ -363,9 +385,58 @@ struct LnBwdArgs {
   int C, warps, teams;
 };
 
+// dw and db of a CTA: its groups' sums, added in pairs through shared memory (groups / 2 times 2 C floats), always in the same
+// order; group 0 writes the result.  `mine`: this thread holds pieces (of a group that repeats them in several lanes, one does).
+template <int VEC, int NV>
+__device__ __forceinline__ void combine_groups(float (&dw)[NV][VEC], float (&db)[NV][VEC], float* smem, int group, int groups,
+                                               int t, int ts, int C, bool mine, float* out) {
+  constexpr int W = VEC >= 4 ? 4 : VEC;
+  struct alignas(4 * W) Piece { float f[W]; };
+  const int nvec = C / VEC;
+  auto each = [&](auto&& f) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = t + i * ts;
+      if (c < nvec) {
+#pragma unroll
+        for (int j = 0; j < VEC; j += W) f(i, j, c * VEC + j);
+      }
+    }
+  };
+  for (int n = groups; n > 1;) {
+    const int half = (n + 1) / 2;
+    float* slot = smem + static_cast<long>(group >= half ? group - half : group) * 2 * C;
+    if (mine && group >= half && group < n)
+      each([&](int i, int j, int at) {
+        Piece p, q;
+#pragma unroll
+        for (int k = 0; k < W; ++k) { p.f[k] = dw[i][j + k]; q.f[k] = db[i][j + k]; }
+        *reinterpret_cast<Piece*>(slot + at) = p;
+        *reinterpret_cast<Piece*>(slot + C + at) = q;
+      });
+    __syncthreads();
+    if (mine && group < n - half)
+      each([&](int i, int j, int at) {
+        const Piece p = *reinterpret_cast<const Piece*>(slot + at), q = *reinterpret_cast<const Piece*>(slot + C + at);
+#pragma unroll
+        for (int k = 0; k < W; ++k) { dw[i][j + k] += p.f[k]; db[i][j + k] += q.f[k]; }
+      });
+    __syncthreads();
+    n = half;
+  }
+  if (mine && group == 0)
+    each([&](int i, int j, int at) {
+      Piece p, q;
+#pragma unroll
+      for (int k = 0; k < W; ++k) { p.f[k] = dw[i][j + k]; q.f[k] = db[i][j + k]; }
+      *reinterpret_cast<Piece*>(out + at) = p;
+      *reinterpret_cast<Piece*>(out + C + at) = q;
+    });
+}
+
 template <typename T, int VEC, int NV, int LANES>
-__global__ void __launch_bounds__(LNB_THREADS, 1) layer_norm_backward_kernel(const __grid_constant__ LnBwdArgs a) {
-  extern __shared__ __align__(16) float sums[];  // w; at the end 2 C: dw and db of this CTA
+__global__ void __launch_bounds__(lnb_threads(VEC), 1) layer_norm_backward_kernel(const __grid_constant__ LnBwdArgs a) {
+  extern __shared__ __align__(16) float sums[];  // w; at the end room for combine_groups
   __shared__ float2 part[2][LNB_MAX_WARPS];
   grid_dep_wait();
   grid_dep_launch();
@@ -400,17 +471,19 @@ __global__ void __launch_bounds__(LNB_THREADS, 1) layer_norm_backward_kernel(con
     nmean = row < a.rows ? a.mean[row] : 0.f;
     nrstd = row < a.rows ? a.rstd[row] : 0.f;
   };
-  request(first + team);
+  constexpr bool PREFETCH = VEC > 1;  // single values: 32 registers that an SM full of warps does better without
+  if (PREFETCH) request(first + team);
   stage_vector<VEC>(sums, a.w, 1.f, a.C);
   __syncthreads();
   int buf = 0;
   for (long base = first; base < a.rows; base += step) {
     const long row = base + team;
+    if (!PREFETCH) request(row);
     Raw<T, VEC> rx[NV], ry[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) { rx[i] = nx[i]; ry[i] = ny[i]; }
     const float mean = nmean, rstd = nrstd;
-    request(row + step);
+    if (PREFETCH) request(row + step);
     // a place without a value has dy = 0 and adds nothing
     float sg = 0.f, sgu = 0.f;
 #pragma unroll
@@ -487,7 +560,7 @@ __global__ void __launch_bounds__(LNB_THREADS, 1) layer_norm_backward_kernel(con
     }
   }
   __syncthreads();  // w is not needed any more
-  // the teams' sums: those of one warp by shuffles, then one group of threads after the other in shared memory
+  // the teams' sums: those of one warp by shuffles, then the warps' or wide teams'
 #pragma unroll
   for (int o = LANES; o < 32; o <<= 1)
 #pragma unroll
@@ -500,37 +573,7 @@ __global__ void __launch_bounds__(LNB_THREADS, 1) layer_norm_backward_kernel(con
   const int group = a.warps > 1 ? team : static_cast<int>(threadIdx.x >> 5);
   const int groups = a.warps > 1 ? a.teams : static_cast<int>(blockDim.x >> 5);
   const bool mine = a.warps > 1 || (threadIdx.x & 31) < LANES;
-  for (int s = 0; s < groups; ++s) {
-    if (group == s && mine) {
-#pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        const int c = t + i * ts;
-        if (c < nvec) {
-          if constexpr (VEC == 1) {
-            sums[c] = dw[i][0] + (s > 0 ? sums[c] : 0.f);
-            sums[a.C + c] = db[i][0] + (s > 0 ? sums[a.C + c] : 0.f);
-          } else {
-#pragma unroll
-            for (int j = 0; j < VEC; j += 4) {
-              float4 p = make_float4(dw[i][j], dw[i][j + 1], dw[i][j + 2], dw[i][j + 3]);
-              float4 q = make_float4(db[i][j], db[i][j + 1], db[i][j + 2], db[i][j + 3]);
-              float4 *sp = reinterpret_cast<float4*>(sums) + (c * VEC + j) / 4, *sq = sp + a.C / 4;
-              if (s > 0) {
-                const float4 op = *sp, oq = *sq;
-                p.x += op.x; p.y += op.y; p.z += op.z; p.w += op.w;
-                q.x += oq.x; q.y += oq.y; q.z += oq.z; q.w += oq.w;
-              }
-              *sp = p;
-              *sq = q;
-            }
-          }
-        }
-      }
-    }
-    __syncthreads();
-  }
-  float* out = a.partial + static_cast<long>(blockIdx.x) * 2 * a.C;
-  for (int c = threadIdx.x; c < 2 * a.C; c += blockDim.x) out[c] = sums[c];
+  combine_groups<VEC, NV>(dw, db, sums, group, groups, t, ts, a.C, mine, a.partial + static_cast<long>(blockIdx.x) * 2 * a.C);
 }
 
 // dw and db: the sums of `parts` partial rows of 2 C values.  Thread k of the 32 of a column adds parts k, k + 32, ...; then the
@@ -582,7 +625,7 @@ __global__ void __launch_bounds__(LNR_THREADS, 1) layer_norm_backward_ring_kerne
                                                                                   const __grid_constant__ LnRing ring) {
   typedef float T;
   constexpr int VEC = 4;
-  extern __shared__ __align__(16) uint8_t ring_smem[];  // w, then the rings (x, dy of a row next to each other); at the end 2 C sums
+  extern __shared__ __align__(16) uint8_t ring_smem[];  // w, then the rings (x, dy of a row next to each other); at the end room for combine_groups
   float* w_smem = reinterpret_cast<float*>(ring_smem);
   uint8_t* rows_smem = ring_smem + 4 * a.C;
   __shared__ float2 part[2][LNR_MAX_WARPS];
@@ -615,11 +658,11 @@ __global__ void __launch_bounds__(LNR_THREADS, 1) layer_norm_backward_ring_kerne
     for (int s = 0; s < ring.depth; ++s) request(first + s * step, s);
   stage_vector<VEC>(w_smem, a.w, 1.f, a.C);
   __syncthreads();
-  float2 dw[NV][VEC / 2], db[NV][VEC / 2];
+  float dw[NV][VEC], db[NV][VEC];
 #pragma unroll
   for (int i = 0; i < NV; ++i)
 #pragma unroll
-    for (int j = 0; j < VEC / 2; ++j) dw[i][j] = db[i][j] = make_float2(0.f, 0.f);
+    for (int j = 0; j < VEC; ++j) dw[i][j] = db[i][j] = 0.f;
   const float inv_c = 1.0f / static_cast<float>(a.C);
   float next_mean = first < a.rows ? a.mean[first] : 0.f, next_rstd = first < a.rows ? a.rstd[first] : 0.f;
   int buf = 0, s = 0, s_before = 0;
@@ -648,8 +691,10 @@ __global__ void __launch_bounds__(LNR_THREADS, 1) layer_norm_backward_ring_kerne
           const float2 u = __fmul2_rn(__fadd2_rn(make_float2(x[j], x[j + 1]), m2), r2), g = __fmul2_rn(d, make_float2(w[j], w[j + 1]));
           sg2 = __fadd2_rn(sg2, g);
           sgu2 = __ffma2_rn(g, u, sgu2);
-          dw[i][j / 2] = __ffma2_rn(d, u, dw[i][j / 2]);
-          db[i][j / 2] = __fadd2_rn(db[i][j / 2], d);
+          const float2 p = __ffma2_rn(d, u, make_float2(dw[i][j], dw[i][j + 1]));
+          const float2 q = __fadd2_rn(make_float2(db[i][j], db[i][j + 1]), d);
+          dw[i][j] = p.x; dw[i][j + 1] = p.y;
+          db[i][j] = q.x; db[i][j + 1] = q.y;
         }
       }
     }
@@ -696,33 +741,8 @@ __global__ void __launch_bounds__(LNR_THREADS, 1) layer_norm_backward_ring_kerne
   }
   __syncthreads();  // every row has landed and been read: the rings hold the sums from here on
   if (s_abort) drain_after_abort();
-  float4* sums = reinterpret_cast<float4*>(rows_smem);
-  for (int k = 0; k < a.teams; ++k) {
-    if (team == k) {
-#pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        const int c = t + i * ts;
-        if (c < nvec) {
-#pragma unroll
-          for (int j = 0; j < VEC; j += 4) {
-            float4 p = make_float4(dw[i][j / 2].x, dw[i][j / 2].y, dw[i][j / 2 + 1].x, dw[i][j / 2 + 1].y);
-            float4 q = make_float4(db[i][j / 2].x, db[i][j / 2].y, db[i][j / 2 + 1].x, db[i][j / 2 + 1].y);
-            float4 *sp = sums + (c * VEC + j) / 4, *sq = sums + (a.C + c * VEC + j) / 4;
-            if (k > 0) {
-              const float4 op = *sp, oq = *sq;
-              p.x += op.x; p.y += op.y; p.z += op.z; p.w += op.w;
-              q.x += oq.x; q.y += oq.y; q.z += oq.z; q.w += oq.w;
-            }
-            *sp = p;
-            *sq = q;
-          }
-        }
-      }
-    }
-    __syncthreads();
-  }
-  float4* out = reinterpret_cast<float4*>(a.partial + static_cast<long>(blockIdx.x) * 2 * a.C);
-  for (int c = threadIdx.x; c < a.C / 2; c += blockDim.x) out[c] = sums[c];
+  combine_groups<VEC, NV>(dw, db, reinterpret_cast<float*>(rows_smem), team, a.teams, t, ts, a.C, true,
+                          a.partial + static_cast<long>(blockIdx.x) * 2 * a.C);
 }
 
 // ----------------------------------------------------------------------------
@@ -734,27 +754,27 @@ __device__ __forceinline__ float cta_sum(float v, float* s) {
   if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = v;
   __syncthreads();
   float r = 0.f;
-  for (int k = 0; k < LNB_MAX_WARPS; ++k) r += s[k];
+  for (int k = 0; k < LNB_WIDE_THREADS / 32; ++k) r += s[k];
   __syncthreads();
   return r;
 }
 
 template <typename T>
-__global__ void __launch_bounds__(LNB_THREADS) layer_norm_wide_kernel(const __grid_constant__ LnFwdArgs a) {
-  __shared__ float s[LNB_MAX_WARPS];
+__global__ void __launch_bounds__(LNB_WIDE_THREADS) layer_norm_wide_kernel(const __grid_constant__ LnFwdArgs a) {
+  __shared__ float s[LNB_WIDE_THREADS / 32];
   grid_dep_wait();
   grid_dep_launch();
   const float inv_c = 1.0f / static_cast<float>(a.C);
   for (long row = blockIdx.x; row < a.rows; row += gridDim.x) {
     const T* x = static_cast<const T*>(a.x) + row * a.ldx;
     float v = 0.f;
-    for (int c = threadIdx.x; c < a.C; c += LNB_THREADS) v += to_float(x[c]);
+    for (int c = threadIdx.x; c < a.C; c += LNB_WIDE_THREADS) v += to_float(x[c]);
     const float mean = cta_sum(v, s) * inv_c;
     v = 0.f;
-    for (int c = threadIdx.x; c < a.C; c += LNB_THREADS) v = fmaf(to_float(x[c]) - mean, to_float(x[c]) - mean, v);
+    for (int c = threadIdx.x; c < a.C; c += LNB_WIDE_THREADS) v = fmaf(to_float(x[c]) - mean, to_float(x[c]) - mean, v);
     const float rstd = 1.0f / sqrtf(cta_sum(v, s) * inv_c + a.eps);
     T* out = static_cast<T*>(a.y) + row * a.C;
-    for (int c = threadIdx.x; c < a.C; c += LNB_THREADS)
+    for (int c = threadIdx.x; c < a.C; c += LNB_WIDE_THREADS)
       from_float(out + c, fmaf((to_float(x[c]) - mean) * rstd, a.w ? a.w[c] : 1.f, a.b ? a.b[c] : 0.f));
     if (threadIdx.x == 0) {
       if (a.mean) a.mean[row] = mean;
@@ -764,8 +784,8 @@ __global__ void __launch_bounds__(LNB_THREADS) layer_norm_wide_kernel(const __gr
 }
 
 template <typename T>
-__global__ void __launch_bounds__(LNB_THREADS) layer_norm_backward_wide_kernel(const __grid_constant__ LnBwdArgs a) {
-  __shared__ float s[LNB_MAX_WARPS];
+__global__ void __launch_bounds__(LNB_WIDE_THREADS) layer_norm_backward_wide_kernel(const __grid_constant__ LnBwdArgs a) {
+  __shared__ float s[LNB_WIDE_THREADS / 32];
   grid_dep_wait();
   grid_dep_launch();
   const float inv_c = 1.0f / static_cast<float>(a.C);
@@ -774,14 +794,14 @@ __global__ void __launch_bounds__(LNB_THREADS) layer_norm_backward_wide_kernel(c
     const T* dy = static_cast<const T*>(a.dy) + row * a.lddy;
     const float mean = a.mean[row], rstd = a.rstd[row];
     float sg = 0.f, sgu = 0.f;
-    for (int c = threadIdx.x; c < a.C; c += LNB_THREADS) {
+    for (int c = threadIdx.x; c < a.C; c += LNB_WIDE_THREADS) {
       const float g = to_float(dy[c]) * (a.w ? a.w[c] : 1.f);
       sg += g;
       sgu = fmaf(g, (to_float(x[c]) - mean) * rstd, sgu);
     }
     const float mg = cta_sum(sg, s) * inv_c, mgu = cta_sum(sgu, s) * inv_c;
     T* out = static_cast<T*>(a.dx) + row * a.C;
-    for (int c = threadIdx.x; c < a.C; c += LNB_THREADS) {
+    for (int c = threadIdx.x; c < a.C; c += LNB_WIDE_THREADS) {
       const float u = (to_float(x[c]) - mean) * rstd;
       from_float(out + c, rstd * (fmaf(to_float(dy[c]), a.w ? a.w[c] : 1.f, -mg) - u * mgu));
     }
@@ -814,33 +834,38 @@ struct LnShape {
   int vec, nv, lanes, warps, teams;
 };
 
-// The pieces a thread, up to `most` values, that leave the fewest places idle, the most of them where that is the same: what a row
-// costs a warp beside its values (two reductions, a barrier, the merge) is as much as sixteen of them.
-LnShape ln_shape(int C, bool aligned_f32, bool aligned_bf16, int most) {
+// The pieces a thread, up to `most` values, with which a row costs its warps least: beside its values a warp spends as much as on
+// sixteen of them (two reductions, a barrier, the merge).
+LnShape ln_shape(int C, int vec, int most) {
   LnShape s;
-  s.vec = aligned_f32 ? 4 : aligned_bf16 ? 8 : 1;
+  s.vec = vec;
   const int nvec = C / s.vec;
   s.nv = 1;
   s.lanes = 32;
   s.warps = 1;
+  const int max_warps = lnb_threads(vec) / 32;
+  if (most > lnb_values(vec)) most = lnb_values(vec);
   if (nvec <= 32) {
     while (s.lanes > 4 && nvec <= s.lanes / 2) s.lanes /= 2;
   } else {
     long best = -1;
-    for (; best < 0 && most <= LNB_PER_THREAD; most *= 2)
-      for (int nv = 1; nv * s.vec <= most; nv = s.vec > 1 ? nv + 1 : nv == 1 ? 4 : 2 * nv) {
+    for (; best < 0 && most <= lnb_values(vec); most *= 2)
+      for (int nv = 1; nv * s.vec <= most; nv = s.vec > 2 ? nv + 1 : 2 * nv) {
         const int warps = (nvec + 32 * nv - 1) / (32 * nv);
-        if (warps > LNB_MAX_WARPS) continue;
-        const long places = static_cast<long>(warps) * nv;
-        if (best < 0 || places <= best) { best = places; s.nv = nv; s.warps = warps; }
+        if (warps > max_warps) continue;
+        const long cost = static_cast<long>(warps) * (16 + nv * s.vec);
+        if (best < 0 || cost <= best) { best = cost; s.nv = nv; s.warps = warps; }
       }
   }
-  s.teams = s.warps > 1 ? LNB_MAX_WARPS / s.warps : LNB_THREADS / s.lanes;
+  s.teams = s.warps > 1 ? max_warps / s.warps : lnb_threads(vec) / s.lanes;
+  if (s.warps > 1 && s.teams > LNB_MAX_TEAMS) s.teams = LNB_MAX_TEAMS;
   return s;
 }
 
-bool row_aligned(const void* p, long ld, bool f32) {
-  return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (ld * (f32 ? 4 : 2)) % 16 == 0;
+// values of a piece: 16 bytes, two values or one, by what every row is aligned for
+int piece_of(const void* p, long ld, int C, int esz) {
+  const uintptr_t at = reinterpret_cast<uintptr_t>(p) | static_cast<uintptr_t>(ld * esz) | static_cast<uintptr_t>(C * static_cast<long>(esz));
+  return at % 16 == 0 ? 16 / esz : at % (2 * esz) == 0 ? 2 : 1;
 }
 
 int cta_threads(const LnShape& s) { return s.teams * (s.warps > 1 ? 32 * s.warps : s.lanes); }
@@ -861,8 +886,8 @@ int with_pieces(const LnShape& s, const F& f) {
   if (s.lanes == 8) return f.template run<T, VEC, 1, 8>();
   if (s.lanes == 16) return f.template run<T, VEC, 1, 16>();
   if (s.nv == 1) return f.template run<T, VEC, 1, 32>();
-  if constexpr (VEC > 1) {
-    if (s.nv == 2) return f.template run<T, VEC, 2, 32>();
+  if (s.nv == 2) return f.template run<T, VEC, 2, 32>();
+  if constexpr (VEC > 2) {
     if (s.nv == 3) return f.template run<T, VEC, 3, 32>();
   }
   if constexpr (VEC < 8) {
@@ -870,15 +895,15 @@ int with_pieces(const LnShape& s, const F& f) {
   }
   if constexpr (VEC == 1) {
     if (s.nv == 8) return f.template run<T, 1, 8, 32>();
-    if (s.nv == 16) return f.template run<T, 1, 16, 32>();
   }
-  set_last_error("layer_norm: no kernel for %d pieces", s.nv);
+  set_last_error("layer_norm: no kernel for %d pieces of %d", s.nv, s.vec);
   return ST_UNSUPPORTED;
 }
 template <typename F>
 int with_shape(const LnShape& s, bool f32, const F& f) {
-  if (f32) return s.vec == 4 ? with_pieces<float, 4>(s, f) : with_pieces<float, 1>(s, f);
-  return s.vec == 8 ? with_pieces<bf16, 8>(s, f) : with_pieces<bf16, 1>(s, f);
+  if (s.vec == 1) return f32 ? with_pieces<float, 1>(s, f) : with_pieces<bf16, 1>(s, f);
+  if (s.vec == 2) return f32 ? with_pieces<float, 2>(s, f) : with_pieces<bf16, 2>(s, f);
+  return f32 ? with_pieces<float, 4>(s, f) : with_pieces<bf16, 8>(s, f);
 }
 
 template <typename K>
@@ -908,6 +933,8 @@ struct LaunchForward {
   }
 };
 
+size_t combine_bytes(int groups, int C) { return static_cast<size_t>(groups / 2) * 2 * C * sizeof(float); }
+
 struct LaunchBackward {
   const LnBwdArgs& a;
   int grid, threads;
@@ -915,13 +942,11 @@ struct LaunchBackward {
   template <typename T, int VEC, int NV, int LANES>
   int run() const {
     auto kern = layer_norm_backward_kernel<T, VEC, NV, LANES>;
-    const size_t smem = 2 * sizeof(float) * a.C;
-    if (smem > 48 * 1024 - 1024) {
-      int rc = check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                               2 * static_cast<int>(sizeof(float)) * LNB_MAX_C),
-                          "cudaFuncSetAttribute(layer_norm_backward)");
-      if (rc) return rc;
-    }
+    const int groups = a.warps > 1 ? a.teams : threads / 32;
+    size_t smem = sizeof(float) * a.C;  // w
+    if (smem < combine_bytes(groups, a.C)) smem = combine_bytes(groups, a.C);
+    int rc = allow_smem(kern, smem, LNR_SMEM);
+    if (rc) return rc;
     launch_dependent(kern, grid, threads, smem, stream, a);
     return after_launch("layer_norm_backward_kernel");
   }
@@ -975,16 +1000,16 @@ int launch_layer_norm(const void* x, long ldx, int f32, const float* w, const fl
                       float* rstd, long rows, int C, cudaStream_t stream) {
   LnFwdArgs a = {x, ldx, w, b, y, mean, rstd, rows, C, 1, 1, eps};
   const int sms = device_sm_count();
-  const bool aligned = C % (f32 ? 4 : 8) == 0 && row_aligned(x, ldx, f32) && row_aligned(y, C, f32);
-  LnShape s = ln_shape(C, f32 && aligned, !f32 && aligned, f32 ? 8 : 16);
+  const int esz = f32 ? 4 : 2, px = piece_of(x, ldx, C, esz), py = piece_of(y, C, C, esz), vec = px < py ? px : py;
+  LnShape s = ln_shape(C, vec, f32 ? 8 : 16);
   const bool many = rows > 2L * sms * s.teams;
-  if (many) s = ln_shape(C, f32 && aligned, !f32 && aligned, f32 ? 16 : 24);
+  if (many) s = ln_shape(C, vec, f32 ? 16 : 24);
   if (!row_fits(C, s)) {
     const int grid = static_cast<int>(rows < 4L * sms ? rows : 4L * sms);
-    launch_dependent(f32 ? layer_norm_wide_kernel<float> : layer_norm_wide_kernel<bf16>, grid, LNB_THREADS, 0, stream, a);
+    launch_dependent(f32 ? layer_norm_wide_kernel<float> : layer_norm_wide_kernel<bf16>, grid, LNB_WIDE_THREADS, 0, stream, a);
     return after_launch("layer_norm_wide_kernel");
   }
-  const int grid = fit_teams(&s, rows, many ? 2 * sms : sms);
+  const int grid = fit_teams(&s, rows, many && s.vec > 2 ? 2 * sms : sms);
   a.warps = s.warps;
   a.teams = s.teams;
   return with_shape(s, f32 != 0, LaunchForward{a, many, grid, cta_threads(s), stream});
@@ -1005,8 +1030,11 @@ int launch_layer_norm_backward(const void* dy, long lddy, const void* x, long ld
   const int sms = device_sm_count();
   int parts = 0;
   if (rows > 0) {
-    const bool aligned = C % (f32 ? 4 : 8) == 0 && row_aligned(x, ldx, f32) && row_aligned(dy, lddy, f32) && row_aligned(dx, C, f32);
-    LnShape s = ln_shape(C, f32 && aligned, !f32 && aligned, f32 ? 8 : 16);
+    const int esz = f32 ? 4 : 2;
+    int vec = piece_of(x, ldx, C, esz);
+    for (const int other : {piece_of(dy, lddy, C, esz), piece_of(dx, C, C, esz)})
+      if (other < vec) vec = other;
+    LnShape s = ln_shape(C, vec, f32 ? 8 : 16);
     if (!row_fits(C, s)) {
       // the columns first: dx may lie where x or dy does
       parts = static_cast<int>(rows < LNB_WIDE_PARTS ? rows : LNB_WIDE_PARTS);
@@ -1016,12 +1044,12 @@ int launch_layer_norm_backward(const void* dy, long lddy, const void* x, long ld
       if (rc) return rc;
       const int grid = static_cast<int>(rows < 4L * sms ? rows : 4L * sms);
       launch_dependent(f32 ? layer_norm_backward_wide_kernel<float> : layer_norm_backward_wide_kernel<bf16>, grid,
-                       LNB_THREADS, 0, stream, a);
+                       LNB_WIDE_THREADS, 0, stream, a);
       rc = after_launch("layer_norm_backward_wide_kernel");
       if (rc) return rc;
     } else {
       const int row_bytes = C * (f32 ? 4 : 2);
-      const bool ring = f32 && s.vec > 1 && row_bytes >= 512;
+      const bool ring = f32 && s.vec == 4 && row_bytes >= 512;
       if (ring) {  // as many teams as threads and shared memory (two rows each) leave room for
         s.teams = LNR_MAX_WARPS / s.warps;
         if (s.warps > 1 && s.teams > LNB_MAX_TEAMS) s.teams = LNB_MAX_TEAMS;
@@ -1035,7 +1063,7 @@ int launch_layer_norm_backward(const void* dy, long lddy, const void* x, long ld
       if (ring) {
         const LnRing r = ring_for(s, C, row_bytes, rows, parts, dev_status);
         size_t smem = static_cast<size_t>(s.teams) * r.depth * 2 * row_bytes;
-        if (smem < 2 * sizeof(float) * C) smem = 2 * sizeof(float) * C;
+        if (smem < combine_bytes(s.teams, C)) smem = combine_bytes(s.teams, C);
         rc = with_ring(s, LaunchBackwardRing{a, r, parts, cta_threads(s), smem + sizeof(float) * C, stream});
       } else {
         rc = with_shape(s, f32 != 0, LaunchBackward{a, parts, cta_threads(s), stream});
