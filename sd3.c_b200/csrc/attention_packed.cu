@@ -190,8 +190,10 @@ attention_packed_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
   uint64_t* s_full = v_full + STAGES;        // STAGES: scores of the tile in this stage complete (its K is free)
   uint64_t* pv_done = s_full + STAGES;       // STAGES: products of the tile in this stage complete (V and P free, O quiescent)
   uint64_t* s_free = pv_done + STAGES;       // 1: scores pulled into registers (4 arrivals)
-  uint64_t* p_ready = s_free + 1;            // 1: P of the tile stored (4 arrivals)
-  uint64_t* o_free = p_ready + 1;            // 1: O of a query tile pulled into registers (4 arrivals)
+  // P_BUFS: P of the tile in this buffer stored (4 arrivals).  One for each buffer: a warp may store P of tile t + 1 before
+  // another has stored its part of tile t, and must not arrive in its place.
+  uint64_t* p_ready = s_free + 1;
+  uint64_t* o_free = p_ready + P_BUFS;       // 1: O of a query tile pulled into registers (4 arrivals)
   uint64_t* unit_full = o_free + 1;          // 2: the next query tile is known
   uint64_t* unit_free = unit_full + 2;       // 2: all who need it have read it (MMA and softmax warps: 5 arrivals)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(unit_free + 2);
@@ -213,7 +215,7 @@ attention_packed_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
       mbar_init(&pv_done[s], 1);
     }
     mbar_init(s_free, 4);
-    mbar_init(p_ready, 4);
+    for (int s = 0; s < P_BUFS; ++s) mbar_init(&p_ready[s], 4);
     mbar_init(o_free, 4);
     for (int s = 0; s < 2; ++s) {
       mbar_init(&unit_full[s], 1);
@@ -340,7 +342,7 @@ attention_packed_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
       if (pj >= 0) {
         const int st = (t - 1) % STAGES;
         ok = mbar_wait_vote(&v_full[st], ((t - 1) / STAGES) & 1, wc, DEV_TIMEOUT_ATTN_KV);
-        if (ok) ok = mbar_wait_vote(p_ready, (t - 1) & 1, wc, DEV_TIMEOUT_ATTN_P);
+        if (ok) ok = mbar_wait_vote(&p_ready[(t - 1) % P_BUFS], ((t - 1) / P_BUFS) & 1, wc, DEV_TIMEOUT_ATTN_P);
         // the first products of a query tile take O over from the one before
         if (ok && pj == 0 && pi > 0) ok = mbar_wait_vote(o_free, (pi - 1) & 1, wc, DEV_TIMEOUT_ATTN_O);
         if (!ok) break;
@@ -471,7 +473,7 @@ attention_packed_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
         tmem_wait_st();
         tc_fence_before_sync();
         __syncwarp();
-        mbar_arrive_lane0(p_ready, lane);
+        mbar_arrive_lane0(&p_ready[t % P_BUFS], lane);
       }
       if (!ok || !mbar_wait_warp(&pv_done[(t - 1) % STAGES], ((t - 1) / STAGES) & 1, wc, DEV_TIMEOUT_ATTN_O)) break;
       tc_fence_after_sync();

@@ -88,6 +88,15 @@ def test_long(sd3, D, causal):
     check(sd3, [3000, 5, 1234], 2, 1, D, causal, seed=1)
 
 
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("extra", [1, 33, 65, 97, 128])
+def test_query_tiles_with_few_rows_and_many_keys(sd3, extra, D, causal):
+    """Warps without rows, or whose rows see nothing of a key tile, run ahead of the others."""
+    for k in (3, 12):
+        check(sd3, [128 * k + extra] * 3, 9, 9, D, causal, seed=extra)
+
+
 @pytest.mark.parametrize("count", [31, 32, 33, 255, 256, 257, 700])
 def test_many_sequences(sd3, count):
     g = torch.Generator().manual_seed(count)
