@@ -12,8 +12,7 @@
 //
 // Which tile a CTA takes is found on the device, from the offsets: their values may come from an earlier kernel and may change
 // between replays of a captured graph.  The grid has room for every way in which the rows can be cut into `count` sequences.
-// Tiles run in the order of their place in their sequence, the last first: with `causal` those are the long ones, and the
-// short ones fill the end.
+// Tiles run in the order of the keys that they see, the most first; the short ones fill the end.
 //
 // Only key tiles that hold the diagonal or the end of the sequence are masked.  Keys behind the end are the next sequence's: their
 // scores become -inf, and their rows of V zeros, because 0 * inf is not 0.
@@ -92,7 +91,8 @@ __device__ Unit find_unit(const PackedArgs& a, int rank) {
   none.begin = none.len = 0;
   none.q0 = -1;
   if (a.count <= 32 * AP_SCAN_CHUNKS) {
-    // by place in the sequence, the highest first, then by sequence: tiles at place >= p number cnt(p) = sum max(0, n_s - p)
+    // Long tiles first.  causal: by place in the sequence, the highest first, then by sequence; tiles at place >= p number
+    // cnt(p) = sum max(0, n_s - p).  Else by length of the sequence; tiles of sequences of more than p number cnt(p) = sum (n_s > p) n_s.
     const int chunks = (a.count + 31) / 32;
     int n[AP_SCAN_CHUNKS], most = 0;
 #pragma unroll
@@ -103,7 +103,7 @@ __device__ Unit find_unit(const PackedArgs& a, int rank) {
     auto cnt = [&](int p) {
       int c = 0;
 #pragma unroll
-      for (int i = 0; i < AP_SCAN_CHUNKS; ++i) c += max(0, n[i] - p);
+      for (int i = 0; i < AP_SCAN_CHUNKS; ++i) c += a.causal ? max(0, n[i] - p) : n[i] > p ? n[i] : 0;
       return __reduce_add_sync(0xffffffffu, c);
     };
     int lo = 0, hi = __reduce_max_sync(0xffffffffu, most);
@@ -113,13 +113,17 @@ __device__ Unit find_unit(const PackedArgs& a, int rank) {
       if (cnt(mid) > rank) lo = mid;
       else hi = mid;
     }
-    int r = rank - cnt(lo + 1);
+    int r = rank - cnt(lo + 1), place = lo;
+    if (!a.causal) {  // among the sequences of lo + 1 tiles, each with all of them
+      place = r % (lo + 1);
+      r /= lo + 1;
+    }
 #pragma unroll
     for (int i = 0; i < AP_SCAN_CHUNKS; ++i) {
-      const unsigned has = __ballot_sync(0xffffffffu, n[i] > lo);
+      const unsigned has = __ballot_sync(0xffffffffu, a.causal ? n[i] > lo : n[i] == lo + 1);
       if (r < __popc(has)) {
         Unit u = sequence_at(a, 32 * i + static_cast<int>(__fns(has, 0, r + 1)));
-        u.q0 = lo * AP_BM;
+        u.q0 = place * AP_BM;
         return u;
       }
       r -= __popc(has);
@@ -547,7 +551,8 @@ attention_packed_heads_kernel(const __grid_constant__ CUtensorMap tmQ, const __g
   uint8_t* k_smem = q_smem + 2 * HP_TILE;
   uint8_t* v_smem = k_smem + HP_STAGES * HP_TILE;
   uint64_t* q_full = reinterpret_cast<uint64_t*>(v_smem + HP_STAGES * HP_TILE);
-  uint64_t* k_full = q_full + 1;           // HP_STAGES
+  uint64_t* q_free = q_full + 1;           // 1: the last scores of both heads of this query tile are complete
+  uint64_t* k_full = q_free + 1;           // HP_STAGES
   uint64_t* v_full = k_full + HP_STAGES;   // HP_STAGES
   uint64_t* k_free = v_full + HP_STAGES;   // HP_STAGES: both heads' scores of the tile in this stage complete
   uint64_t* v_free = k_free + HP_STAGES;   // HP_STAGES: both heads' products complete
@@ -555,17 +560,20 @@ attention_packed_heads_kernel(const __grid_constant__ CUtensorMap tmQ, const __g
   uint64_t* s_free = s_full + 2;           // 2: A, B has pulled its scores (4 arrivals)
   uint64_t* p_ready = s_free + 2;          // 2 (4 arrivals)
   uint64_t* pv_done = p_ready + 2;         // 2
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(pv_done + 2);
+  uint64_t* o_free = pv_done + 2;          // 2: O of a query tile pulled into registers (4 arrivals)
+  uint64_t* unit_full = o_free + 2;        // 2: the next query tile is known
+  uint64_t* unit_free = unit_full + 2;     // 2: all who need it have read it (MMA and softmax warps: 9 arrivals)
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(unit_free + 2);
   int* s_abort = reinterpret_cast<int*>(tmem_slot + 1);
-  int* s_unit = s_abort + 1;  // 3
+  int* s_unit = s_abort + 1;  // two times 4: first row, length, first query (below 0: no more), head A
 
   const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0);  // known uniform
   const int lane = threadIdx.x & 31;
   const int pairs = a.heads / 2;
-  const int h0 = 2 * (static_cast<int>(blockIdx.x) % pairs);
 
   if (threadIdx.x == 32) {
     mbar_init(q_full, 1);
+    mbar_init(q_free, 1);
     for (int s = 0; s < HP_STAGES; ++s) {
       mbar_init(&k_full[s], 1);
       mbar_init(&v_full[s], 1);
@@ -577,6 +585,9 @@ attention_packed_heads_kernel(const __grid_constant__ CUtensorMap tmQ, const __g
       mbar_init(&s_free[x], 4);
       mbar_init(&p_ready[x], 4);
       mbar_init(&pv_done[x], 1);
+      mbar_init(&o_free[x], 4);
+      mbar_init(&unit_full[x], 1);
+      mbar_init(&unit_free[x], 9);
     }
     *s_abort = 0;
     fence_barrier_init();
@@ -591,54 +602,78 @@ attention_packed_heads_kernel(const __grid_constant__ CUtensorMap tmQ, const __g
   }
   grid_dep_wait();  // the offsets may be the work of the preceding kernel
   grid_dep_launch();
+  Unit u;  // warp 0: the query tile of the coming round, and its first head
+  int h0 = 0;
+  auto find = [&](int i) {
+    const long w = tile_of_round(i);
+    const long rank = w / pairs;
+    h0 = 2 * static_cast<int>(w - rank * pairs);
+    u = find_unit(a, rank < (1L << 30) ? static_cast<int>(rank) : (1 << 30));
+  };
+  auto write_unit = [&](int i) {
+    int* to = s_unit + 4 * (i & 1);
+    to[0] = u.begin;
+    to[1] = u.len;
+    to[2] = u.q0;
+    to[3] = h0;
+  };
   if (warp == 0) {
-    const Unit u = find_unit(a, static_cast<int>(blockIdx.x) / pairs);
-    if (lane == 0) {
-      s_unit[0] = u.begin;
-      s_unit[1] = u.len;
-      s_unit[2] = u.q0;
-    }
+    find(0);
+    if (lane == 0) write_unit(0);
   }
   tc_fence_before_sync();
   __syncthreads();
   tc_fence_after_sync();
   const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_slot, 0);
   const WaitCtx wc{s_abort, a.status};
-  const int begin = __shfl_sync(0xffffffffu, s_unit[0], 0), len = __shfl_sync(0xffffffffu, s_unit[1], 0);
-  const int q0 = __shfl_sync(0xffffffffu, s_unit[2], 0);
-  const int keys = a.causal ? min(len, q0 + AP_BM) : len;  // that this tile's queries see
-  const int nkv = q0 < 0 ? 0 : (keys + HP_BN - 1) / HP_BN;
+  auto key_tiles = [&](int len, int q0) { return ((a.causal ? min(len, q0 + AP_BM) : len) + HP_BN - 1) / HP_BN; };  // that its queries see
 
+  // K, V, score and P buffers go round over all key tiles of all query tiles: tile number t uses stage t % HP_STAGES.
   if (warp < 4) {
     setmaxnreg_dec<HP_REGS_ISSUE>();
-    if (warp == 0 && nkv > 0) {
+    if (warp == 0) {
       // ------------------------------ TMA producer (a converged warp, one lane issues) ------
       const bool issuer = elect_one();
-      const int g = h0 / a.group;
       auto load = [&](const CUtensorMap* tm, uint8_t* to, uint64_t* bar, int head, int row) {
         tma_load_3d(to, tm, bar, 0, head, row);
         tma_load_3d(to + HP_SUB, tm, bar, 64, head, row);
       };
-      if (issuer) {
-        mbar_expect_tx(q_full, 2 * HP_TILE);
-        load(&tmQ, q_smem, q_full, h0, begin + q0);
-        load(&tmQ, q_smem + HP_TILE, q_full, h0 + 1, begin + q0);
-      }
-      for (int j = 0; j < nkv; ++j) {
-        const int st = j % HP_STAGES;
-        const uint32_t prev = ((j / HP_STAGES) + 1) & 1;  // parity of this stage's previous use
-        if (j >= HP_STAGES && !mbar_wait_vote(&k_free[st], prev, wc, DEV_TIMEOUT_ATTN_KV)) break;
+      if (lane == 0) mbar_arrive(&unit_full[0]);  // nobody waits for the first one: it is known since the barrier above
+      bool ok = true;
+      for (int i = 0, t = 0; ok && u.q0 >= 0; ++i) {
+        const Unit now = u;
+        const int g = h0 / a.group, nkv = key_tiles(now.len, now.q0);
+        if (i >= 1 && !mbar_wait_vote(q_free, (i - 1) & 1, wc, DEV_TIMEOUT_ATTN_Q)) break;
         if (issuer) {
-          mbar_expect_tx(&k_full[st], HP_TILE);
-          load(&tmK, k_smem + st * HP_TILE, &k_full[st], g, begin + j * HP_BN);
+          mbar_expect_tx(q_full, 2 * HP_TILE);
+          load(&tmQ, q_smem, q_full, h0, now.begin + now.q0);
+          load(&tmQ, q_smem + HP_TILE, q_full, h0 + 1, now.begin + now.q0);
         }
-        if (j >= HP_STAGES && !mbar_wait_vote(&v_free[st], prev, wc, DEV_TIMEOUT_ATTN_KV)) break;
-        if (issuer) {
-          mbar_expect_tx(&v_full[st], HP_TILE);
-          load(&tmV, v_smem + st * HP_TILE, &v_full[st], g, begin + j * HP_BN);
+        for (int j = 0; j < nkv && ok; ++j, ++t) {
+          const int st = t % HP_STAGES;
+          const uint32_t prev = ((t / HP_STAGES) + 1) & 1;  // parity of this stage's previous use
+          if (t >= HP_STAGES) ok = mbar_wait_vote(&k_free[st], prev, wc, DEV_TIMEOUT_ATTN_KV);
+          if (ok && issuer) {
+            mbar_expect_tx(&k_full[st], HP_TILE);
+            load(&tmK, k_smem + st * HP_TILE, &k_full[st], g, now.begin + j * HP_BN);
+          }
+          if (ok && t >= HP_STAGES) ok = mbar_wait_vote(&v_free[st], prev, wc, DEV_TIMEOUT_ATTN_KV);
+          if (ok && issuer) {
+            mbar_expect_tx(&v_full[st], HP_TILE);
+            load(&tmV, v_smem + st * HP_TILE, &v_full[st], g, now.begin + j * HP_BN);
+          }
+          if (ok && j == 0) {  // while the first tiles are under way: the next query tile, for the others too
+            find(i + 1);
+            if (i >= 1) ok = mbar_wait_vote(&unit_free[(i + 1) & 1], (((i + 1) >> 1) + 1) & 1, wc, DEV_TIMEOUT_ATTN_Q);
+            if (ok && lane == 0) {
+              write_unit(i + 1);
+              mbar_arrive(&unit_full[(i + 1) & 1]);
+            }
+            __syncwarp();
+          }
         }
       }
-    } else if (warp == 1 && nkv > 0) {
+    } else if (warp == 1) {
       // ------------------------------ MMA issuer (a converged warp, one lane issues) ------
       constexpr uint32_t IDESC_S = make_idesc(1, 1, AP_BM, HP_BN, 0, 0);  // Q K^T, both K-major
       constexpr uint32_t IDESC_O = make_idesc(1, 1, AP_BM, HP_D, 0, 1);   // P V, V is MN-major
@@ -646,60 +681,81 @@ attention_packed_heads_kernel(const __grid_constant__ CUtensorMap tmQ, const __g
       const uint64_t k_desc0 = make_smem_desc_sw128(smem_u32(k_smem), 16, 1024);
       const uint64_t v_desc0 = make_smem_desc_sw128(smem_u32(v_smem), HP_SUB, 1024);
       const bool issuer = elect_one();
-      auto issue_s = [&](int x, int j) {
-        const int st = j % HP_STAGES;
-        if (issuer) {
-#pragma unroll
-          for (int k = 0; k < HP_D / 16; ++k) {  // 16 of head_dim: 32 bytes of a 128-byte row, four to a 64-wide half
-            const uint64_t adv = static_cast<uint64_t>(((k / 4) * HP_SUB + (k % 4) * 32) >> 4);
-            mma_f16_ss(tmem_base + HP_S_COL, q_desc + static_cast<uint32_t>(x * (HP_TILE >> 4)) + adv,
-                       k_desc0 + static_cast<uint32_t>(st * (HP_TILE >> 4)) + adv, IDESC_S, k != 0);
-          }
-          mma_commit(&s_full[x]);
-          if (x == 1) mma_commit(&k_free[st]);
-        }
+      bool ok = true;
+      int nkv = 0;  // of the current query tile
+      auto next = [&](int i) {
+        if (i > 0) ok = mbar_wait_vote(&unit_full[i & 1], (i >> 1) & 1, wc, DEV_TIMEOUT_ATTN_Q);
+        if (!ok) return false;
+        const int len = __shfl_sync(0xffffffffu, s_unit[4 * (i & 1) + 1], 0), q0 = __shfl_sync(0xffffffffu, s_unit[4 * (i & 1) + 2], 0);
+        if (lane == 0) mbar_arrive(&unit_free[i & 1]);
+        nkv = key_tiles(len, q0);
+        return q0 >= 0;
       };
-      auto issue_pv = [&](int x, int j) {
-        const int st = j % HP_STAGES;
-        if (issuer) {
-#pragma unroll
-          for (int k = 0; k < HP_BN / 16; ++k)  // 16 keys: 8 columns of bf16 pairs, 16 rows of V (128 bytes each)
-            mma_f16_ts(tmem_base + HP_O_COL + x * HP_D, tmem_base + HP_P_COL + x * (HP_BN / 2) + 8 * k,
-                       v_desc0 + static_cast<uint32_t>(st * (HP_TILE >> 4)) + static_cast<uint64_t>((k * 16 * 128) >> 4), IDESC_O,
-                       (j != 0 || k != 0));
-          mma_commit(&pv_done[x]);
-          if (x == 1) mma_commit(&v_free[st]);
-        }
-      };
-      // In the order in which what they wait for comes about: scores A j+1 when B has pulled its scores j from the shared columns,
-      // products A j when P is stored, scores B j+1 when A has pulled its scores j+1, products B j.  (Products before scores: the
-      // scores waited for a whole softmax, 4130 cycles for a tile of both heads.)
-      bool ok = mbar_wait_vote(q_full, 0, wc, DEV_TIMEOUT_ATTN_Q);
-      for (int j = 0; j <= nkv && ok; ++j) {
+      // Step t: scores of tile t, products of tile t - 1, head A then head B, across query tiles, in the order in which what they
+      // wait for comes about: scores A t when B has pulled its scores t - 1 from the shared columns, products A t - 1 when P is
+      // stored, scores B t when A has pulled its scores t, products B t - 1.  (Products before scores: the scores waited for a
+      // whole softmax, 4130 cycles for a tile of both heads.)
+      int i = 0, j = 0;     // query tile, key tile in it
+      int pi = 0, pj = -1;  // those of tile t - 1; pj < 0: none
+      bool more = next(0);
+      for (int t = 0; ok && (more || pj >= 0); ++t) {
+        const int st = t % HP_STAGES, sp = (t - 1) % HP_STAGES;
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-          if (ok && j < nkv) {  // scores, once the other head has pulled those before
-            if (x == 0) ok = mbar_wait_vote(&k_full[j % HP_STAGES], (j / HP_STAGES) & 1, wc, DEV_TIMEOUT_ATTN_KV);
-            if (ok && (x == 1 || j > 0)) ok = mbar_wait_vote(&s_free[x ^ 1], (x == 1 ? j : j - 1) & 1, wc, DEV_TIMEOUT_ATTN_S);
+          if (ok && more) {
+            if (x == 0 && j == 0) ok = mbar_wait_vote(q_full, i & 1, wc, DEV_TIMEOUT_ATTN_Q);
+            if (ok && x == 0) ok = mbar_wait_vote(&k_full[st], (t / HP_STAGES) & 1, wc, DEV_TIMEOUT_ATTN_KV);
+            if (ok && (x == 1 || t > 0)) ok = mbar_wait_vote(&s_free[x ^ 1], (x == 1 ? t : t - 1) & 1, wc, DEV_TIMEOUT_ATTN_S);
             if (ok) {
               tc_fence_after_sync();
-              issue_s(x, j);
+              if (issuer) {
+#pragma unroll
+                for (int k = 0; k < HP_D / 16; ++k) {  // 16 of head_dim: 32 bytes of a 128-byte row, four to a 64-wide half
+                  const uint64_t adv = static_cast<uint64_t>(((k / 4) * HP_SUB + (k % 4) * 32) >> 4);
+                  mma_f16_ss(tmem_base + HP_S_COL, q_desc + static_cast<uint32_t>(x * (HP_TILE >> 4)) + adv,
+                             k_desc0 + static_cast<uint32_t>(st * (HP_TILE >> 4)) + adv, IDESC_S, k != 0);
+                }
+                mma_commit(&s_full[x]);
+                if (x == 1) {
+                  mma_commit(&k_free[st]);
+                  if (j == nkv - 1) mma_commit(q_free);
+                }
+              }
             }
           }
-          if (ok && j > 0) {  // products of the tile before
-            if (x == 0) ok = mbar_wait_vote(&v_full[(j - 1) % HP_STAGES], ((j - 1) / HP_STAGES) & 1, wc, DEV_TIMEOUT_ATTN_KV);
-            if (ok) ok = mbar_wait_vote(&p_ready[x], (j - 1) & 1, wc, DEV_TIMEOUT_ATTN_P);
+          if (ok && pj >= 0) {
+            if (x == 0) ok = mbar_wait_vote(&v_full[sp], ((t - 1) / HP_STAGES) & 1, wc, DEV_TIMEOUT_ATTN_KV);
+            if (ok) ok = mbar_wait_vote(&p_ready[x], (t - 1) & 1, wc, DEV_TIMEOUT_ATTN_P);
+            // the first products of a query tile take O over from the one before
+            if (ok && pj == 0 && pi > 0) ok = mbar_wait_vote(&o_free[x], (pi - 1) & 1, wc, DEV_TIMEOUT_ATTN_O);
             if (ok) {
               tc_fence_after_sync();
-              issue_pv(x, j - 1);
+              if (issuer) {
+#pragma unroll
+                for (int k = 0; k < HP_BN / 16; ++k)  // 16 keys: 8 columns of bf16 pairs, 16 rows of V (128 bytes each)
+                  mma_f16_ts(tmem_base + HP_O_COL + x * HP_D, tmem_base + HP_P_COL + x * (HP_BN / 2) + 8 * k,
+                             v_desc0 + static_cast<uint32_t>(sp * (HP_TILE >> 4)) + static_cast<uint64_t>((k * 16 * 128) >> 4),
+                             IDESC_O, (pj != 0 || k != 0));
+                mma_commit(&pv_done[x]);
+                if (x == 1) mma_commit(&v_free[sp]);
+              }
             }
+          }
+        }
+        pj = -1;
+        if (ok && more) {
+          pi = i;
+          pj = j;
+          if (++j == nkv) {
+            j = 0;
+            more = next(++i);
           }
         }
       }
     }
   } else {
     setmaxnreg_inc<HP_REGS_SOFTMAX>();
-    if (nkv > 0) {
+    {
       // ------------------------------ softmax + epilogue ------------------------
       const int x = (warp - 4) >> 2;  // A, B
       const int quad = warp & 3;
@@ -708,100 +764,115 @@ attention_packed_heads_kernel(const __grid_constant__ CUtensorMap tmQ, const __g
       const uint32_t s_tmem = lane_base + HP_S_COL, p_tmem = lane_base + HP_P_COL + x * (HP_BN / 2);
       const uint32_t o_tmem = lane_base + HP_O_COL + x * HP_D;
       const float c = a.scale_log2e;
-      const int seen = a.causal ? min(len, q0 + row + 1) : len;  // keys that this row sees, at least one
-      float m_used = -INFINITY;  // running maximum (raw score units) that the exponentials refer to
-      float2 l2 = make_float2(0.f, 0.f);
       bool ok = true;
       uint32_t r0[32], r1[32], r2[32], r3[32];
-      for (int j = 0; j < nkv; ++j) {
-        const int kv0 = j * HP_BN;
-        const bool masked = j == nkv - 1;
-        if (!mbar_wait_warp(&s_full[x], j & 1, wc, DEV_TIMEOUT_ATTN_S)) { ok = false; break; }
+      for (int i = 0, t = 0; ok; ++i) {
+        if (i > 0 && !mbar_wait_warp(&unit_full[i & 1], (i >> 1) & 1, wc, DEV_TIMEOUT_ATTN_Q)) break;
+        const int* unit = s_unit + 4 * (i & 1);
+        const int begin = __shfl_sync(0xffffffffu, unit[0], 0), len = __shfl_sync(0xffffffffu, unit[1], 0);
+        const int q0 = __shfl_sync(0xffffffffu, unit[2], 0), h = __shfl_sync(0xffffffffu, unit[3], 0) + x;
+        mbar_arrive_lane0(&unit_free[i & 1], lane);
+        if (q0 < 0) break;
+        const int nkv = key_tiles(len, q0);
+        const int seen = a.causal ? min(len, q0 + row + 1) : len;  // keys that this row sees, at least one
+        float m_used = -INFINITY;  // running maximum (raw score units) that the exponentials refer to
+        float2 l2 = make_float2(0.f, 0.f);
+        for (int j = 0; j < nkv; ++j, ++t) {
+          const int kv0 = j * HP_BN;
+          const bool masked = j == nkv - 1;
+          if (!mbar_wait_warp(&s_full[x], t & 1, wc, DEV_TIMEOUT_ATTN_S)) { ok = false; break; }
+          tc_fence_after_sync();
+          tmem_ld_32x32b_x32(s_tmem, r0);
+          tmem_ld_32x32b_x32(s_tmem + 32, r1);
+          tmem_ld_32x32b_x32(s_tmem + 64, r2);
+          tmem_ld_32x32b_x32(s_tmem + 96, r3);
+          tmem_wait_ld();
+          tc_fence_before_sync();
+          __syncwarp();
+          mbar_arrive_lane0(&s_free[x], lane);  // the columns can take the other head's scores
+          if (masked) {
+            mask_cols(r0, kv0, seen);
+            mask_cols(r1, kv0 + 32, seen);
+            mask_cols(r2, kv0 + 64, seen);
+            mask_cols(r3, kv0 + 96, seen);
+          }
+          uint32_t pre_pv = 1;
+          if (j >= 1) pre_pv = mbar_test_wait(&pv_done[x], (t - 1) & 1);
+          const float mx = fmaxf(max_of2(r0, r1), max_of2(r2, r3));
+          const bool need = (mx - m_used) * c > 8.0f;  // always true in the first tile (m_used = -inf)
+          if (__any_sync(0xffffffffu, need)) {
+            float alpha = 1.0f;
+            if (need) {
+              alpha = ex2_approx((m_used - mx) * c);
+              m_used = mx;
+              l2.x *= alpha;
+              l2.y *= alpha;
+            }
+            if (j >= 1) {
+              ok = mbar_wait_pre(pre_pv, &pv_done[x], (t - 1) & 1, wc, DEV_TIMEOUT_ATTN_O);
+              pre_pv = 1;
+              if (ok) rescale_row<HP_D>(o_tmem, alpha);
+            }
+          }
+          const float nmc = -m_used * c;
+          exp_pack<false>(r0, c, nmc, l2);
+          exp_pack<false>(r1, c, nmc, l2);
+          // P is free once the products of the previous tile are complete
+          if (j >= 1 && ok) ok = mbar_wait_pre(pre_pv, &pv_done[x], (t - 1) & 1, wc, DEV_TIMEOUT_ATTN_O);
+          if (!ok) break;
+          tmem_st_32x32b_x16(p_tmem, reinterpret_cast<uint32_t(&)[16]>(r0));
+          tmem_st_32x32b_x16(p_tmem + 16, reinterpret_cast<uint32_t(&)[16]>(r1));
+          exp_pack<false>(r2, c, nmc, l2);
+          exp_pack<false>(r3, c, nmc, l2);
+          tmem_st_32x32b_x16(p_tmem + 32, reinterpret_cast<uint32_t(&)[16]>(r2));
+          tmem_st_32x32b_x16(p_tmem + 48, reinterpret_cast<uint32_t(&)[16]>(r3));
+          if (kv0 + HP_BN > len) {
+            // rows of V behind the sequence's end become zeros, whatever they are (both heads' warps write the same zeros)
+            ok = mbar_wait_warp(&v_full[t % HP_STAGES], (t / HP_STAGES) & 1, wc, DEV_TIMEOUT_ATTN_KV);
+            if (ok && kv0 + row >= len) {
+#pragma unroll
+              for (int s = 0; s < 2; ++s)
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
+                  *reinterpret_cast<uint4*>(v_smem + (t % HP_STAGES) * HP_TILE + s * HP_SUB + row * 128 + k * 16) =
+                      make_uint4(0, 0, 0, 0);
+            }
+            fence_proxy_async_smem();
+          }
+          tmem_wait_st();
+          tc_fence_before_sync();
+          __syncwarp();
+          mbar_arrive_lane0(&p_ready[x], lane);
+        }
+        if (!ok || !mbar_wait_warp(&pv_done[x], (t - 1) & 1, wc, DEV_TIMEOUT_ATTN_O)) break;
         tc_fence_after_sync();
-        tmem_ld_32x32b_x32(s_tmem, r0);
-        tmem_ld_32x32b_x32(s_tmem + 32, r1);
-        tmem_ld_32x32b_x32(s_tmem + 64, r2);
-        tmem_ld_32x32b_x32(s_tmem + 96, r3);
+        const float inv = 1.0f / (l2.x + l2.y);
+        uint4* to = reinterpret_cast<uint4*>(a.out + static_cast<long>(begin + q0 + row) * a.ldo + h * HP_D);
+        auto store = [&](uint32_t (&o)[32], int part) {
+          if (q0 + row < len) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              uint4 v;
+              v.x = pack_bf16x2(__uint_as_float(o[8 * k]) * inv, __uint_as_float(o[8 * k + 1]) * inv);
+              v.y = pack_bf16x2(__uint_as_float(o[8 * k + 2]) * inv, __uint_as_float(o[8 * k + 3]) * inv);
+              v.z = pack_bf16x2(__uint_as_float(o[8 * k + 4]) * inv, __uint_as_float(o[8 * k + 5]) * inv);
+              v.w = pack_bf16x2(__uint_as_float(o[8 * k + 6]) * inv, __uint_as_float(o[8 * k + 7]) * inv);
+              to[4 * part + k] = v;
+            }
+          }
+        };
+        tmem_ld_32x32b_x32(o_tmem, r0);
+        tmem_ld_32x32b_x32(o_tmem + 32, r1);
+        tmem_ld_32x32b_x32(o_tmem + 64, r2);
+        tmem_ld_32x32b_x32(o_tmem + 96, r3);
         tmem_wait_ld();
         tc_fence_before_sync();
         __syncwarp();
-        mbar_arrive_lane0(&s_free[x], lane);  // the columns can take the other head's scores
-        if (masked) {
-          mask_cols(r0, kv0, seen);
-          mask_cols(r1, kv0 + 32, seen);
-          mask_cols(r2, kv0 + 64, seen);
-          mask_cols(r3, kv0 + 96, seen);
-        }
-        uint32_t pre_pv = 1;
-        if (j >= 1) pre_pv = mbar_test_wait(&pv_done[x], (j - 1) & 1);
-        const float mx = fmaxf(max_of2(r0, r1), max_of2(r2, r3));
-        const bool need = (mx - m_used) * c > 8.0f;  // always true in the first tile (m_used = -inf)
-        if (__any_sync(0xffffffffu, need)) {
-          float alpha = 1.0f;
-          if (need) {
-            alpha = ex2_approx((m_used - mx) * c);
-            m_used = mx;
-            l2.x *= alpha;
-            l2.y *= alpha;
-          }
-          if (j >= 1) {
-            ok = mbar_wait_pre(pre_pv, &pv_done[x], (j - 1) & 1, wc, DEV_TIMEOUT_ATTN_O);
-            pre_pv = 1;
-            if (ok) rescale_row<HP_D>(o_tmem, alpha);
-          }
-        }
-        const float nmc = -m_used * c;
-        exp_pack<false>(r0, c, nmc, l2);
-        exp_pack<false>(r1, c, nmc, l2);
-        // P is free once the products of the previous tile are complete
-        if (j >= 1 && ok) ok = mbar_wait_pre(pre_pv, &pv_done[x], (j - 1) & 1, wc, DEV_TIMEOUT_ATTN_O);
-        if (!ok) break;
-        tmem_st_32x32b_x16(p_tmem, reinterpret_cast<uint32_t(&)[16]>(r0));
-        tmem_st_32x32b_x16(p_tmem + 16, reinterpret_cast<uint32_t(&)[16]>(r1));
-        exp_pack<false>(r2, c, nmc, l2);
-        exp_pack<false>(r3, c, nmc, l2);
-        tmem_st_32x32b_x16(p_tmem + 32, reinterpret_cast<uint32_t(&)[16]>(r2));
-        tmem_st_32x32b_x16(p_tmem + 48, reinterpret_cast<uint32_t(&)[16]>(r3));
-        if (kv0 + HP_BN > len) {
-          // rows of V behind the sequence's end become zeros, whatever they are (both heads' warps write the same zeros)
-          ok = mbar_wait_warp(&v_full[j % HP_STAGES], (j / HP_STAGES) & 1, wc, DEV_TIMEOUT_ATTN_KV);
-          if (ok && kv0 + row >= len) {
-#pragma unroll
-            for (int s = 0; s < 2; ++s)
-#pragma unroll
-              for (int i = 0; i < 8; ++i)
-                *reinterpret_cast<uint4*>(v_smem + (j % HP_STAGES) * HP_TILE + s * HP_SUB + row * 128 + i * 16) =
-                    make_uint4(0, 0, 0, 0);
-          }
-          fence_proxy_async_smem();
-        }
-        tmem_wait_st();
-        tc_fence_before_sync();
-        __syncwarp();
-        mbar_arrive_lane0(&p_ready[x], lane);
-      }
-      const float l = l2.x + l2.y;
-      if (ok && mbar_wait_warp(&pv_done[x], (nkv - 1) & 1, wc, DEV_TIMEOUT_ATTN_O)) {
-        tc_fence_after_sync();
-        const float inv = 1.0f / l;
-        uint4* to = reinterpret_cast<uint4*>(a.out + static_cast<long>(begin + q0 + row) * a.ldo + (h0 + x) * HP_D);
-#pragma unroll 1
-        for (int part = 0; part < HP_D / 32; ++part) {
-          uint32_t o[32];
-          tmem_ld_32x32b_x32(o_tmem + 32 * part, o);
-          tmem_wait_ld();
-          if (q0 + row < len) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              uint4 u;
-              u.x = pack_bf16x2(__uint_as_float(o[8 * i]) * inv, __uint_as_float(o[8 * i + 1]) * inv);
-              u.y = pack_bf16x2(__uint_as_float(o[8 * i + 2]) * inv, __uint_as_float(o[8 * i + 3]) * inv);
-              u.z = pack_bf16x2(__uint_as_float(o[8 * i + 4]) * inv, __uint_as_float(o[8 * i + 5]) * inv);
-              u.w = pack_bf16x2(__uint_as_float(o[8 * i + 6]) * inv, __uint_as_float(o[8 * i + 7]) * inv);
-              to[4 * part + i] = u;
-            }
-          }
-        }
+        mbar_arrive_lane0(&o_free[x], lane);  // the next query tile's products may begin
+        store(r0, 0);
+        store(r1, 1);
+        store(r2, 2);
+        store(r3, 3);
       }
     }
   }
@@ -844,7 +915,9 @@ int launch_heads(const CUtensorMap* tm, const PackedArgs& a, long units, cudaStr
   static bool done[64] = {false};
   int rc = prepare_kernel(attention_packed_heads_kernel, HP_SMEM_BYTES, HP_REGS_LAUNCH, done);
   if (rc) return rc;
-  launch_dependent(attention_packed_heads_kernel, static_cast<unsigned>(units * (a.heads / 2)), HP_THREADS, HP_SMEM_BYTES, stream,
+  const long tiles = units * (a.heads / 2), slots = device_sm_count();
+  const bool rounds = tiles > slots && packed_rounds(a.rows, a.count);
+  launch_dependent(attention_packed_heads_kernel, static_cast<unsigned>(rounds ? slots : tiles), HP_THREADS, HP_SMEM_BYTES, stream,
                    tm[0], tm[1], tm[2], a);
   return after_launch("attention_packed_heads_kernel");
 }
