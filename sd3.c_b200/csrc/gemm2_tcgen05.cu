@@ -418,6 +418,13 @@ bool narrow_tiles_built(const GemmEpilogue& epi) {
   return epi.mode == EPI_BIAS || epi.mode == EPI_BIAS_GELU || epi.mode == EPI_QKV_NORM;
 }
 
+// whether TMA boxes can describe the rows of the output and of what is added
+bool act_resid_boxes(const GemmEpilogue& e) {
+  const long esz = e.out_f32 ? 4 : 2;
+  return (e.ldo * esz) % 16 == 0 && (reinterpret_cast<uintptr_t>(e.out) & 15) == 0 &&
+         (!e.add || ((e.ld_add * esz) % 16 == 0 && (reinterpret_cast<uintptr_t>(e.add) & 15) == 0));
+}
+
 // Tensor maps and arguments of one problem for pair tiles of width pbn.
 int build_problem(PairProblem* pp, const GemmProblem& q, int operand_dtype, int N, int K, int pbn,
                   int* dev_status) {
@@ -451,11 +458,6 @@ int build_problem(PairProblem* pp, const GemmProblem& q, int operand_dtype, int 
     rc = encode_tmap_2d(&pp->tmR, epi.resid, 4, (uint64_t)N, (uint64_t)M, (uint64_t)epi.ldo * 4, 32, 32);
     if (rc) return rc;
   }
-  if (epi.mode == EPI_ACT_RESID) {  // boxes of 128 bytes x 32 rows; what lies outside (M, N) is neither read nor written
-    rc = encode_tmap_2d(&pp->tmR, epi.out, f32 ? 4 : 2, (uint64_t)N, (uint64_t)M, (uint64_t)epi.ldo * (f32 ? 4 : 2),
-                        f32 ? 32 : 64, 32);
-    if (rc) return rc;
-  }
   // bf16 outputs leave through a TMA store when every warp's 32 rows are 32 consecutive
   // output rows that all exist
   g.tma_store = 0;
@@ -467,6 +469,12 @@ int build_problem(PairProblem* pp, const GemmProblem& q, int operand_dtype, int 
                                 ? (uint64_t)(M / epi.rows_in - 1) * epi.rows_out + epi.row_off + epi.rows_in
                                 : (uint64_t)M;
     rc = encode_tmap_2d(&pp->tmR, epi.out, 2, (uint64_t)N, extent, (uint64_t)epi.ldo * 2, 64, 32);
+    if (rc) return rc;
+    g.tma_store = 1;
+  }
+  if (epi.mode == EPI_ACT_RESID && act_resid_boxes(epi)) {  // what lies outside (M, N) is neither read nor written
+    rc = encode_tmap_2d(&pp->tmR, epi.out, f32 ? 4 : 2, (uint64_t)N, (uint64_t)M, (uint64_t)epi.ldo * (f32 ? 4 : 2),
+                        f32 ? 32 : 64, 32);
     if (rc) return rc;
     g.tma_store = 1;
   }
@@ -528,7 +536,7 @@ int launch_gemm_pair(const GemmProblem* q, int n, int operand_dtype, int N, int 
     end[i] = count;
   }
   const PairTiles tiles{end[0], end[1], end[2], sum ? 1 : 0};
-  if (a.epi.mode == EPI_ACT_RESID && a.epi.add) {
+  if (a.epi.mode == EPI_ACT_RESID && a.epi.add && act_resid_boxes(a.epi)) {
     const int esz = a.epi.out_f32 ? 4 : 2;
     int rc = encode_tmap_2d(&p[1].tmR, a.epi.add, esz, (uint64_t)N, (uint64_t)a.M, (uint64_t)a.epi.ld_add * esz,
                             128 / esz, 32);

@@ -500,6 +500,8 @@ __device__ __forceinline__ void load_bias32(const float* p, int n, int N, bool w
 // epilogue, out-projection of 32768 rows: 0.18 ms by registers, 0.14 through boxes).  Two buffers: the box to
 // add is requested two boxes ahead, across tiles, into the buffer that its result will leave from.  Chunk c (16 bytes) of
 // row r lies at chunk c ^ (r & 7): the 128-byte swizzle of the tensor maps, free of bank conflicts row by row.
+// Rows that no TMA box can describe (row pitches and addresses that are no multiples of 16 bytes) go through a box as well, 32 fp32
+// columns at a time, and from there row by row, a column a lane: whole lines, whatever the pitch.
 template <int BN, bool OUT_F32>
 struct ActResidBoxes {
   static constexpr int COLS = OUT_F32 ? 32 : 64;  // of a box
@@ -517,7 +519,7 @@ struct ActResidBoxes {
     tm_out = out_map; tm_add = add_map; g = &args; buf = buffers; bar = bars;
     quad = quad_; half = half_; rank = rank_; num_pairs = num_pairs_;
     ahead_tile = pair; ahead_box = 0; count = 0;
-    if (g->epi.add) {
+    if (g->epi.add && g->tma_store) {
       request(0);
       request(1);
     }
@@ -536,6 +538,41 @@ struct ActResidBoxes {
           tma_load_2d(buf + b * 4096, tm_add, &bar[b], n, m);
         }
         return;
+      }
+    }
+  }
+  // 32 columns of this lane's row, bias and activation done: through the warp's box to rows m, columns n of the output
+  __device__ __forceinline__ void put_rows(const float (&v)[32], int m, int n) const {
+    const GemmEpilogue& e = g->epi;
+    const int lane = threadIdx.x & 31, swz = lane & 7;
+    __syncwarp();  // the chunk before has been read
+#pragma unroll
+    for (int c = 0; c < 8; ++c)
+      *reinterpret_cast<float4*>(buf + lane * 128 + ((c ^ swz) << 4)) = make_float4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
+    __syncwarp();
+    if (n + lane >= g->N) return;
+    const int rows = min(32, g->M - m);
+    const long at = static_cast<long>(m) * e.ldo + n + lane, from = static_cast<long>(m) * e.ld_add + n + lane;
+#pragma unroll 1
+    for (int r0 = 0; r0 < rows; r0 += 8) {
+      float o[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {  // the last row again for those that do not exist
+        const long r = min(r0 + k, rows - 1);
+        o[k] = 0.f;
+        if (e.add) {
+          if constexpr (OUT_F32) o[k] = static_cast<const float*>(e.add)[from + r * e.ld_add];
+          else o[k] = __bfloat162float(static_cast<const bf16*>(e.add)[from + r * e.ld_add]);
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int r = r0 + k;
+        if (r < rows) {
+          o[k] += *reinterpret_cast<const float*>(buf + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4);
+          if constexpr (OUT_F32) static_cast<float*>(e.out)[at + r * e.ldo] = o[k];
+          else static_cast<bf16*>(e.out)[at + r * e.ldo] = __float2bfloat16_rn(o[k]);
+        }
       }
     }
   }
@@ -607,7 +644,7 @@ struct ActResidBoxes {
     for (int i = 0; i < BOXES; ++i) {
       const int n = nw + i * COLS;
       if (!exists(*g, m, n)) break;
-      if (!open_box(wc)) return false;
+      if (g->tma_store && !open_box(wc)) return false;
 #pragma unroll
       for (int h = 0; h < COLS / 32; ++h) {
         uint32_t r[32];
@@ -618,9 +655,10 @@ struct ActResidBoxes {
         for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]) + bb[j];
         load_bias32(e.bias, n + (h + 1) * 32, g->N, whole, bb);  // the next chunk's
         activate_chunk(v, e.act);
-        put(v, h);
+        if (g->tma_store) put(v, h);
+        else put_rows(v, m, n + h * 32);
       }
-      close_box(m, n);
+      if (g->tma_store) close_box(m, n);
     }
     return true;
   }
@@ -651,6 +689,10 @@ struct ActResidBoxes {
 #pragma unroll
       for (int j = 0; j < 32; ++j) v[j] = sums[i * 32 + j];
       activate_chunk(v, e.act);
+      if (!g->tma_store) {
+        put_rows(v, m, n);
+        continue;
+      }
       if (!open_box(wc)) return false;
       put(v, 0);
       close_box(m, n);

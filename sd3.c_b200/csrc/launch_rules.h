@@ -84,12 +84,13 @@ inline int pair_tile_width(long tiles256, long after256, int K, bool fp8, bool g
 //   512  1536  1536   64/1  9.2     P  9.6
 //   600  1536  1536   64/1  8.7     P  9.6
 //   1024 1536  6144   P 24.9        128/1 36.1
-//   1357 1001  1544   128/1 17.3    64/1 24.4   (rows that no TMA store can write)
+//   1357 1001  1544   P 16.3        128/1 17.3   64/1 24.4
+//   5843 4693  1496   P 168         128/1 254    (fp32)
 struct LinearPlan {
   bool pair;
   int bn, split;
 };
-inline LinearPlan linear_plan(int M, int N, int k_blocks, bool tma_out, bool f32, int sms) {
+inline LinearPlan linear_plan(int M, int N, int k_blocks, bool f32, int sms) {
   const long rows = (M + 127) / 128;
   const long tiles64 = rows * ((N + 63) / 64);
   if (tiles64 <= sms) {
@@ -97,18 +98,31 @@ inline LinearPlan linear_plan(int M, int N, int k_blocks, bool tma_out, bool f32
     while (split < 8 && 2 * split <= k_blocks && 2 * split * tiles64 <= sms) split *= 2;
     return {false, 64, split};
   }
-  if (tma_out && rows > 1) return {true, 0, 1};
-  // fp32 sums of more than 2048 of K want more accumulators than 128-wide tiles leave room for
+  if (rows > 1) return {true, 0, 1};
+  // fp32 sums are kept in parts of 512 of K, and 128-wide tiles leave room for four (linear_residual.cu): 77 x 12288 with K
+  // 4096 is off by 1.0e-6 in them (24 us), by 4.8e-7 in 64-wide ones (30 us)
   return {false, f32 && k_blocks > 32 ? 64 : 128, 1};
 }
 
-// Packed attention: whether two query heads of one key / value head share a CTA.
+// Packed attention: whether two query heads of one key / value head share a CTA (they read it once, and the softmax of one
+// runs under the products of the other; a CTA per SM, so short sequences leave more of it idle).  us, one / two heads, 32 heads
+// over 8 of 128:
+//   sequences x tokens   32 x 128    16 x 512    8 x 768     1 x 1024    8 x 1024    4 x 2048    1 x 8192
+//   causal               38.3 47.5   70.5 75.7   67.0 69.3   24.5 21.7   99.9 98.4   187 170     553 505
+//   all keys             30.4 39.5   88.2 91.2   103 101     26.2 23.0   154 143     289 271     1084 969
+// (8 heads over 1, causal: 12.0 11.8, 22.2 22.4, 20.0 20.6, 18.5 20.6, 27.6 27.1, 43.7 40.6, 144 124)
 inline bool packed_two_heads(int head_dim, int group, int rows, int count) {
-  return head_dim == 128 && group % 2 == 0 && rows >= 256L * count;
+  return head_dim == 128 && group % 2 == 0 && rows >= 768L * count;
 }
 
 // Packed attention, one head a CTA: whether the CTAs that fit the SMs go through the tiles in rounds, or each tile has a CTA of
-// its own (where tiles are long, the order in which SMs become free shares them out better).
-inline bool packed_rounds(int rows, int count) { return rows < 1024L * count; }
+// its own (where tiles are long, the order in which SMs become free shares them out better, and starting a CTA is nothing).
+// us, own / rounds:
+//   sequences x tokens             64 x 1      32 x 200    16 x 512    8 x 1024    4 x 2048    1 x 8192
+//   16 heads of 64, all keys       26.8 19.9   33.4 25.9   40.7 33.4   59.8 57.3   101 104     357 380
+//   32 over 8 of 64, causal        48.9 33.3   55.9 40.4   65.2 50.5   84.7 73.0   122 117     366 378
+//   16 heads of 128, causal        26.9 20.8   41.2 31.2   49.1 42.0   62.3 53.3   90.7 89.4   278 277
+//   16 heads of 128, all keys      32.3 24.8   48.6 37.7   58.3 50.1   85.5 81.7   146 158     510 574
+inline bool packed_rounds(int rows, int count) { return rows < 2048L * count; }
 
 }  // namespace sd3

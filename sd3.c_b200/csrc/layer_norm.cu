@@ -380,16 +380,19 @@ struct LnBwdArgs {
   long ldx;
   const float *w, *mean, *rstd;
   void* dx;
-  float* partial;  // (gridDim.x, 2, C): this CTA's share of dw and db
+  float* partial;  // (gridDim.x, 2, C): the CTAs' shares of dw and db; null: a lone CTA writes them itself
+  float *dw, *db;
   long rows;
   int C, warps, teams;
+  __device__ __forceinline__ float* part_w() const { return partial ? partial + static_cast<long>(blockIdx.x) * 2 * C : dw; }
+  __device__ __forceinline__ float* part_b() const { return partial ? partial + (static_cast<long>(blockIdx.x) * 2 + 1) * C : db; }
 };
 
 // dw and db of a CTA: its groups' sums, added in pairs through shared memory (groups / 2 times 2 C floats), always in the same
 // order; group 0 writes the result.  `mine`: this thread holds pieces (of a group that repeats them in several lanes, one does).
 template <int VEC, int NV>
 __device__ __forceinline__ void combine_groups(float (&dw)[NV][VEC], float (&db)[NV][VEC], float* smem, int group, int groups,
-                                               int t, int ts, int C, bool mine, float* out) {
+                                               int t, int ts, int C, bool mine, float* to_w, float* to_b) {
   constexpr int W = VEC >= 4 ? 4 : VEC;
   struct alignas(4 * W) Piece { float f[W]; };
   const int nvec = C / VEC;
@@ -429,8 +432,8 @@ __device__ __forceinline__ void combine_groups(float (&dw)[NV][VEC], float (&db)
       Piece p, q;
 #pragma unroll
       for (int k = 0; k < W; ++k) { p.f[k] = dw[i][j + k]; q.f[k] = db[i][j + k]; }
-      *reinterpret_cast<Piece*>(out + at) = p;
-      *reinterpret_cast<Piece*>(out + C + at) = q;
+      if (to_w) *reinterpret_cast<Piece*>(to_w + at) = p;
+      if (to_b) *reinterpret_cast<Piece*>(to_b + at) = q;
     });
 }
 
@@ -573,7 +576,7 @@ __global__ void __launch_bounds__(lnb_threads(VEC), 1) layer_norm_backward_kerne
   const int group = a.warps > 1 ? team : static_cast<int>(threadIdx.x >> 5);
   const int groups = a.warps > 1 ? a.teams : static_cast<int>(blockDim.x >> 5);
   const bool mine = a.warps > 1 || (threadIdx.x & 31) < LANES;
-  combine_groups<VEC, NV>(dw, db, sums, group, groups, t, ts, a.C, mine, a.partial + static_cast<long>(blockIdx.x) * 2 * a.C);
+  combine_groups<VEC, NV>(dw, db, sums, group, groups, t, ts, a.C, mine, a.part_w(), a.part_b());
 }
 
 // dw and db: the sums of `parts` partial rows of 2 C values.  Thread k of the 32 of a column adds parts k, k + 32, ...; then the
@@ -741,8 +744,7 @@ __global__ void __launch_bounds__(LNR_THREADS, 1) layer_norm_backward_ring_kerne
   }
   __syncthreads();  // every row has landed and been read: the rings hold the sums from here on
   if (s_abort) drain_after_abort();
-  combine_groups<VEC, NV>(dw, db, reinterpret_cast<float*>(rows_smem), team, a.teams, t, ts, a.C, true,
-                          a.partial + static_cast<long>(blockIdx.x) * 2 * a.C);
+  combine_groups<VEC, NV>(dw, db, reinterpret_cast<float*>(rows_smem), team, a.teams, t, ts, a.C, true, a.part_w(), a.part_b());
 }
 
 // ----------------------------------------------------------------------------
@@ -1026,7 +1028,7 @@ size_t layer_norm_backward_scratch_bytes(long rows, int C) {
 int launch_layer_norm_backward(const void* dy, long lddy, const void* x, long ldx, int f32, const float* w,
                                const float* mean, const float* rstd, void* dx, float* dw, float* db, long rows, int C,
                                float* scratch, int* dev_status, cudaStream_t stream) {
-  LnBwdArgs a = {dy, lddy, x, ldx, w, mean, rstd, dx, scratch, rows, C, 1, 1};
+  LnBwdArgs a = {dy, lddy, x, ldx, w, mean, rstd, dx, scratch, dw, db, rows, C, 1, 1};
   const int sms = device_sm_count();
   int parts = 0;
   if (rows > 0) {
@@ -1056,7 +1058,10 @@ int launch_layer_norm_backward(const void* dy, long lddy, const void* x, long ld
         const long most = (LNR_SMEM - 4L * C) / (4L * row_bytes);
         if (s.teams > most) s.teams = static_cast<int>(most);
       }
-      parts = fit_teams(&s, rows, sms);
+      // Few rows: a lone CTA with a row a team, which needs no second kernel (one row of 64: 3.0 -> 2.1 us, and a launch less)
+      const bool lone = rows <= s.teams && ((reinterpret_cast<uintptr_t>(dw) | reinterpret_cast<uintptr_t>(db)) & 15) == 0;
+      parts = fit_teams(&s, rows, lone ? 1 : sms);
+      if (lone) a.partial = nullptr;
       a.warps = s.warps;
       a.teams = s.teams;
       int rc;
@@ -1068,7 +1073,7 @@ int launch_layer_norm_backward(const void* dy, long lddy, const void* x, long ld
       } else {
         rc = with_shape(s, f32 != 0, LaunchBackward{a, parts, cta_threads(s), stream});
       }
-      if (rc) return rc;
+      if (rc || lone) return rc;
     }
   }
   launch_dependent(layer_norm_columns_kernel, (2 * C + 31) / 32, 1024, 0, stream, scratch, parts, C, dw, db);

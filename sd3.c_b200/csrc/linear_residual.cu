@@ -1,5 +1,4 @@
-// out = act(x w^T + bias) + add for the sizes that the CTA-pair GEMM does not cover or would leave most SMs idle with:
-// few rows, odd widths, outputs whose rows no TMA store can write.
+// out = act(x w^T + bias) + add for the sizes that would leave most SMs idle in the CTA-pair GEMM: few rows, few columns.
 //
 //   acc[m, n] = sum_k x[m, k] w[n, k],   out = act(acc + bias[n]) + add[m, n]
 //
@@ -26,7 +25,6 @@ namespace sd3 {
 int encode_tmap_2d(CUtensorMap* map, const void* base, int elem_bytes, uint64_t inner, uint64_t outer, uint64_t ld_bytes,
                    uint32_t box_inner, uint32_t box_outer);
 int device_sm_count();
-bool gemm_pair_supported(int operand_dtype, int M, int N, int K, const GemmEpilogue& epi);
 int launch_gemm_pair(const GemmProblem* q, int n, int operand_dtype, int N, int K, int* dev_status, cudaStream_t stream);
 
 namespace {
@@ -392,11 +390,9 @@ int launch_inst(const CUtensorMap& tmA, const CUtensorMap& tmW, const LinearArgs
 int launch_linear_residual(const bf16* x, long lda, const bf16* w, long ldw, int M, int N, int K, const GemmEpilogue& epi,
                            int* dev_status, cudaStream_t stream) {
   const long esz = epi.out_f32 ? 4 : 2;
-  const bool tma_out = (epi.ldo * esz) % 16 == 0 && (reinterpret_cast<uintptr_t>(epi.out) & 15) == 0 &&
-                       (!epi.add || ((epi.ld_add * esz) % 16 == 0 && (reinterpret_cast<uintptr_t>(epi.add) & 15) == 0));
   const int sms = device_sm_count();
   const int k_blocks = (K + 63) / 64;
-  const LinearPlan plan = linear_plan(M, N, k_blocks, tma_out, epi.out_f32 != 0, sms);
+  const LinearPlan plan = linear_plan(M, N, k_blocks, epi.out_f32 != 0, sms);
   if (plan.pair) {
     GemmProblem q;
     q.A = x; q.lda = lda; q.W = w; q.ldw = ldw; q.M = M; q.epi = epi;

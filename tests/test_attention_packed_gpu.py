@@ -110,6 +110,14 @@ def test_rows_behind_the_last_sequence(sd3, D):
     check(sd3, [50, 130], 2, 2, D, True, extra=200)
 
 
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("lengths", [[1], [127], [129], [1, 1, 1], [0, 5, 0, 0, 130, 0], [300, 1, 64, 129, 2, 511], [1000]])
+@pytest.mark.parametrize("heads,kv_heads,D", [(4, 2, 64), (3, 3, 128), (4, 2, 128), (32, 8, 128)])
+def test_short_sequences_in_a_long_buffer(sd3, heads, kv_heads, D, lengths, causal):
+    # the variants are chosen by the rows there are, not by the sequences' (the host does not see the offsets)
+    check(sd3, lengths, heads, kv_heads, D, causal, seed=sum(lengths), extra=2048 * len(lengths))
+
+
 @pytest.mark.parametrize("spread,scale", [(8.0, None), (0.01, None), (1.0, 3.0), (3.0, 1e-6)])
 @pytest.mark.parametrize("D", [64, 128])
 def test_scores_of_all_sizes(sd3, spread, scale, D):
