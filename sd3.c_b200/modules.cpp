@@ -13,7 +13,8 @@
 //   Dit_block      modules.cpp:1508-1514
 //   DiT_block_cuda cuda/dit.cu:919-925
 //   linear :538, layer_norm :51, rms_norm :200, conv2d :1065,
-//   sinusoidal_embedding :920, positional_embedding :997, mha :901, mlp :1167
+//   layer_norm_backward :87, sinusoidal_embedding :920, positional_embedding :997, mha :901, mlp :1167
+// and of a transformer layer over packed prompts, which the reference does not have: linear_residual, mha_packed
 #include <ATen/cuda/CUDAContext.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
