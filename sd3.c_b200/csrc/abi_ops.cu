@@ -397,10 +397,20 @@ int sd3_layernorm_modulate(const float* x, int B, int T, int E, float eps, const
   return launch_ln_modulate(p, nullptr, E, eps, mod_stride, out_dtype == SD3_DTYPE_F32, S(stream));
 }
 
+namespace {
+// whether every pointer (null ones included) is a multiple of the size of what it points to
+bool aligned_to(uintptr_t size, std::initializer_list<const void*> pointers) {
+  for (const void* p : pointers)
+    if (reinterpret_cast<uintptr_t>(p) % size) return false;
+  return true;
+}
+}  // namespace
+
 int sd3_layer_norm(const void* x, long ldx, int dtype, const float* w, const float* b, float eps, void* y, float* mean,
                    float* rstd, long rows, int C, void* stream) {
   if (!dtype_ok(dtype) || rows < 0 || C <= 0 || C > (1 << 24) || (ldx < C && ldx != 0) || !(eps >= 0.f) ||
-      (rows > 0 && (!x || !y)) || (y == x && ldx != C)) {
+      (rows > 0 && (!x || !y)) || (y == x && ldx != C) || !aligned_to(dtype == SD3_DTYPE_F32 ? 4 : 2, {x, y}) ||
+      !aligned_to(4, {w, b, mean, rstd})) {
     set_last_error("sd3_layer_norm: invalid argument (dtype %d rows %ld C %d ldx %ld)", dtype, rows, C, ldx);
     return SD3_ERR_INVALID_ARG;
   }
@@ -416,7 +426,8 @@ int sd3_layer_norm_backward(const void* dy, long lddy, const void* x, long ldx, 
                             const float* mean, const float* rstd, void* dx, float* dw, float* db, long rows, int C,
                             void* scratch, long scratch_bytes, void* stream) {
   if (!dtype_ok(dtype) || rows < 0 || C <= 0 || C > (1 << 24) || (ldx < C && ldx != 0) || (lddy < C && lddy != 0) ||
-      (rows > 0 && (!dy || !x || !mean || !rstd || !dx)) || (dx == x && ldx != C) || (dx == dy && lddy != C)) {
+      (rows > 0 && (!dy || !x || !mean || !rstd || !dx)) || (dx == x && ldx != C) || (dx == dy && lddy != C) ||
+      !aligned_to(dtype == SD3_DTYPE_F32 ? 4 : 2, {dy, x, dx}) || !aligned_to(4, {w, mean, rstd, dw, db})) {
     set_last_error("sd3_layer_norm_backward: invalid argument (dtype %d rows %ld C %d ldx %ld lddy %ld)", dtype, rows, C,
                    ldx, lddy);
     return SD3_ERR_INVALID_ARG;

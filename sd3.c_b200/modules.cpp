@@ -242,6 +242,7 @@ Rows rows_of(const Tensor& t, const char* name) {
   TORCH_CHECK(t.is_cuda(), "custom_modules: '", name, "' must be a CUDA tensor (this build has no CPU path)");
   TORCH_CHECK(t.dim() >= 1 && t.size(-1) > 0, name, ": rows of at least one value expected");
   const int64_t C = t.size(-1), rows = t.numel() / C;
+  TORCH_CHECK(C < (1ll << 31), name, ": rows of fewer than 2^31 values expected");
   if (t.dim() == 2 && t.stride(1) == 1 && rows > 1 && (t.stride(0) >= C || t.stride(0) == 0)) return {t, rows, C, t.stride(0)};
   return {t.contiguous(), rows, C, C};
 }
@@ -524,7 +525,8 @@ Tensor mha_packed(const Tensor& q_in, const Tensor& k_in, const Tensor& v_in, co
   TORCH_CHECK(offsets.device() == q.device() && offsets.scalar_type() == torch::kInt32 && offsets.dim() == 1 &&
                   offsets.numel() >= 1 && offsets.is_contiguous(),
               "mha_packed: offsets must be contiguous int32 row numbers on q's device, one more than there are sequences");
-  TORCH_CHECK(q.size(0) < (1ll << 31) && q.size(1) <= 65536, "mha_packed: fewer than 2^31 rows and at most 65536 heads expected");
+  TORCH_CHECK(q.size(0) < (1ll << 31) && offsets.numel() <= (1ll << 31) && q.size(1) <= 65536,
+              "mha_packed: fewer than 2^31 rows, fewer than 2^31 sequences and at most 65536 heads expected");
   Tensor out = out_in ? *out_in : fresh(q.sizes(), torch::kBFloat16, q);
   if (out_in) {
     TORCH_CHECK(out.device() == q.device() && out.sizes() == q.sizes() && out.scalar_type() == torch::kBFloat16,

@@ -204,6 +204,8 @@ def _rows(t, what, like=None):
     if t.dim() != 2 or not t.is_cuda or t.shape[1] < 1:
         raise Sd3Error("%s: 2-D CUDA tensor expected" % what)
     rows, C = t.shape
+    if C >= 2 ** 31:
+        raise Sd3Error("%s: rows of fewer than 2^31 values expected" % what)
     if C > 1 and t.stride(1) != 1:
         raise Sd3Error("%s: rows must be contiguous" % what)
     if like is not None and (t.shape != like.shape or t.dtype != like.dtype or t.device != like.device):
@@ -227,6 +229,8 @@ def linear_residual(x_bf16, w_nk_bf16, bias=None, act=ACT_NONE, residual=None, o
     N, Kw, ldw = _rows(w_nk_bf16, "linear_residual: w")
     if x_bf16.dtype != torch.bfloat16 or w_nk_bf16.dtype != torch.bfloat16 or K != Kw or w_nk_bf16.device != x_bf16.device:
         raise Sd3Error("linear_residual: bfloat16 x (M, K) and w (N, K) on one device expected")
+    if max(M, N) >= 2 ** 31:
+        raise Sd3Error("linear_residual: sizes below 2^31 expected")
     if out is None:
         out = torch.empty((M, N), device=x_bf16.device,
                           dtype=out_dtype or (residual.dtype if residual is not None else torch.bfloat16))
@@ -353,6 +357,8 @@ def attention_packed(q, k, v, offsets, causal=False, scale=None, out=None):
     if (offsets.dtype != torch.int32 or offsets.dim() != 1 or offsets.numel() < 1 or not offsets.is_contiguous()
             or offsets.device != q.device):
         raise Sd3Error("attention_packed: offsets must be contiguous int32 row numbers on q's device")
+    if T >= 2 ** 31 or offsets.numel() > 2 ** 31 or H > 65536:
+        raise Sd3Error("attention_packed: fewer than 2^31 rows and sequences and at most 65536 heads expected")
     if out is None:
         out = torch.empty((T, H, D), device=q.device, dtype=q.dtype)
     if out.shape != q.shape or out.device != q.device:
