@@ -670,13 +670,15 @@ __global__ void __launch_bounds__(LNR_THREADS, 1) layer_norm_backward_ring_kerne
   float next_mean = first < a.rows ? a.mean[first] : 0.f, next_rstd = first < a.rows ? a.rstd[first] : 0.f;
   int buf = 0, s = 0, s_before = 0;
   uint32_t parity = 0;
+  bool late = false;
   for (long row = first; row < a.rows; row += step) {
     const float mean = next_mean, rstd = next_rstd;
     if (row + step < a.rows) {
       next_mean = a.mean[row + step];
       next_rstd = a.rstd[row + step];
     }
-    if (!mbar_wait(&bar[s], parity, wc, DEV_TIMEOUT_LN_ROW)) break;
+    // a thread that gave up goes on: its team's barriers count on it
+    if (!late) late = !mbar_wait(&bar[s], parity, wc, DEV_TIMEOUT_LN_ROW);
     const uint8_t* px = mine + s * 2 * ring.row_bytes;
     float2 sg2 = make_float2(0.f, 0.f), sgu2 = sg2;
     const float2 m2 = make_float2(-mean, -mean), r2 = make_float2(rstd, rstd);
@@ -717,7 +719,7 @@ __global__ void __launch_bounds__(LNR_THREADS, 1) layer_norm_backward_ring_kerne
       __syncwarp();
     }
     // everyone has finished the row before, which is read twice
-    if (t == 0 && row != first) request(row + (ring.depth - 1) * step, s_before);
+    if (t == 0 && row != first && !late) request(row + (ring.depth - 1) * step, s_before);
     s_before = s;
     if (++s == ring.depth) { s = 0; parity ^= 1; }
     const float mg = sg * inv_c, mgu = sgu * inv_c;
