@@ -37,6 +37,10 @@ constexpr int LR_SLOT = 2;  // K blocks of a stage: a hand-over takes longer tha
 constexpr int LR_MAX_STAGES = 12;
 constexpr int LR_THREADS = 64 + 32 * EPI_WARPS;
 constexpr int LR_SMEM = 227 * 1024;
+// A CTA of a cluster that waits for tensor memory keeps the others waiting, so no SM may hold clusters' CTAs that ask for more than
+// its 512 columns together (two streams could then wait for each other on two SMs).  The CTA-pair GEMM takes all of them with at
+// least 193 KiB of shared memory: a cluster's CTA takes more than the 33 KiB that this leaves.
+constexpr int LR_CLUSTER_SMEM = 36 * 1024;
 
 struct LinearArgs {
   int M, N, k_blocks, tiles_m, tiles_n;
@@ -427,7 +431,8 @@ int launch_linear_residual(const bf16* x, long lda, const bf16* w, long ldw, int
   if (rc) return rc;
   rc = encode_tmap_2d(&tmW, w, 2, (uint64_t)K, (uint64_t)N, (uint64_t)ldw * 2, 64, plan.bn);
   if (rc) return rc;
-  const int smem = 1024 + a.stages * a.stage_bytes + partial_bytes(a.split, a.a_rows, a.cols) + bars;
+  int smem = 1024 + a.stages * a.stage_bytes + partial_bytes(a.split, a.a_rows, a.cols) + bars;
+  if (a.split > 1 && smem < LR_CLUSTER_SMEM) smem = LR_CLUSTER_SMEM;
   if (plan.bn == 64)
     return epi.out_f32 ? launch_inst<64, true>(tmA, tmW, a, smem, stream) : launch_inst<64, false>(tmA, tmW, a, smem, stream);
   return epi.out_f32 ? launch_inst<128, true>(tmA, tmW, a, smem, stream) : launch_inst<128, false>(tmA, tmW, a, smem, stream);
