@@ -102,6 +102,23 @@ __device__ __forceinline__ float lanes_sum(float v) {
   return v;
 }
 
+// What the warps of a team have left in shared memory, a lane each, added up by every warp for itself.  (One after the other, 32
+// are 300 instructions of every warp: 6000 rows of 8191, bf16, 187 us against 100.)
+__device__ __forceinline__ void merge_sums(const float2* part, int warps, float& a, float& b) {
+  const int lane = threadIdx.x & 31;
+  const float2 p = lane < warps ? part[lane] : make_float2(0.f, 0.f);
+  a = lanes_sum<32>(p.x);
+  b = lanes_sum<32>(p.y);
+}
+// the same for means and squared deviations of n_of values each
+__device__ __forceinline__ void merge_deviations(const float2* part, const float* n_of, int warps, float inv_c, float& mean, float& m2) {
+  const int lane = threadIdx.x & 31;
+  const float2 p = lane < warps ? part[lane] : make_float2(0.f, 0.f);
+  const float n = lane < warps ? n_of[lane] : 0.f;
+  mean = lanes_sum<32>(p.x * n) * inv_c;
+  m2 = lanes_sum<32>(fmaf((p.x - mean) * (p.x - mean), n, p.y));
+}
+
 struct LnFwdArgs {
   const void* x;
   long ldx;
@@ -179,16 +196,7 @@ __global__ void __launch_bounds__(lnb_threads(VEC), 1) layer_norm_kernel(const _
       const int warp = threadIdx.x >> 5;
       if ((threadIdx.x & 31) == 0) part[buf][warp] = make_float2(mean, m2);
       team_barrier(1 + team, ts);
-      float s = 0.f;
-#pragma unroll 4
-      for (int k = 0; k < a.warps; ++k) s = fmaf(part[buf][warp0 + k].x, n_of[warp0 + k], s);
-      mean = s * inv_c;
-      m2 = 0.f;
-#pragma unroll 4
-      for (int k = 0; k < a.warps; ++k) {
-        const float2 p = part[buf][warp0 + k];
-        m2 += fmaf((p.x - mean) * (p.x - mean), n_of[warp0 + k], p.y);
-      }
+      merge_deviations(part[buf] + warp0, n_of + warp0, a.warps, inv_c, mean, m2);
       buf ^= 1;
     }
     const float rstd = rsqrtf(m2 * inv_c + a.eps);
@@ -329,16 +337,7 @@ __global__ void __launch_bounds__(lnb_threads(VEC), VEC <= 2 ? 1 : 2) layer_norm
     if (a.warps > 1) {
       if ((threadIdx.x & 31) == 0) part[buf][threadIdx.x >> 5] = make_float2(mean, m2);
       team_barrier(1 + team, ts);
-      float total = 0.f;
-#pragma unroll 4
-      for (int k = 0; k < a.warps; ++k) total = fmaf(part[buf][warp0 + k].x, n_of[warp0 + k], total);
-      mean = total * inv_c;
-      m2 = 0.f;
-#pragma unroll 4
-      for (int k = 0; k < a.warps; ++k) {
-        const float2 p = part[buf][warp0 + k];
-        m2 += fmaf((p.x - mean) * (p.x - mean), n_of[warp0 + k], p.y);
-      }
+      merge_deviations(part[buf] + warp0, n_of + warp0, a.warps, inv_c, mean, m2);
       buf ^= 1;
     }
     const float rstd = rsqrtf(m2 * inv_c + a.eps);
@@ -525,13 +524,7 @@ __global__ void __launch_bounds__(lnb_threads(VEC), 1) layer_norm_backward_kerne
     if (a.warps > 1) {
       if ((threadIdx.x & 31) == 0) part[buf][threadIdx.x >> 5] = make_float2(sg, sgu);
       team_barrier(1 + team, ts);
-      sg = 0.f;
-      sgu = 0.f;
-#pragma unroll 4
-      for (int k = 0; k < a.warps; ++k) {
-        sg += part[buf][warp0 + k].x;
-        sgu += part[buf][warp0 + k].y;
-      }
+      merge_sums(part[buf] + warp0, a.warps, sg, sgu);
       buf ^= 1;
     }
     const float mg = sg * inv_c, mgu = sgu * inv_c;
@@ -707,13 +700,7 @@ __global__ void __launch_bounds__(LNR_THREADS, 1) layer_norm_backward_ring_kerne
     if (a.warps > 1) {
       if ((threadIdx.x & 31) == 0) part[buf][threadIdx.x >> 5] = make_float2(sg, sgu);
       team_barrier(1 + team, ts);
-      sg = 0.f;
-      sgu = 0.f;
-#pragma unroll 4
-      for (int k = 0; k < a.warps; ++k) {
-        sg += part[buf][warp0 + k].x;
-        sgu += part[buf][warp0 + k].y;
-      }
+      merge_sums(part[buf] + warp0, a.warps, sg, sgu);
       buf ^= 1;
     } else {
       __syncwarp();
