@@ -372,6 +372,15 @@ __global__ void __launch_bounds__(lnb_threads(VEC), VEC <= 2 ? 1 : 2) layer_norm
   }
 }
 
+__device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
+
+template <typename T>
+__device__ __forceinline__ float2 pair_of(const Raw<T, 1>& p, const Raw<T, 1>& q) {
+  float a[1], b[1];
+  p.get(a);
+  q.get(b);
+  return make_float2(a[0], b[0]);
+}
 struct LnBwdArgs {
   const void* dy;
   long lddy;
@@ -474,13 +483,25 @@ __global__ void __launch_bounds__(lnb_threads(VEC), 1) layer_norm_backward_kerne
     nrstd = row < a.rows ? a.rstd[row] : 0.f;
   };
   constexpr bool PREFETCH = VEC > 1;  // single values: 32 registers that an SM full of warps does better without
+  constexpr bool PAIRS = VEC == 1 && NV > 1;  // single values: two pieces an instruction (bf16, 1516 rows of 4271: 38 -> 30 us)
+  // the weights of pieces i and i + 1; a place without a value takes the last one's, its dy is 0
+  auto weights = [&](int i) { return make_float2(sums[min(t + i * ts, nvec - 1)], sums[min(t + (i + 1) * ts, nvec - 1)]); };
   if (PREFETCH) request(first + team);
   stage_vector<VEC>(sums, a.w, 1.f, a.C);
   __syncthreads();
   int buf = 0;
   for (long base = first; base < a.rows; base += step) {
     const long row = base + team;
-    if (!PREFETCH) request(row);
+    if (!PREFETCH) {
+      request(row);
+      // fp32: the coming row as far as L2, a lane for each piece of its warp, which is a line (6000 rows of 8191: 187 -> 135 us; in bf16,
+      // where a piece is half a line, 20000 rows of 333 lose: 31 -> 34 us)
+      const int c = (t & ~31) + (threadIdx.x & 31) * ts;
+      if (sizeof(T) == 4 && LANES == 32 && (threadIdx.x & 31) < NV && c < nvec && row + step < a.rows) {
+        prefetch_l2(static_cast<const T*>(a.x) + (row + step) * a.ldx + c);
+        prefetch_l2(static_cast<const T*>(a.dy) + (row + step) * a.lddy + c);
+      }
+    }
     Raw<T, VEC> rx[NV], ry[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) { rx[i] = nx[i]; ry[i] = ny[i]; }
@@ -488,35 +509,51 @@ __global__ void __launch_bounds__(lnb_threads(VEC), 1) layer_norm_backward_kerne
     if (PREFETCH) request(row + step);
     // a place without a value has dy = 0 and adds nothing
     float sg = 0.f, sgu = 0.f;
+    if constexpr (PAIRS) {  // sg: of rstd g.  Where there is no value, mean * rstd might be no number; mean * 0 is 0
+      float2 g2 = make_float2(0.f, 0.f), gu2 = g2;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      if (t + i * ts >= nvec) continue;
-      float x[VEC], dy[VEC], w[VEC];
-      rx[i].get(x);
-      ry[i].get(dy);
-      staged<VEC>(sums, t + i * ts, nvec, w);
-      if constexpr (VEC == 1) {
-        const float u = (x[0] - mean) * rstd, g = dy[0] * w[0];
-        sg += g;
-        sgu = fmaf(g, u, sgu);
-        dw[i][0] = fmaf(dy[0], u, dw[i][0]);
-        db[i][0] += dy[0];
-      } else {
-        float2 g2 = make_float2(0.f, 0.f), gu2 = g2;
+      for (int i = 0; i < NV; i += 2) {
+        const float2 d = pair_of(ry[i], ry[i + 1]), e = __fadd2_rn(pair_of(rx[i], rx[i + 1]), make_float2(-mean, -mean));
+        const float2 dr = __fmul2_rn(d, make_float2(rstd, rstd)), gr = __fmul2_rn(dr, weights(i));
+        g2 = __fadd2_rn(g2, gr);
+        gu2 = __ffma2_rn(gr, e, gu2);
+        const float2 p = __ffma2_rn(dr, e, make_float2(dw[i][0], dw[i + 1][0])), q = __fadd2_rn(make_float2(db[i][0], db[i + 1][0]), d);
+        dw[i][0] = p.x; dw[i + 1][0] = p.y;
+        db[i][0] = q.x; db[i + 1][0] = q.y;
+      }
+      sg = g2.x + g2.y;
+      sgu = gu2.x + gu2.y;
+    } else {
 #pragma unroll
-        for (int j = 0; j < VEC; j += 2) {
-          const float2 d = make_float2(dy[j], dy[j + 1]);
-          const float2 u = __fmul2_rn(__fadd2_rn(make_float2(x[j], x[j + 1]), make_float2(-mean, -mean)), make_float2(rstd, rstd));
-          const float2 g = __fmul2_rn(d, make_float2(w[j], w[j + 1]));
-          g2 = __fadd2_rn(g2, g);
-          gu2 = __ffma2_rn(g, u, gu2);
-          const float2 p = __ffma2_rn(d, u, make_float2(dw[i][j], dw[i][j + 1]));
-          const float2 q = __fadd2_rn(make_float2(db[i][j], db[i][j + 1]), d);
-          dw[i][j] = p.x; dw[i][j + 1] = p.y;
-          db[i][j] = q.x; db[i][j + 1] = q.y;
+      for (int i = 0; i < NV; ++i) {
+        if (t + i * ts >= nvec) continue;
+        float x[VEC], dy[VEC], w[VEC];
+        rx[i].get(x);
+        ry[i].get(dy);
+        staged<VEC>(sums, t + i * ts, nvec, w);
+        if constexpr (VEC == 1) {
+          const float u = (x[0] - mean) * rstd, g = dy[0] * w[0];
+          sg += g;
+          sgu = fmaf(g, u, sgu);
+          dw[i][0] = fmaf(dy[0], u, dw[i][0]);
+          db[i][0] += dy[0];
+        } else {
+          float2 g2 = make_float2(0.f, 0.f), gu2 = g2;
+#pragma unroll
+          for (int j = 0; j < VEC; j += 2) {
+            const float2 d = make_float2(dy[j], dy[j + 1]);
+            const float2 u = __fmul2_rn(__fadd2_rn(make_float2(x[j], x[j + 1]), make_float2(-mean, -mean)), make_float2(rstd, rstd));
+            const float2 g = __fmul2_rn(d, make_float2(w[j], w[j + 1]));
+            g2 = __fadd2_rn(g2, g);
+            gu2 = __ffma2_rn(g, u, gu2);
+            const float2 p = __ffma2_rn(d, u, make_float2(dw[i][j], dw[i][j + 1]));
+            const float2 q = __fadd2_rn(make_float2(db[i][j], db[i][j + 1]), d);
+            dw[i][j] = p.x; dw[i][j + 1] = p.y;
+            db[i][j] = q.x; db[i][j + 1] = q.y;
+          }
+          sg += g2.x + g2.y;
+          sgu += gu2.x + gu2.y;
         }
-        sg += g2.x + g2.y;
-        sgu += gu2.x + gu2.y;
       }
     }
     sg = lanes_sum<LANES>(sg);
@@ -530,27 +567,39 @@ __global__ void __launch_bounds__(lnb_threads(VEC), 1) layer_norm_backward_kerne
     const float mg = sg * inv_c, mgu = sgu * inv_c;
     if (row < a.rows) {
       T* out = static_cast<T*>(a.dx) + row * a.C;
+      if constexpr (PAIRS) {
 #pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        const int c = t + i * ts;
-        if (c < nvec) {
-          float x[VEC], dy[VEC], w[VEC], o[VEC];
-          rx[i].get(x);
-          ry[i].get(dy);
-          staged<VEC>(sums, c, nvec, w);
-          if constexpr (VEC == 1) {
-            o[0] = rstd * (fmaf(dy[0], w[0], -mg) - (x[0] - mean) * rstd * mgu);
-          } else {
+        for (int i = 0; i < NV; i += 2) {
+          const float2 e = __fadd2_rn(pair_of(rx[i], rx[i + 1]), make_float2(-mean, -mean)), u = __fmul2_rn(e, make_float2(rstd, rstd));
+          const float2 dr = __fmul2_rn(pair_of(ry[i], ry[i + 1]), make_float2(rstd, rstd));
+          const float2 d = __ffma2_rn(u, make_float2(-mgu * rstd, -mgu * rstd), __ffma2_rn(dr, weights(i), make_float2(-mg, -mg)));
+          const float lo[1] = {d.x}, hi[1] = {d.y};
+          if (t + i * ts < nvec) Raw<T, 1>::store(out + t + i * ts, lo);
+          if (t + (i + 1) * ts < nvec) Raw<T, 1>::store(out + t + (i + 1) * ts, hi);
+        }
+      } else {
 #pragma unroll
-            for (int j = 0; j < VEC; j += 2) {
-              const float2 u = __fmul2_rn(__fadd2_rn(make_float2(x[j], x[j + 1]), make_float2(-mean, -mean)), make_float2(rstd, rstd));
-              const float2 g = __ffma2_rn(make_float2(dy[j], dy[j + 1]), make_float2(w[j], w[j + 1]), make_float2(-mg, -mg));
-              const float2 d = __fmul2_rn(__ffma2_rn(u, make_float2(-mgu, -mgu), g), make_float2(rstd, rstd));
-              o[j] = d.x;
-              o[j + 1] = d.y;
+        for (int i = 0; i < NV; ++i) {
+          const int c = t + i * ts;
+          if (c < nvec) {
+            float x[VEC], dy[VEC], w[VEC], o[VEC];
+            rx[i].get(x);
+            ry[i].get(dy);
+            staged<VEC>(sums, c, nvec, w);
+            if constexpr (VEC == 1) {
+              o[0] = rstd * (fmaf(dy[0], w[0], -mg) - (x[0] - mean) * rstd * mgu);
+            } else {
+#pragma unroll
+              for (int j = 0; j < VEC; j += 2) {
+                const float2 u = __fmul2_rn(__fadd2_rn(make_float2(x[j], x[j + 1]), make_float2(-mean, -mean)), make_float2(rstd, rstd));
+                const float2 g = __ffma2_rn(make_float2(dy[j], dy[j + 1]), make_float2(w[j], w[j + 1]), make_float2(-mg, -mg));
+                const float2 d = __fmul2_rn(__ffma2_rn(u, make_float2(-mgu, -mgu), g), make_float2(rstd, rstd));
+                o[j] = d.x;
+                o[j + 1] = d.y;
+              }
             }
+            Raw<T, VEC>::store(out + c * VEC, o);
           }
-          Raw<T, VEC>::store(out + c * VEC, o);
         }
       }
     }
@@ -597,40 +646,70 @@ __global__ void __launch_bounds__(1024) layer_norm_columns_kernel(const float* p
 }
 
 // ----------------------------------------------------------------------------
-// Backward of aligned fp32 rows of 512 bytes and more: the same teams, with rows that come through shared memory.  Each team has a ring
-// of its own, `depth` rows of x and dy that its first thread requests ahead by bulk copies; behind the team's barrier of a row
-// everyone has finished the row before, whose place is then requested anew.  With neither the coming row nor the weight in
-// registers, 1024 threads fit an SM.
+// Backward of fp32 rows of 512 bytes and more that are aligned for 16 or 8 bytes: the same teams, with rows that come through shared
+// memory.  Each team has a ring of its own, `depth` rows of x and dy that its first thread requests ahead by bulk copies; behind the
+// team's barrier of a row everyone has finished the row before, whose place is then requested anew.  With neither the coming row
+// nor the weight in registers, 1024 threads fit an SM.
+// A row that is aligned for 8 bytes (VEC 2) comes as the 16-byte pieces that it touches.  A piece that would read in front of the first
+// row or behind the last one is left out: the thread that owns its columns loads them.  (1516 rows of 4270: 44 us with the rows in
+// registers, 29 so.  Rows aligned for 4 bytes, and bf16 ones, lose: 1357 rows of 777 13 against 16 us, 1516 of 4270 in bf16 23 against 28.)
 // ----------------------------------------------------------------------------
 constexpr int LNR_THREADS = 1024;
 constexpr int LNR_MAX_WARPS = LNR_THREADS / 32;
 constexpr int LNR_SMEM = 200 * 1024;
 
 struct LnRing {
-  int depth, row_bytes;
+  int depth, slot_bytes;  // of one row of x or dy
   int* status;
 };
 
-__device__ __forceinline__ void load16(const uint8_t* p, float (&f)[4]) {
+// Rows of x or dy as bulk copies take them.
+struct RowPieces {
+  const uint8_t* base;
+  long ld_bytes, rows;
+  int row_bytes;
+  __device__ __forceinline__ RowPieces(const void* p, long ld, long rows_, int C)
+      : base(static_cast<const uint8_t*>(p)), ld_bytes(ld * 4), rows(rows_), row_bytes(C * 4) {}
+  __device__ __forceinline__ const uint8_t* at(long row) const { return base + row * ld_bytes; }
+  // where the row begins in its first piece
+  __device__ __forceinline__ int shift(long row) const {
+    return (static_cast<uint32_t>(reinterpret_cast<uintptr_t>(base)) + static_cast<uint32_t>(row) * static_cast<uint32_t>(ld_bytes)) & 15;
+  }
+  // bytes that are left out of the first row's beginning, and first byte of the last row that is
+  __device__ __forceinline__ int head() const { return (16 - shift(0)) & 15; }
+  __device__ __forceinline__ int tail() const { return row_bytes - ((shift(rows - 1) + row_bytes) & 15); }
+  // what is copied: from the row's byte `from` (below 0: before its beginning) on, `bytes`
+  __device__ __forceinline__ void piece(long row, int& from, int& bytes) const {
+    const int sh = shift(row);
+    from = row == 0 ? head() : -sh;
+    const int end = row == rows - 1 ? tail() : ((sh + row_bytes + 15) & ~15) - sh;
+    bytes = end - from;
+  }
+};
+
+__device__ __forceinline__ void load_piece(const uint8_t* p, float (&f)[4]) {
   const float4 v = *reinterpret_cast<const float4*>(p);
   f[0] = v.x; f[1] = v.y; f[2] = v.z; f[3] = v.w;
 }
+__device__ __forceinline__ void load_piece(const uint8_t* p, float (&f)[2]) {
+  const float2 v = *reinterpret_cast<const float2*>(p);
+  f[0] = v.x; f[1] = v.y;
+}
 
-template <int NV>
+template <int VEC, int NV>
 __global__ void __launch_bounds__(LNR_THREADS, 1) layer_norm_backward_ring_kernel(const __grid_constant__ LnBwdArgs a,
                                                                                   const __grid_constant__ LnRing ring) {
-  typedef float T;
-  constexpr int VEC = 4;
+  constexpr bool PIECES = VEC == 2;  // else whole rows
   extern __shared__ __align__(16) uint8_t ring_smem[];  // w, then the rings (x, dy of a row next to each other); at the end room for combine_groups
   float* w_smem = reinterpret_cast<float*>(ring_smem);
-  uint8_t* rows_smem = ring_smem + 4 * a.C;
+  uint8_t* rows_smem = ring_smem + ((4 * a.C + 15) & ~15);
   __shared__ float2 part[2][LNR_MAX_WARPS];
   __shared__ uint64_t full[LNR_MAX_WARPS * 8];
   __shared__ int s_abort;
   const int ts = 32 * a.warps, team = threadIdx.x / ts, t = threadIdx.x % ts, warp0 = team * a.warps;
   const int nvec = a.C / VEC;
   uint64_t* bar = full + team * 8;
-  uint8_t* mine = rows_smem + static_cast<long>(team) * ring.depth * 2 * ring.row_bytes;
+  uint8_t* mine = rows_smem + static_cast<long>(team) * ring.depth * 2 * ring.slot_bytes;
   if (t == 0) {
     for (int s = 0; s < ring.depth; ++s) mbar_init(&bar[s], 1);
     if (threadIdx.x == 0) s_abort = 0;
@@ -642,16 +721,28 @@ __global__ void __launch_bounds__(LNR_THREADS, 1) layer_norm_backward_ring_kerne
   const WaitCtx wc{&s_abort, ring.status};
   const long step = static_cast<long>(gridDim.x) * a.teams;
   const long first = static_cast<long>(blockIdx.x) * a.teams + team;
+  const RowPieces xs(a.x, a.ldx, a.rows, a.C), ys(a.dy, a.lddy, a.rows, a.C);
   auto request = [&](long row, int s) {
     if (row < a.rows) {
-      uint8_t* to = mine + s * 2 * ring.row_bytes;
-      mbar_expect_tx(&bar[s], 2 * ring.row_bytes);
-      bulk_load(to, static_cast<const T*>(a.x) + row * a.ldx, ring.row_bytes, &bar[s]);
-      bulk_load(to + ring.row_bytes, static_cast<const T*>(a.dy) + row * a.lddy, ring.row_bytes, &bar[s]);
+      uint8_t* to = mine + s * 2 * ring.slot_bytes;
+      int fx = 0, nx = xs.row_bytes, fy = 0, ny = xs.row_bytes;
+      if constexpr (PIECES) {
+        xs.piece(row, fx, nx);
+        ys.piece(row, fy, ny);
+      }
+      mbar_expect_tx(&bar[s], nx + ny);
+      bulk_load(to + (PIECES ? xs.shift(row) + fx : 0), xs.at(row) + fx, nx, &bar[s]);
+      bulk_load(to + ring.slot_bytes + (PIECES ? ys.shift(row) + fy : 0), ys.at(row) + fy, ny, &bar[s]);
     }
   };
   if (t == 0)
     for (int s = 0; s < ring.depth; ++s) request(first + s * step, s);
+  // the end of the last row, which no piece brings (8 bytes or none): on its way from the start
+  __shared__ float2 last_x, last_y;
+  if (PIECES && first < a.rows && (a.rows - 1 - first) % step == 0 && t == (nvec - 1) % ts) {
+    last_x = *reinterpret_cast<const float2*>(xs.at(a.rows - 1) + xs.row_bytes - 8);
+    last_y = *reinterpret_cast<const float2*>(ys.at(a.rows - 1) + ys.row_bytes - 8);
+  }
   stage_vector<VEC>(w_smem, a.w, 1.f, a.C);
   __syncthreads();
   float dw[NV][VEC], db[NV][VEC];
@@ -672,7 +763,28 @@ __global__ void __launch_bounds__(LNR_THREADS, 1) layer_norm_backward_ring_kerne
     }
     // a thread that gave up goes on: its team's barriers count on it
     if (!late) late = !mbar_wait(&bar[s], parity, wc, DEV_TIMEOUT_LN_ROW);
-    const uint8_t* px = mine + s * 2 * ring.row_bytes;
+    uint8_t* px = mine + s * 2 * ring.slot_bytes;
+    uint8_t* py = px + ring.slot_bytes;
+    if constexpr (PIECES) {
+      px += xs.shift(row);
+      py += ys.shift(row);
+      // what the pieces left out, by the thread whose columns they are
+      if (row == 0 && t == 0) {
+        if (xs.head()) *reinterpret_cast<float2*>(px) = *reinterpret_cast<const float2*>(xs.at(0));
+        if (ys.head()) *reinterpret_cast<float2*>(py) = *reinterpret_cast<const float2*>(ys.at(0));
+        fence_proxy_async();  // before the place is copied to again
+      }
+      if (row == a.rows - 1 && t == (nvec - 1) % ts) {
+        *reinterpret_cast<float2*>(px + xs.row_bytes - 8) = last_x;
+        *reinterpret_cast<float2*>(py + ys.row_bytes - 8) = last_y;
+      }
+    }
+    // piece c of the row: x, dy, w
+    auto values = [&](int c, float (&x)[VEC], float (&dy)[VEC], float (&w)[VEC]) {
+      load_piece(px + c * (VEC * 4), x);
+      load_piece(py + c * (VEC * 4), dy);
+      staged<VEC>(w_smem, c, nvec, w);
+    };
     float2 sg2 = make_float2(0.f, 0.f), sgu2 = sg2;
     const float2 m2 = make_float2(-mean, -mean), r2 = make_float2(rstd, rstd);
 #pragma unroll
@@ -680,9 +792,7 @@ __global__ void __launch_bounds__(LNR_THREADS, 1) layer_norm_backward_ring_kerne
       const int c = t + i * ts;
       if (c < nvec) {
         float x[VEC], dy[VEC], w[VEC];
-        load16(px + c * 16, x);
-        load16(px + ring.row_bytes + c * 16, dy);
-        staged<VEC>(w_smem, c, nvec, w);
+        values(c, x, dy, w);
 #pragma unroll
         for (int j = 0; j < VEC; j += 2) {
           const float2 d = make_float2(dy[j], dy[j + 1]);
@@ -710,15 +820,13 @@ __global__ void __launch_bounds__(LNR_THREADS, 1) layer_norm_backward_ring_kerne
     s_before = s;
     if (++s == ring.depth) { s = 0; parity ^= 1; }
     const float mg = sg * inv_c, mgu = sgu * inv_c;
-    T* out = static_cast<T*>(a.dx) + row * a.C;
+    float* out = static_cast<float*>(a.dx) + row * a.C;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c = t + i * ts;
       if (c < nvec) {
         float x[VEC], dy[VEC], w[VEC], o[VEC];
-        load16(px + c * 16, x);
-        load16(px + ring.row_bytes + c * 16, dy);
-        staged<VEC>(w_smem, c, nvec, w);
+        values(c, x, dy, w);
 #pragma unroll
         for (int j = 0; j < VEC; j += 2) {
           const float2 u = __fmul2_rn(__fadd2_rn(make_float2(x[j], x[j + 1]), m2), r2);
@@ -727,7 +835,7 @@ __global__ void __launch_bounds__(LNR_THREADS, 1) layer_norm_backward_ring_kerne
           o[j] = d.x;
           o[j + 1] = d.y;
         }
-        Raw<T, VEC>::store(out + c * VEC, o);
+        Raw<float, VEC>::store(out + c * VEC, o);
       }
     }
   }
@@ -943,10 +1051,11 @@ struct LaunchBackward {
   }
 };
 
-// The ring kernel: f.template run<NV>() of the shape
+// The ring kernel: f.template run<VEC, NV>() of the shape
 template <typename F>
 int with_ring(const LnShape& s, const F& f) {
-  return s.nv == 1 ? f.template run<1>() : s.nv == 2 ? f.template run<2>() : s.nv == 3 ? f.template run<3>() : f.template run<4>();
+  if (s.vec == 2) return s.nv == 1 ? f.template run<2, 1>() : s.nv == 2 ? f.template run<2, 2>() : f.template run<2, 4>();
+  return s.nv == 1 ? f.template run<4, 1>() : s.nv == 2 ? f.template run<4, 2>() : s.nv == 3 ? f.template run<4, 3>() : f.template run<4, 4>();
 }
 
 struct LaunchBackwardRing {
@@ -955,25 +1064,25 @@ struct LaunchBackwardRing {
   int grid, threads;
   size_t smem;
   cudaStream_t stream;
-  template <int NV>
+  template <int VEC, int NV>
   int run() const {
-    int rc = allow_smem(layer_norm_backward_ring_kernel<NV>, smem, LNR_SMEM);
+    int rc = allow_smem(layer_norm_backward_ring_kernel<VEC, NV>, smem, LNR_SMEM);
     if (rc) return rc;
-    launch_dependent(layer_norm_backward_ring_kernel<NV>, grid, threads, smem, stream, a, ring);
+    launch_dependent(layer_norm_backward_ring_kernel<VEC, NV>, grid, threads, smem, stream, a, ring);
     return after_launch("layer_norm_backward_ring_kernel");
   }
 };
 
 // The ring of a team: at least two rows, eight at most, no more than the team goes through and shared memory holds.
-LnRing ring_for(const LnShape& s, int C, int row_bytes, long rows, int grid, int* status) {
+LnRing ring_for(const LnShape& s, int vectors, int slot_bytes, long rows, int grid, int* status) {
   LnRing r;
   const long per_team = (rows + static_cast<long>(grid) * s.teams - 1) / (static_cast<long>(grid) * s.teams);
-  long depth = (LNR_SMEM - 4L * C) / (2L * s.teams * row_bytes);
+  long depth = (LNR_SMEM - vectors) / (2L * s.teams * slot_bytes);
   if (depth > 8) depth = 8;
   if (depth > per_team) depth = per_team;
   if (depth < 2) depth = 2;
   r.depth = static_cast<int>(depth);
-  r.row_bytes = row_bytes;
+  r.slot_bytes = slot_bytes;
   r.status = status;
   return r;
 }
@@ -1039,12 +1148,13 @@ int launch_layer_norm_backward(const void* dy, long lddy, const void* x, long ld
       rc = after_launch("layer_norm_backward_wide_kernel");
       if (rc) return rc;
     } else {
-      const int row_bytes = C * (f32 ? 4 : 2);
-      const bool ring = f32 && s.vec == 4 && row_bytes >= 512;
+      const int row_bytes = C * esz;
+      const bool ring = f32 && s.vec >= 2 && row_bytes >= 512 && (s.vec == 4 || (ldx != 0 && lddy != 0));
+      const int slot_bytes = s.vec == 2 ? row_bytes / 16 * 16 + 32 : row_bytes, vectors = (4 * C + 15) / 16 * 16;
       if (ring) {  // as many teams as threads and shared memory (two rows each) leave room for
         s.teams = LNR_MAX_WARPS / s.warps;
         if (s.warps > 1 && s.teams > LNB_MAX_TEAMS) s.teams = LNB_MAX_TEAMS;
-        const long most = (LNR_SMEM - 4L * C) / (4L * row_bytes);
+        const long most = (LNR_SMEM - vectors) / (4L * slot_bytes);
         if (s.teams > most) s.teams = static_cast<int>(most);
       }
       // Few rows: a lone CTA with a row a team, which needs no second kernel (one row of 64: 3.0 -> 2.1 us, and a launch less)
@@ -1055,10 +1165,10 @@ int launch_layer_norm_backward(const void* dy, long lddy, const void* x, long ld
       a.teams = s.teams;
       int rc;
       if (ring) {
-        const LnRing r = ring_for(s, C, row_bytes, rows, parts, dev_status);
-        size_t smem = static_cast<size_t>(s.teams) * r.depth * 2 * row_bytes;
+        const LnRing r = ring_for(s, vectors, slot_bytes, rows, parts, dev_status);
+        size_t smem = static_cast<size_t>(s.teams) * r.depth * 2 * slot_bytes;
         if (smem < combine_bytes(s.teams, C)) smem = combine_bytes(s.teams, C);
-        rc = with_ring(s, LaunchBackwardRing{a, r, parts, cta_threads(s), smem + sizeof(float) * C, stream});
+        rc = with_ring(s, LaunchBackwardRing{a, r, parts, cta_threads(s), smem + vectors, stream});
       } else {
         rc = with_shape(s, f32 != 0, LaunchBackward{a, parts, cta_threads(s), stream});
       }

@@ -90,6 +90,41 @@ def test_addresses_that_are_not_aligned(sd3, dtype):
     check(sd3, shifted, w, b, dy)
 
 
+def carved(t, at, pad):
+    """t's rows, `pad` elements apart, `at` elements into a buffer of NaN"""
+    rows, C = t.shape
+    flat = torch.full((at + rows * (C + pad) + 64,), float("nan"), device="cuda", dtype=t.dtype)
+    view = flat[at:at + rows * (C + pad)].view(rows, C + pad)[:, :C]
+    view.copy_(t)
+    return view
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,C", [(1, 777), (2, 777), (3, 300), (40, 257), (149, 1001), (700, 333), (3, 8191), (400, 2047), (60, 4098)])
+@pytest.mark.parametrize("at_x,at_dy,pad", [(0, 0, 0), (1, 3, 0), (6, 0, 1), (7, 2, 2), (5, 5, 9)])
+def test_rows_between_other_values(sd3, rows, C, at_x, at_dy, pad, dtype):
+    x, w, b, dy = make(rows, C, dtype, seed=rows + C + at_x)
+    check(sd3, carved(x, at_x, pad), w, b, carved(dy, at_dy, pad))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("onto", ["x", "dy"])
+@pytest.mark.parametrize("rows,C", [(1, 777), (700, 777), (30, 8191), (900, 1024)])
+def test_gradient_onto_its_operands(sd3, rows, C, onto, dtype):
+    x, w, b, dy = (t.contiguous() for t in make(rows, C, dtype, seed=rows))
+    _, mean, rstd = sd3.layer_norm(x, w, b, EPS)
+    want = sd3.layer_norm_backward(dy, x, w, mean, rstd)
+    dw, db = torch.empty_like(w), torch.empty_like(w)
+    nbytes = sd3.lib().sd3_layer_norm_backward_scratch_bytes(rows, C)
+    scratch = torch.empty(nbytes, device="cuda", dtype=torch.uint8)
+    dx = x if onto == "x" else dy
+    sd3.check(sd3.lib().sd3_layer_norm_backward(*(sd3.ptr(dy), C, sd3.ptr(x), C, sd3.dtype_tag(x)), sd3.ptr(w), sd3.ptr(mean),
+                                                sd3.ptr(rstd), sd3.ptr(dx), sd3.ptr(dw), sd3.ptr(db), rows, C, sd3.ptr(scratch),
+                                                nbytes, sd3.stream_ptr()), "sd3_layer_norm_backward")
+    for p, q in zip((dx, dw, db), want):
+        assert torch.equal(p, q)
+
+
 def test_no_rows(sd3):
     x = torch.empty(0, 96, device="cuda")
     y, mean, rstd = sd3.layer_norm(x, None, None)
@@ -108,6 +143,19 @@ def test_a_row_of_equal_values_and_values_far_from_zero(sd3):
     y = sd3.layer_norm(x, None, None, EPS)[0]
     ref = torch.nn.functional.layer_norm(x.double(), (1536,), eps=EPS)
     assert (y.double() - ref).abs().max() <= 0.01
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("C", [200, 333, 777, 1024, 1538])
+def test_rows_of_one_huge_value(sd3, C, dtype):
+    # mean * rstd is no fp32 number, every deviation is 0: u = 0, dx = rstd (g - mean(g)) with rstd = eps^-1/2
+    x = torch.full((5, C), 2.0 ** 124, device="cuda", dtype=dtype)
+    dy = torch.ones(5, C, device="cuda", dtype=dtype)
+    mean = torch.full((5,), 2.0 ** 124, device="cuda")
+    rstd = torch.full((5,), EPS ** -0.5, device="cuda")
+    w = torch.ones(C, device="cuda")
+    dx, dw, db = sd3.layer_norm_backward(dy, x, w, mean, rstd)
+    assert dx.float().abs().max() <= C * 2.0 ** -24 * EPS ** -0.5 and (dw == 0).all() and (db == 5).all()
 
 
 def test_infinities_stay_in_their_row(sd3):
