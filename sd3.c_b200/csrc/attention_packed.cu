@@ -14,6 +14,13 @@
 // between replays of a captured graph.  The grid has room for every way in which the rows can be cut into `count` sequences.
 // Tiles run in the order of the keys that they see, the most first; the short ones fill the end.
 //
+// Bound by the tensor cores and the MUFU unit (128 exponentials a row take as long as the products of a tile), under the power cap where
+// sequences are long; by the chain of loads, scores, softmax and products of one tile where they are short.  us:
+//   8192 tokens, causal, 32 heads over 8 of 128   494-515 (1.07-1.11 PFLOP/s of 1.39 that plain products sustain)
+//   8192 tokens, all keys, the same               908-970 (1.13-1.21)
+//   8192 tokens, causal, 32 heads over 8 of 64    368 (0.75)
+//   32 x 200 tokens, 16 heads of 64               26;  one sequence of 128: 5.7
+//
 // Only key tiles that hold the diagonal or the end of the sequence are masked.  Keys behind the end are the next sequence's: their
 // scores become -inf, and their rows of V zeros, because 0 * inf is not 0.
 #include <cuda.h>

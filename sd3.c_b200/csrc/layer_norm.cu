@@ -5,13 +5,17 @@
 //
 // Both are bound by memory: the forward reads x and writes y, the backward reads x and dy and writes dx, once each.
 // A row belongs to a team of threads and lives in its registers between the load and the store: part of a warp for
-// narrow rows, one to sixteen warps (at most 16 values a thread) for wide ones.  A team goes through many rows, and a
-// thread always has the same columns: weight and bias stay in its registers, and so do its columns' sums for dw and
-// db, which leave the SM once (one partial row per CTA, added up by a second kernel in a fixed order: no atomics, the
-// same bits every time).  The next row is requested before the current one is reduced.  A row takes one barrier:
-// the forward's warps form their own mean and squared deviations and merge both,
+// narrow rows, one to 32 warps (at most 24 values a thread) for wide ones.  A team goes through many rows, and a
+// thread always has the same columns: their sums for dw and db stay in its registers and leave the SM once (one partial row per
+// CTA, added up by a second kernel in a fixed order: no atomics, the same bits every time).  The next row is requested before the
+// current one is reduced.  A row takes one barrier: the forward's warps form their own mean and squared deviations and merge both,
 //   M2 = sum_w M2_w + sum_w n_w (mean_w - mean)^2,
 // the backward's two sums are known in one pass.
+// Measured, us, forward / gradient, and the share of the copy rate:
+//   32768 x 1536  fp32 73 / 107 (0.84, 0.87)   bf16 35 / 62 (0.87, 0.75: unpacking and four sums a value fill the issue slots)
+//   8192 x 4096   fp32 48 / 81 (0.85, 0.76)    bf16 30 / 44 (0.69, 0.70)
+//   1357 x 776    fp32 4.9 / 9.7               bf16 4.6 / 8.7   (two rows a team: latency; the gradient's second kernel is 2 us)
+//   1357 x 777    fp32 7.0 / 11.6              bf16 7.0 / 12.0  (rows aligned for one value: four to eight times the loads and stores)
 #include "kernels.h"
 #include "ptx.cuh"
 
@@ -221,7 +225,7 @@ __global__ void __launch_bounds__(lnb_threads(VEC), 1) layer_norm_kernel(const _
 }
 
 // Several rows a team: weight and bias in shared memory, so that two CTAs of 512 threads fit an SM (in registers, 32 more a thread,
-// one does: 32768 x 1536, bf16, 52 us against 46; fp32 105 against 79).  VEC 8: the lower halves of all pieces, then the upper ones, so that the 16 bytes that
+// one does: 32768 x 1536, bf16, 46 us against 35; fp32 98 against 72).  VEC 8: the lower halves of all pieces, then the upper ones, so that the 16 bytes that
 // neighbouring threads read are neighbours.
 template <int VEC>
 __device__ __forceinline__ int vector_at(int c, int nvec) {  // of column c
@@ -652,7 +656,7 @@ __global__ void __launch_bounds__(1024) layer_norm_columns_kernel(const float* p
 // nor the weight in registers, 1024 threads fit an SM.
 // A row that is aligned for 8 bytes (VEC 2) comes as the 16-byte pieces that it touches.  A piece that would read in front of the first
 // row or behind the last one is left out: the thread that owns its columns loads them.  (1516 rows of 4270: 44 us with the rows in
-// registers, 29 so.  Rows aligned for 4 bytes, and bf16 ones, lose: 1357 rows of 777 13 against 16 us, 1516 of 4270 in bf16 23 against 28.)
+// registers, 28 so.  Rows aligned for 4 bytes, and bf16 ones, lose: 1357 rows of 777 13 against 16 us, 1516 of 4270 in bf16 23 against 28.)
 // ----------------------------------------------------------------------------
 constexpr int LNR_THREADS = 1024;
 constexpr int LNR_MAX_WARPS = LNR_THREADS / 32;
@@ -1102,6 +1106,8 @@ int launch_layer_norm(const void* x, long ldx, int f32, const float* w, const fl
   const int sms = device_sm_count();
   const int esz = f32 ? 4 : 2, px = piece_of(x, ldx, C, esz), py = piece_of(y, C, C, esz), vec = px < py ? px : py;
   LnShape s = ln_shape(C, vec, f32 ? 8 : 16);
+  // More than two rows a team: the kernel that stages w and b.  us, staged / in registers, 1536 columns, bf16: 148 rows 5.6 / 2.2,
+  // 592 4.6 / 3.7, 2368 5.4 / 7.0, 32768 35 / 46; fp32 3.5 / 2.0, 3.5 / 3.1, 7.2 / 7.2, 72 / 98; 64 columns, fp32: 4736 rows 2.3 / 1.7
   const bool many = rows > 2L * sms * s.teams;
   if (many) s = ln_shape(C, vec, f32 ? 16 : 24);
   if (!row_fits(C, s)) {

@@ -10,6 +10,9 @@
 // bits every time), applies bias, activation and residual and writes its columns, neighbouring threads neighbouring
 // columns: coalesced whatever the row pitch, element by element where rows are not aligned.  fp32 outputs are summed in
 // several accumulators, added in registers: the tensor cores cut a sum off at every step (gemm2_tcgen05.cu).
+//
+// Bound by latency: launch, the first bytes of the weights, the hand-over of the partial sums and the epilogue, about 5 us around the
+// reading.  One row, K 1536, N 6144: 7.2 us (2.9 at the copy rate); 333 x 1001, K 1544, fp32 with residual: 9.8 (1.0).
 #include <cuda.h>
 
 #include <mutex>
