@@ -240,3 +240,22 @@ def test_captured_and_on_another_stream(sd3):
     y, mean, rstd = sd3.layer_norm(x, w, b, EPS)
     for p, q in zip((gy, gm, gr) + got, (y, mean, rstd) + sd3.layer_norm_backward(dy, x, w, mean, rstd)):
         assert torch.equal(p, q)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,C", [(7, 64), (700, 777), (3, 8191), (900, 1024), (5, 20000)])
+def test_forward_onto_its_operand(sd3, rows, C, dtype):
+    x, w, b, _ = (t.contiguous() for t in make(rows, C, dtype, seed=rows))
+    y, mean, rstd = sd3.layer_norm(x, w, b, EPS)
+    m, r = torch.empty_like(mean), torch.empty_like(rstd)
+    sd3.check(sd3.lib().sd3_layer_norm(sd3.ptr(x), C, sd3.dtype_tag(x), sd3.ptr(w), sd3.ptr(b), EPS, sd3.ptr(x), sd3.ptr(m), sd3.ptr(r),
+                                       rows, C, sd3.stream_ptr()), "sd3_layer_norm")
+    assert torch.equal(x, y) and torch.equal(m, mean) and torch.equal(r, rstd)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,C", [(40, 96), (700, 778), (300, 777), (2000, 1536), (6, 9001)])
+def test_one_row_for_all(sd3, rows, C, dtype):
+    x, w, b, dy = make(rows, C, dtype, seed=C)
+    check(sd3, x[:1].contiguous().expand(rows, C), w, b, dy)
+    check(sd3, x, w, b, dy[:1].contiguous().expand(rows, C))

@@ -106,3 +106,39 @@ def test_gradient_of_a_norm_in_a_chain(sd3):
     # fp32 throughout: a few hundred half steps of 2^-24 of the largest values
     for got, want in ((dx, X.grad), (dw, W.grad), (db, B.grad)):
         assert (got.double() - want).abs().max() <= 2e-5 * want.abs().max()
+
+
+def test_two_streams_at_once(sd3):
+    """Each operator in small and large sizes (clusters that share K, CTA pairs, two heads a CTA) in two streams that run at the same
+    time, in opposite orders: the same bits as alone."""
+    g = torch.Generator(device="cuda").manual_seed(11)
+
+    def normal(*shape, dtype=torch.bfloat16):
+        return torch.randn(*shape, device="cuda", generator=g).to(dtype)
+
+    calls = []
+    for M, N, K, out in ((1, 1536, 6144, torch.bfloat16), (64, 512, 1536, torch.float32), (300, 1001, 520, torch.float32),
+                         (2000, 1536, 768, torch.float32), (1500, 1000, 1024, torch.bfloat16), (40, 64, 4096, torch.float32)):
+        x, w, r = normal(M, K), normal(N, K), normal(M, N, dtype=out)
+        calls.append(lambda x=x, w=w, r=r: sd3.linear_residual(x, w, None, sd3.ACT_SILU, r))
+    for heads, kv, D, lengths in ((12, 12, 64, [77, 77]), (8, 2, 128, [1500]), (4, 4, 128, [3, 200, 64])):
+        q, k, v = normal(sum(lengths), heads, D), normal(sum(lengths), kv, D), normal(sum(lengths), kv, D)
+        o = torch.tensor([sum(lengths[:i]) for i in range(len(lengths) + 1)], device="cuda", dtype=torch.int32)
+        calls.append(lambda q=q, k=k, v=v, o=o: sd3.attention_packed(q, k, v, o, True))
+    for rows, C, dtype in ((5, 777, torch.float32), (1000, 1536, torch.float32), (1000, 777, torch.bfloat16), (400, 4098, torch.float32)):
+        x, dy, w = normal(rows, C, dtype=dtype), normal(rows, C, dtype=dtype), normal(C, dtype=torch.float32)
+        _, mean, rstd = sd3.layer_norm(x, w)
+        calls.append(lambda x=x, dy=dy, w=w, m=mean, r=rstd: torch.cat([t.flatten().float() for t in sd3.layer_norm_backward(dy, x, w, m, r)]))
+    want = [c() for c in calls]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream(), torch.cuda.Stream()], [[], []]
+    for _ in range(10):
+        for i in range(len(calls)):
+            for s, order in ((0, i), (1, len(calls) - 1 - i)):
+                with torch.cuda.stream(streams[s]):
+                    got[s].append((order, calls[order]()))
+    torch.cuda.synchronize()
+    sd3.assert_healthy()
+    for results in got:
+        for i, t in results:
+            assert torch.equal(t, want[i])
