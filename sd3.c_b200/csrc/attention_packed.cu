@@ -22,7 +22,8 @@
 //   32 x 200 tokens, 16 heads of 64               26;  one sequence of 128: 5.7
 //
 // Only key tiles that hold the diagonal or the end of the sequence are masked.  Keys behind the end are the next sequence's: their
-// scores become -inf, and their rows of V zeros, because 0 * inf is not 0.
+// scores become -inf, and their rows of V zeros, because 0 * inf is not 0.  The rows of V behind a causal query are other queries'
+// keys and stay: mend_row.
 #include <cuda.h>
 
 #include <mutex>
@@ -71,6 +72,8 @@ struct PackedArgs {
   int heads, group;
   long ldo;
   bf16* out;
+  const bf16 *q, *k, *v;  // what the tensor maps describe, for mend_row
+  long ldq, ldk, ldv;
   float scale_log2e;
   int causal;
   int* status;
@@ -173,6 +176,74 @@ __device__ __noinline__ void rescale_row(uint32_t o_tmem, float alpha) {
     tmem_st_32x32b_x16(o_tmem + 16 * part, o0);
   }
   tmem_wait_st();
+}
+
+__device__ __forceinline__ void unpack8(const uint4& u, float (&f)[8]) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    f[2 * i] = __uint_as_float(w[i] << 16);
+    f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+  }
+}
+
+__device__ __forceinline__ void sum_up(const uint32_t (&o)[32], float2& total) {
+#pragma unroll
+  for (int k = 0; k < 32; k += 2) total = __fadd2_rn(total, make_float2(__uint_as_float(o[k]), __uint_as_float(o[k + 1])));
+}
+
+// causal: a value of V that is not finite, in a row behind the query but in its last key tile, meets a P of 0 in the products, and 0
+// times it is NaN.  A query whose output has a NaN comes here, if its tile goes on to key `last`: where a later row of the tile
+// explains a column's NaN, the column is formed again from the keys that the query sees, one by one.  Rows behind it
+// and this loop are all that such a row of V costs; nobody else comes here.
+template <int D>
+__device__ __noinline__ void mend_row(const PackedArgs& a, int begin, int i, int last, int h, float m_used, float inv) {
+  const int g = h / a.group;
+  bf16* out = a.out + static_cast<long>(begin + i) * a.ldo + h * D;
+  const bf16* v0 = a.v + static_cast<long>(begin) * a.ldv + g * D;
+  const bf16* k0 = a.k + static_cast<long>(begin) * a.ldk + g * D;
+  const bf16* q = a.q + static_cast<long>(begin + i) * a.ldq + h * D;
+  float acc[D];
+  bool any = false;
+#pragma unroll 1
+  for (int d = 0; d < D; ++d) {
+    bool later = false;  // a product with 0 that is no number
+#pragma unroll 1
+    for (int j = i + 1; j < last && !later; ++j) {
+      const float v = __bfloat162float(v0[j * a.ldv + d]);
+      later = !(fabsf(v) <= 3.4e38f);
+    }
+    const float o = __bfloat162float(out[d]);
+    acc[d] = later && o != o ? 0.f : NAN;
+    any |= acc[d] == 0.f;
+  }
+#pragma unroll 1
+  for (int j = i; any && j >= 0; --j) {  // a NaN of a key that the query does see stays
+    float s = 0.f;
+#pragma unroll 1
+    for (int d = 0; d < D; d += 8) {
+      float x[8], y[8];
+      unpack8(*reinterpret_cast<const uint4*>(q + d), x);
+      unpack8(*reinterpret_cast<const uint4*>(k0 + j * a.ldk + d), y);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s = fmaf(x[e], y[e], s);
+    }
+    const float p = ex2_approx((s - m_used) * a.scale_log2e);
+    any = false;
+#pragma unroll 1
+    for (int d = 0; d < D; d += 8) {
+      float y[8];
+      unpack8(*reinterpret_cast<const uint4*>(v0 + j * a.ldv + d), y);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        acc[d + e] = fmaf(p, y[e], acc[d + e]);
+        any |= acc[d + e] == acc[d + e];
+      }
+    }
+  }
+#pragma unroll 1
+  for (int d = 0; d < D; ++d)
+    if (acc[d] == acc[d]) out[d] = __float2bfloat16_rn(acc[d] * inv);
 }
 
 // Which of the grid's tiles a CTA takes in its round `i`: rounds go through the tiles, long ones first, in alternating
@@ -490,6 +561,7 @@ attention_packed_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
       tc_fence_after_sync();
       const float inv = 1.0f / (l2.x + l2.y);
       uint4* to = reinterpret_cast<uint4*>(a.out + static_cast<long>(begin + q0 + row) * a.ldo + h * D);
+      float2 total = make_float2(0.f, 0.f);  // NaN where an output is
       auto store = [&](uint32_t (&o)[32], int part) {
         if (q0 + row < len) {
 #pragma unroll
@@ -502,6 +574,7 @@ attention_packed_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
             to[4 * part + k] = u;
           }
         }
+        sum_up(o, total);
       };
       tmem_ld_32x32b_x32(o_tmem, ra);
       tmem_ld_32x32b_x32(o_tmem + 32, rb);
@@ -519,6 +592,8 @@ attention_packed_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
         store(rc, 2);
         store(rd, 3);
       }
+      if (a.causal && !(total.x + total.y == total.x + total.y) && q0 + row < len)
+        mend_row<D>(a, begin, q0 + row, min(len, nkv * BN), h, m_used, inv);
     }
   }
 
@@ -855,6 +930,7 @@ attention_packed_heads_kernel(const __grid_constant__ CUtensorMap tmQ, const __g
         tc_fence_after_sync();
         const float inv = 1.0f / (l2.x + l2.y);
         uint4* to = reinterpret_cast<uint4*>(a.out + static_cast<long>(begin + q0 + row) * a.ldo + h * HP_D);
+        float2 total = make_float2(0.f, 0.f);  // NaN where an output is
         auto store = [&](uint32_t (&o)[32], int part) {
           if (q0 + row < len) {
 #pragma unroll
@@ -867,6 +943,7 @@ attention_packed_heads_kernel(const __grid_constant__ CUtensorMap tmQ, const __g
               to[4 * part + k] = v;
             }
           }
+          sum_up(o, total);
         };
         tmem_ld_32x32b_x32(o_tmem, r0);
         tmem_ld_32x32b_x32(o_tmem + 32, r1);
@@ -880,6 +957,8 @@ attention_packed_heads_kernel(const __grid_constant__ CUtensorMap tmQ, const __g
         store(r1, 1);
         store(r2, 2);
         store(r3, 3);
+        if (a.causal && !(total.x + total.y == total.x + total.y) && q0 + row < len)
+          mend_row<HP_D>(a, begin, q0 + row, min(len, nkv * HP_BN), h, m_used, inv);
       }
     }
   }
@@ -970,6 +1049,8 @@ int launch_attention_packed(const PackedAttention& p, int* dev_status, cudaStrea
   a.group = p.heads / p.kv_heads;
   a.ldo = p.ldo;
   a.out = p.out;
+  a.q = p.q; a.k = p.k; a.v = p.v;
+  a.ldq = p.ldq; a.ldk = p.ldk; a.ldv = p.ldv;
   a.scale_log2e = p.scale * 1.4426950408889634f;
   a.causal = p.causal;
   a.status = dev_status;

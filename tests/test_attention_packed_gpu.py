@@ -164,6 +164,28 @@ def test_later_keys_reach_nothing(sd3):
         assert torch.equal(sd3.attention_packed(q, k, v, offsets_of([300]), True)[:150], first[:150])
 
 
+@pytest.mark.parametrize("whole", [False, True])
+@pytest.mark.parametrize("at", [0, 1, 63, 64, 127, 128, 200, 298])
+@pytest.mark.parametrize("heads,kv_heads,D,extra", [(2, 1, 64, 0), (3, 3, 128, 0), (4, 2, 128, 3000)])
+def test_values_of_later_keys_that_are_no_numbers(sd3, heads, kv_heads, D, extra, at, whole):
+    lengths = [90, 300]  # extra: rows enough for two heads a CTA
+    q, k, v = (t.contiguous() for t in make(390 + extra, heads, kv_heads, D, seed=at))
+    want, size, scores = oracle(q, k, v, lengths, True, D ** -0.5)
+    bad = v.clone()
+    bad[90 + at, :, 3:(D if whole else 4)] = float("nan")
+    bad[90 + at + 1, :, 1] = float("-inf")
+    got = sd3.attention_packed(q, k, bad, offsets_of(lengths), True)[:390].double()
+    torch.cuda.synchronize()
+    sd3.assert_healthy()
+    nan, inf = torch.zeros_like(got, dtype=torch.bool), torch.zeros_like(got, dtype=torch.bool)
+    nan[90 + at:, :, 3:(D if whole else 4)] = True
+    inf[90 + at + 1:, :, 1] = True
+    assert torch.isnan(got[nan]).all() and (got[inf] == float("-inf")).all()
+    ok = ~(nan | inf)
+    off = (got - want[:390]).abs() - (2.0 ** -8 + 8.5e-4 + scores) * size[:390] - 2.0 ** -8 * want[:390].abs()
+    assert torch.isfinite(got[ok]).all() and (off[ok] <= 0).all()
+
+
 def test_separate_tensors_and_strides(sd3):
     q, k, v = (t.contiguous() for t in make(200, 4, 2, 64, seed=7))
     want = sd3.attention_packed(q, k, v, offsets_of([200]), True)
