@@ -130,9 +130,11 @@ __device__ Unit find_unit(const PackedArgs& a, int rank) {
     }
 #pragma unroll
     for (int i = 0; i < AP_SCAN_CHUNKS; ++i) {
-      const unsigned has = __ballot_sync(0xffffffffu, a.causal ? n[i] > lo : n[i] == lo + 1);
+      const bool mine = a.causal ? n[i] > lo : n[i] == lo + 1;
+      const unsigned has = __ballot_sync(0xffffffffu, mine);
       if (r < __popc(has)) {
-        Unit u = sequence_at(a, 32 * i + static_cast<int>(__fns(has, 0, r + 1)));
+        const unsigned at = __ballot_sync(0xffffffffu, mine && __popc(has & ((1u << lane) - 1)) == r);  // the one with r before it
+        Unit u = sequence_at(a, 32 * i + __ffs(at) - 1);
         u.q0 = place * AP_BM;
         return u;
       }
@@ -248,9 +250,9 @@ __device__ __noinline__ void mend_row(const PackedArgs& a, int begin, int i, int
 
 // Which of the grid's tiles a CTA takes in its round `i`: rounds go through the tiles, long ones first, in alternating
 // directions, so that a CTA that gets the longest of one round gets the shortest of the next.
-__device__ __forceinline__ long tile_of_round(int i) {
-  const long g = gridDim.x;
-  return i * g + ((i & 1) ? g - 1 - blockIdx.x : blockIdx.x);
+__device__ __forceinline__ unsigned tile_of_round(int i) {
+  const long g = gridDim.x, w = i * g + ((i & 1) ? g - 1 - blockIdx.x : blockIdx.x);
+  return static_cast<unsigned>(min(w, 0x7fffffffL));  // there are fewer; divisions of 64 bits cost every round 200 cycles
 }
 
 template <int D>
@@ -319,10 +321,9 @@ attention_packed_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
   Unit u;  // warp 0: the query tile of the coming round, and its head
   int h = 0;
   auto find = [&](int i) {
-    const long w = tile_of_round(i);
-    const long rank = w / a.heads;
+    const unsigned w = tile_of_round(i), rank = w / static_cast<unsigned>(a.heads);
     h = static_cast<int>(w - rank * a.heads);
-    u = find_unit(a, rank < (1L << 30) ? static_cast<int>(rank) : (1 << 30));
+    u = find_unit(a, static_cast<int>(min(rank, 1u << 30)));
   };
   auto write_unit = [&](int i) {
     int* to = s_unit + 4 * (i & 1);
@@ -687,10 +688,9 @@ attention_packed_heads_kernel(const __grid_constant__ CUtensorMap tmQ, const __g
   Unit u;  // warp 0: the query tile of the coming round, and its first head
   int h0 = 0;
   auto find = [&](int i) {
-    const long w = tile_of_round(i);
-    const long rank = w / pairs;
+    const unsigned w = tile_of_round(i), rank = w / static_cast<unsigned>(pairs);
     h0 = 2 * static_cast<int>(w - rank * pairs);
-    u = find_unit(a, rank < (1L << 30) ? static_cast<int>(rank) : (1 << 30));
+    u = find_unit(a, static_cast<int>(min(rank, 1u << 30)));
   };
   auto write_unit = [&](int i) {
     int* to = s_unit + 4 * (i & 1);
